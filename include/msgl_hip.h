@@ -390,6 +390,106 @@ int msgl_prepare_decode_paged(const int32_t* req_pool_indices, int32_t* seq_lens
                               int32_t* status, int bs, int page_size, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * Speculative decoding with a drafted token tree.  A step verifies, per request, the last
+ * accepted token (node 0, the root, whose K/V is not in the cache yet) and the drafted
+ * tokens that hang off it: msgl_prepare_extend lays the step out, the model runs over all
+ * nodes at once with msgl_tree_attention in place of the decode attention, and
+ * msgl_accept_tree keeps the nodes the model confirms.  The reference has no counterpart (it
+ * decodes one token per request and step, mini_sglang/managers/scheduler.py:409-419).
+ * Trees: `parents`, packed per request behind cu_seqlens_q, holds indices inside the request;
+ * a parent is an earlier node, any other value (a drafter's -1) means the root.
+ * ------------------------------------------------------------------------- */
+#define MSGL_TREE_MAX_WORDS 16 /* mask words of 64 nodes: up to 1024 nodes per request */
+
+/* Slots, positions and page-table entries of an extend step, from the lengths alone: what
+ * BatchInfo.prepare_for_extend (mini_sglang/managers/batch_info.py:135-245) does on the host,
+ * with the allocator's page order (PageAllocator.alloc, mini_sglang/mem_cache/token2kv.py:186-196).
+ * Request b has L = prefix_lens[b] cached tokens, n = new_lens[b] new ones (0 is fine) and table
+ * entries for its first A = alloc_lens[b] >= L positions; A runs ahead of L when a step before
+ * had some of its drafts rejected.  Position p of L .. L+n-1 keeps its entry below A, continues
+ * the run of a partly backed page up to that page's end, and beyond takes pages from
+ * free_pages[free_range[0] ..], in batch order.
+ *   positions[t] = L + i (trees: L + depth of node i), out_cache_loc[t] = slot of position L + i,
+ *   for t = cu_seqlens_q[b] + i;  cu_seqlens_q = prefix sums of new_lens;  seq_lens[b] = L + n;
+ *   tree_mask[t][.]: bit j set iff j is node i or one of its ancestors (parents given);
+ *   alloc_out[b] = max(A, L + n);  free_range_out[0] = free_range[0] + pages taken.
+ * positions / out_cache_loc / tree_mask have `capacity` rows; rows behind the last token are set
+ * to position 0, the dummy slot 0 and an empty mask, so that a captured step of fixed size writes
+ * nothing that belongs to a request.  alloc_out may be alloc_lens and free_range_out may be
+ * free_range (in place); no other output may be an input.
+ * All or nothing: *status (left as it is on success, sticky like msgl_prepare_decode's) becomes
+ * 1 (free list exhausted), 2 (a request outgrows its table row of max_ctx entries), 3 (a negative
+ * length, alloc_lens outside prefix_lens .. max_ctx, a table row outside 0 .. table_rows - 1) or
+ * 4 (more tokens than `capacity`, more nodes than the mask has bits); then cu_seqlens_q is all 0,
+ * every row is a row behind the last token, and lengths, table and free range stay as they were.
+ * req_to_page (NULL = none) gets the page ids of pages taken.  parents and tree_mask: both or
+ * neither.  workspace: msgl_prepare_extend_workspace_bytes(bs) bytes, 16-byte aligned. */
+size_t msgl_prepare_extend_workspace_bytes(int bs);
+int msgl_prepare_extend(const int32_t* req_pool_indices, const int32_t* prefix_lens, const int32_t* new_lens, const int32_t* alloc_lens,
+                        const int32_t* free_pages, int32_t free_capacity, const int32_t* free_range, int32_t* req_to_token,
+                        int64_t r2t_stride, int32_t table_rows, int32_t max_ctx, int32_t* req_to_page, int64_t r2p_stride,
+                        const int32_t* parents, uint64_t* tree_mask, int mask_words, int32_t* positions, int32_t* out_cache_loc,
+                        int32_t capacity, int32_t* cu_seqlens_q, int32_t* seq_lens, int32_t* alloc_out, int32_t* free_range_out,
+                        int32_t* status, int bs, int page_size, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Attention of the tree's nodes over the paged cache:
+ *   out[t, h] = softmax(scale * q[t, h] . K) . V   over the keys node t sees: positions
+ *   [0, prefix_lens[b]) of req_to_token[req_pool_indices[b]], and prefix_lens[b] + j for the set bits
+ *   j of tree_mask[t] (the node itself is not implied).  A node that sees nothing gets zeros, and
+ *   the K/V of nodes it does not see never reach it, NaN and infinity included.
+ * q, out: [total_tokens, Hq, D] bf16, strides per token in elements; request b's nodes are rows
+ * cu_seqlens_q[b] .. cu_seqlens_q[b+1] - 1, rows behind the last request are left as they are.  Their K/V must
+ * be in the pool already.  Any page size: the table is read per token.
+ * tree_mask: [total_tokens, mask_words] 64-bit words, dense.
+ * max_seqlen_q: upper bound on the nodes per request, at most 64 * mask_words (nodes beyond it are not
+ * computed); max_seqlen_k: upper bound on prefix + nodes and total_kv (0 = unknown) the sum of prefix + nodes
+ * over the batch: both steer the cut of long contexts only, results hold for any values.
+ * workspace: msgl_tree_attention_workspace_bytes(total_tokens, Hq, D, splits) bytes, 16-byte aligned, for
+ * splits = msgl_tree_attention_splits(...) of the same bounds; a smaller one (NULL) is legal, long contexts are
+ * then cut less.  Different cuts agree to fp32 rounding of the sums; one cut always gives the same bits.
+ * Supported: D == 128; Hq/Hkv in {1, 2, 4, 8}; Hkv in {1, 2, 4, 8}; 0 <= scale. */
+int msgl_tree_attention_splits(int bs, int max_seqlen_q, int max_seqlen_k, int64_t total_kv, int Hq, int Hkv);
+size_t msgl_tree_attention_workspace_bytes(int64_t total_tokens, int Hq, int D, int splits);
+int msgl_tree_attention(const void* q, int64_t q_stride, const void* k_cache, const void* v_cache, int64_t cache_stride,
+                        const int32_t* req_to_token, int64_t r2t_stride, const int32_t* req_pool_indices, const int32_t* cu_seqlens_q,
+                        const int32_t* prefix_lens, const uint64_t* tree_mask, int mask_words, void* out, int64_t out_stride,
+                        int64_t total_tokens, int bs, int max_seqlen_q, int max_seqlen_k, int64_t total_kv, int Hq, int Hkv, int D, float scale,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+/* Greedy acceptance and what follows from it.  From the root on, the accepted path goes to the first (lowest) node
+ * that hangs off the current one and whose draft_tokens entry is target_tokens[current], the model's
+ * token after the current node (msgl_argmax of its logits), and ends where there is none or after max_accept nodes.
+ *   accept_lens[b] = nodes on the path (at least 1; 0 for a request without nodes);
+ *   accept_rows[b, i] = row (in the packed arrays) of the i-th node, accept_tokens[b, i] = target_tokens of that row, i.e. the
+ *   i-th token generated; -1 behind the path ([bs, max_accept] both, dense);
+ *   next_tokens[b] = the last of these (the next step's root; left as it is for a request without nodes);
+ *   seq_lens[b] = prefix_lens[b] + accept_lens[b]  (seq_lens may be prefix_lens);
+ *   and in every layer the K and V rows of the i-th node move to the slot of position prefix_lens[b] + i, which is
+ *   out_cache_loc[cu_seqlens_q[b] + i].
+ * kv_layers: device array [num_layers][2] of the K and V cache addresses ([slots, Hkv, D] bf16, slot stride cache_stride
+ * elements in every layer); num_layers = 0 moves nothing. */
+int msgl_accept_tree(const int32_t* draft_tokens, const int32_t* target_tokens, const int32_t* parents, const int32_t* cu_seqlens_q,
+                     const int32_t* prefix_lens, const int32_t* out_cache_loc, const uint64_t* kv_layers, int num_layers,
+                     int64_t cache_stride, int Hkv, int D, int32_t* accept_lens, int32_t* accept_rows, int32_t* accept_tokens,
+                     int32_t* next_tokens, int32_t* seq_lens, int bs, int max_accept, void* stream);
+
+/* Log probabilities: for every row of logits [rows, vocab] (bf16 or fp32: elem_bytes 2 or 4, any row stride and alignment)
+ *   logprobs[r] = log softmax(logits[r])[token_ids[r]]   (NaN for an id outside [0, vocab)),
+ *   entropy[r]  = -sum p log p  in nats (a token at -inf adds 0),
+ *   top_ids / top_logprobs [rows, top]: the `top` most probable tokens in falling order, ties to the lower id, NaN above
+ *   everything, as msgl_argmax orders.
+ * A row with a NaN or +inf in it, or with nothing above -inf, has NaN log probabilities and entropy, as torch's log_softmax.
+ * Next to the sampled token's choice (mini_sglang/layers/sampler.py:13-23) this is what a caller that reports log
+ * probabilities needs; sums in fp32, one read of the logits.
+ * 0 <= top <= min(vocab, MSGL_LOGPROBS_MAX_TOP), vocab <= 2^30.  workspace: msgl_token_logprobs_workspace_bytes bytes, 16-byte
+ * aligned. */
+#define MSGL_LOGPROBS_MAX_TOP 32
+size_t msgl_token_logprobs_workspace_bytes(int rows, int vocab, int elem_bytes, int top);
+int msgl_token_logprobs(const void* logits, int64_t row_stride, int elem_bytes, const int32_t* token_ids, float* logprobs,
+                        float* entropy, int32_t* top_ids, float* top_logprobs, int rows, int vocab, int top, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
  * Measurement utility (no counterpart in the reference): reads `bytes` bytes at src
  * once, 16 bytes per lane with the non-temporal hint, and stores nothing (sink: 256
  * bytes of device memory that are practically never written).  bench.py times it as

@@ -13,7 +13,7 @@ from ctypes import c_char_p, c_float, c_int, c_int64, c_size_t, c_void_p
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("MSGL_HIP_LIB", os.path.join(_HERE, "libmsgl_hip.so"))
 
-ABI_VERSION = 17
+ABI_VERSION = 18
 
 # name -> (restype, argtypes); mirrors include/msgl_hip.h and include/msgl_comm.h one to one
 SIGNATURES = {
@@ -79,6 +79,30 @@ SIGNATURES = {
         c_int,
         [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p, c_void_p,
          c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p],
+    ),
+    "msgl_prepare_extend_workspace_bytes": (c_size_t, [c_int]),
+    "msgl_prepare_extend": (
+        c_int,
+        [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p, c_int64,
+         c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
+         c_void_p, c_size_t, c_void_p],
+    ),
+    "msgl_tree_attention_splits": (c_int, [c_int, c_int, c_int, c_int64, c_int, c_int]),
+    "msgl_tree_attention_workspace_bytes": (c_size_t, [c_int64, c_int, c_int, c_int]),
+    "msgl_tree_attention": (
+        c_int,
+        [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
+         c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_int64, c_int, c_int, c_int, c_float, c_void_p, c_size_t, c_void_p],
+    ),
+    "msgl_accept_tree": (
+        c_int,
+        [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int, c_int, c_void_p, c_void_p,
+         c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p],
+    ),
+    "msgl_token_logprobs_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "msgl_token_logprobs": (
+        c_int,
+        [c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_size_t, c_void_p],
     ),
     "msgl_stream_read": (c_int, [c_void_p, c_size_t, c_void_p, c_void_p]),
     "msgl_stream_read_cfg": (c_int, [c_void_p, c_size_t, c_void_p, c_int, c_int, c_void_p]),

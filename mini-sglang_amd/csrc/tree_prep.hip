@@ -1,0 +1,371 @@
+// The two ends of a speculative step, on the device.
+//
+// msgl_prepare_extend: from the cached lengths and the number of new tokens of every request to their positions, pool slots and
+// page-table entries, and (for drafted trees) the mask of ancestors of every node.  What BatchInfo.prepare_for_extend does on the
+// host (mini_sglang/managers/batch_info.py:135-245) with the page allocator's take-from-the-front order
+// (mini_sglang/mem_cache/token2kv.py:186-196), for requests whose length is anything, page aligned or not, and whose table row may
+// already be backed further than the length (slots left over from rejected drafts).
+//
+// msgl_accept_tree: the walk from a tree's root along the nodes the model confirms, and the move of those nodes' cache rows to
+// consecutive positions in every layer.
+#include "msgl_common.h"
+
+namespace msgl {
+
+struct ExtendPrepParams {
+    const int32_t* req_idx;
+    const int32_t* prefix;    // [bs] cached tokens
+    const int32_t* new_lens;  // [bs] tokens this step adds
+    const int32_t* alloc;     // [bs] positions that have a table entry
+    const int32_t* free_pages;
+    int32_t free_capacity;
+    const int32_t* free_range;
+    int32_t* r2t;
+    int64_t r2t_stride;
+    int32_t* r2p;
+    int64_t r2p_stride;
+    int32_t table_rows, max_ctx;
+    const int32_t* parents;  // optional [capacity]: tree of every request, indices inside the request
+    int32_t* positions;      // [capacity]
+    int32_t* out_loc;        // [capacity]
+    int32_t* cu;             // [bs + 1]
+    int32_t* seq_lens;       // [bs]
+    uint64_t* mask;          // [capacity, words]
+    int32_t* alloc_out;
+    int32_t* free_range_out;
+    int32_t* status;
+    int4* scratch;  // [bs]: prefix, alloc, page of the first page boundary at or behind alloc minus that boundary's page index, row
+    int32_t capacity, words;
+    int bs, ps;
+};
+
+constexpr int kScanThreads = 1024;
+
+// Exclusive prefix sums of two counts over the work group, and their totals.  Every thread calls it.
+__device__ __forceinline__ void block_scan2(int64_t a, int64_t b, int64_t (*lds)[2], int64_t& a_before, int64_t& b_before, int64_t& a_total, int64_t& b_total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int64_t x = a, y = b;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int64_t u = __shfl_up(x, d), v = __shfl_up(y, d);
+        if (lane >= d) x += u, y += v;
+    }
+    __syncthreads();  // lds may still be read from the previous call
+    if (lane == 63) lds[wave][0] = x, lds[wave][1] = y;
+    __syncthreads();
+    int64_t xb = 0, yb = 0, xt = 0, yt = 0;
+#pragma unroll
+    for (int w = 0; w < kScanThreads / 64; ++w) {
+        const int64_t u = lds[w][0], v = lds[w][1];
+        if (w < wave) xb += u, yb += v;
+        xt += u, yt += v;
+    }
+    a_before = xb + x - a, b_before = yb + y - b, a_total = xt, b_total = yt;
+}
+
+// Positions and page-table entry of one new token: its slot.
+__device__ __forceinline__ int32_t place_token(const ExtendPrepParams& p, const int4 rq, int pos) {
+    const int alloc = rq.y, ps = p.ps;
+    int32_t* row = p.r2t + (int64_t)rq.w * p.r2t_stride;
+    if (pos < alloc) return row[pos];
+    int32_t slot;
+    if (pos < (alloc + ps - 1) / ps * ps) {
+        slot = row[alloc - 1] + (pos - alloc + 1);  // the rest of a page that is partly backed
+    } else {
+        slot = p.free_pages[rq.z + pos / ps] * ps + pos % ps;
+        if (p.r2p && ps > 1 && pos % ps == 0) p.r2p[(int64_t)rq.w * p.r2p_stride + pos / ps] = slot / ps;
+    }
+    row[pos] = slot;
+    return slot;
+}
+
+// Phase 1, one work group: totals, refusal, prefix sums, the state's update.
+__global__ __launch_bounds__(kScanThreads) void extend_prepare_scan_kernel(ExtendPrepParams p) {
+    __shared__ int64_t lds[kScanThreads / 64][2];
+    const int tid = threadIdx.x;
+    const int head = p.free_range[0];
+    const int end = min(p.free_range[1], p.free_capacity);
+    const int earlier = *p.status;
+    int64_t tokens = 0, pages = 0;
+    bool too_long = false, bad = false, too_wide = false;
+    for (int c0 = 0; c0 < p.bs; c0 += kScanThreads) {
+        const int i = c0 + tid;
+        int L = 0, n = 0, A = 0, row = 0;
+        if (i < p.bs) L = p.prefix[i], n = p.new_lens[i], A = p.alloc[i], row = p.req_idx[i];
+        const bool wrong = L < 0 || n < 0 || A < L || A > p.max_ctx || row < 0 || row >= p.table_rows;
+        const bool longer = !wrong && (int64_t)L + n > p.max_ctx;
+        bad |= wrong, too_long |= longer, too_wide |= p.words && n > p.words * 64;
+        if (wrong || longer) n = 0, L = 0, A = 0, row = 0;
+        const int have = (A + p.ps - 1) / p.ps;
+        const int need = max(0, (L + n + p.ps - 1) / p.ps - have);
+        int64_t t0, g0, tt, gt;
+        block_scan2(n, need, lds, t0, g0, tt, gt);
+        if (i < p.bs) {
+            p.cu[i] = (int32_t)(tokens + t0);
+            p.seq_lens[i] = L + n;
+            p.scratch[i] = make_int4(L, A, (int32_t)(head + pages + g0 - have), row);
+        }
+        tokens += tt, pages += gt;
+    }
+    const bool any_bad = __syncthreads_or(bad), any_long = __syncthreads_or(too_long), any_wide = __syncthreads_or(too_wide);
+    int refuse = earlier;
+    if (!refuse) refuse = any_bad ? 3 : any_long ? 2 : (any_wide || tokens > p.capacity) ? 4 : (head < 0 || pages > (int64_t)end - head) ? 1 : 0;
+    if (refuse) {  // no token at all: every cu entry 0, lengths, table and free list as they were
+        for (int i = tid; i < p.bs; i += kScanThreads) {
+            p.cu[i] = 0;
+            p.seq_lens[i] = p.prefix[i];
+            if (p.alloc_out != p.alloc) p.alloc_out[i] = p.alloc[i];
+        }
+        __syncthreads();  // every thread has read the status word and the free range
+        if (tid == 0) {
+            p.cu[p.bs] = 0;
+            *p.status = refuse;
+            if (p.free_range_out != p.free_range) p.free_range_out[0] = head, p.free_range_out[1] = p.free_range[1];
+        }
+        return;
+    }
+    for (int i = tid; i < p.bs; i += kScanThreads) p.alloc_out[i] = max(p.alloc[i], p.prefix[i] + p.new_lens[i]);
+    const int32_t valid_end = p.free_range[1];
+    __syncthreads();
+    if (tid == 0) {
+        p.cu[p.bs] = (int32_t)tokens;
+        p.free_range_out[0] = head + (int32_t)pages;
+        p.free_range_out[1] = valid_end;
+    }
+}
+
+// Phase 2, plain runs of tokens: one thread per entry of the output arrays.
+__global__ __launch_bounds__(256) void extend_prepare_fill_kernel(ExtendPrepParams p) {
+    const int t = blockIdx.x * 256 + threadIdx.x;
+    if (t >= p.capacity) return;
+    if (t >= p.cu[p.bs]) {  // behind the last request: the dummy slot
+        p.positions[t] = 0;
+        p.out_loc[t] = 0;
+        return;
+    }
+    int lo = 0, hi = p.bs - 1;  // last request that starts at or before t and is not empty
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (p.cu[mid] <= t) lo = mid;
+        else hi = mid - 1;
+    }
+    const int4 rq = p.scratch[lo];
+    const int pos = rq.x + t - p.cu[lo];
+    p.positions[t] = pos;
+    p.out_loc[t] = place_token(p, rq, pos);
+}
+
+// Phase 2, trees: a wave per request; nodes in chunks of 64, a node per lane.  Inside a chunk the ancestors are collected by pointer
+// doubling (a lane's pointer jumps to its pointer's pointer, collecting the nodes jumped over), so a chunk costs log2(depth) steps;
+// what lies in earlier chunks is the finished mask row of the first ancestor there.
+__global__ __launch_bounds__(256) void extend_prepare_tree_kernel(ExtendPrepParams p) {
+    const int lane = threadIdx.x & 63;
+    const int b = blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int total = p.cu[p.bs];
+    for (int t = total + (blockIdx.x * 256 + threadIdx.x); t < p.capacity; t += gridDim.x * 256) {  // behind the last request
+        p.positions[t] = 0;
+        p.out_loc[t] = 0;
+        for (int w = 0; w < p.words; ++w) p.mask[(int64_t)t * p.words + w] = 0;
+    }
+    if (b >= p.bs) return;
+    const int base = p.cu[b];
+    const int n = min(p.cu[b + 1] - base, p.words * 64);
+    const int4 rq = p.scratch[b];
+    for (int c = 0; c * 64 < n; ++c) {
+        const int node = c * 64 + lane;
+        const bool live = node < n;
+        int par = live ? p.parents[base + node] : 0;
+        if (par < 0 || par >= node) par = 0;  // anything but an earlier node hangs off the root
+        const bool local = live && node > 0 && par >= c * 64;
+        int ptr = local ? par - c * 64 : lane;
+        const int outer = (live && node > 0 && !local) ? par : -1;
+        uint64_t m = local ? 1ull << lane : 0;
+        while (__any(__shfl(ptr, ptr) != ptr)) {
+            m |= __shfl(m, ptr);
+            ptr = __shfl(ptr, ptr);
+        }
+        m |= (1ull << ptr) | (1ull << lane);
+        const int up = __shfl(outer, ptr);
+        int depth = __popcll(m) - 1;
+        if (live) {
+            uint64_t* row = p.mask + (int64_t)(base + node) * p.words;
+            for (int w = 0; w < p.words; ++w) {
+                uint64_t v = w == c ? m : 0;
+                if (w < c && up >= 0) v = p.mask[(int64_t)(base + up) * p.words + w], depth += __popcll(v);
+                row[w] = v;
+            }
+            const int pos = rq.x + node;
+            p.positions[base + node] = rq.x + depth;
+            p.out_loc[base + node] = place_token(p, rq, pos);
+        }
+        __threadfence_block();  // the next chunk reads these mask rows from other lanes of this wave
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------ acceptance
+struct AcceptParams {
+    const int32_t* draft;
+    const int32_t* target;
+    const int32_t* parents;
+    const int32_t* cu;
+    const int32_t* prefix;
+    const int32_t* loc;
+    const uint64_t* layers;  // [layers][2]: addresses of the K and the V cache
+    int64_t slot_bytes;
+    int32_t row_chunks;  // 16-byte chunks of one layer's K (or V) row
+    int32_t* lens;
+    int32_t* rows;
+    int32_t* tokens;
+    int32_t* next;
+    int32_t* seq_lens;
+    int bs, num_layers, most, layers_per_group;
+};
+
+constexpr int kMoveBatch = 8;
+
+// Work group = one request and a run of layers.  Every wave walks the tree by itself (no exchange needed): a node's child is the first
+// later node that hangs off it and drafted the token the model put after it.  Path indices rise, and row i of the path goes to node
+// i's slot with i <= path[i]; the source of a later row is therefore never an earlier row's destination, and a thread that carries
+// the same 16 bytes of every row may load a batch of rows before it stores them.
+__global__ __launch_bounds__(256) void accept_tree_kernel(AcceptParams p) {
+    __shared__ int32_t path_lds[4][1024];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int b = blockIdx.x;
+    const int base = p.cu[b];
+    const int n = p.cu[b + 1] - base;
+    const bool writer = blockIdx.y == 0 && wave == 0;
+    int32_t* path = path_lds[wave];
+    int len = 0;
+    if (n > 0) {
+        int par0 = lane < n ? p.parents[base + lane] : -1;
+        const int tok0 = lane < n ? p.draft[base + lane] : 0;
+        const int tgt0 = lane < n ? p.target[base + lane] : 0;
+        if (lane < n && (par0 < 0 || par0 >= lane)) par0 = 0;
+        int cur = 0;
+        while (true) {
+            const int want = cur < 64 ? __shfl(tgt0, cur) : p.target[base + cur];
+            if (lane == 0) path[len] = cur;
+            if (writer && lane == 0) p.rows[(int64_t)b * p.most + len] = base + cur, p.tokens[(int64_t)b * p.most + len] = want;
+            ++len;
+            if (writer && lane == 0) p.next[b] = want;
+            if (len == p.most) break;
+            int child = -1;
+            if (cur < 63) {
+                const uint64_t hit = __ballot(lane < n && lane > cur && par0 == cur && tok0 == want);
+                if (hit) child = __ffsll((unsigned long long)hit) - 1;
+            }
+            for (int c = max(64, (cur + 1) & ~63); child < 0 && c < n; c += 64) {
+                const int node = c + lane;
+                bool is = false;
+                if (node < n && node > cur) {
+                    int par = p.parents[base + node];
+                    if (par < 0 || par >= node) par = 0;
+                    is = par == cur && p.draft[base + node] == want;
+                }
+                const uint64_t hit = __ballot(is);
+                if (hit) child = c + __ffsll((unsigned long long)hit) - 1;
+            }
+            if (child < 0) break;
+            cur = child;
+        }
+    }
+    if (writer) {
+        for (int i = len + lane; i < p.most; i += 64) p.rows[(int64_t)b * p.most + i] = -1, p.tokens[(int64_t)b * p.most + i] = -1;
+        if (lane == 0) {
+            p.lens[b] = len;
+            p.seq_lens[b] = p.prefix[b] + len;
+        }
+    }
+    __builtin_amdgcn_wave_barrier();
+    __threadfence_block();
+    const int l0 = blockIdx.y * p.layers_per_group, layers = min(p.num_layers - l0, p.layers_per_group);
+    for (int e = threadIdx.x; e < layers * 2 * p.row_chunks; e += 256) {  // K chunks, then V chunks, layer after layer
+        const int half = e / p.row_chunks;
+        char* cache = reinterpret_cast<char*>(p.layers[2 * l0 + half]) + (int64_t)(e - half * p.row_chunks) * 16;
+        for (int i0 = 1; i0 < len; i0 += kMoveBatch) {
+            uint4 v[kMoveBatch];
+            const int count = min(kMoveBatch, len - i0);
+#pragma unroll
+            for (int j = 0; j < kMoveBatch; ++j) v[j] = *reinterpret_cast<const uint4*>(cache + p.loc[base + path[i0 + min(j, count - 1)]] * p.slot_bytes);
+#pragma unroll
+            for (int j = 0; j < kMoveBatch; ++j)
+                if (j < count) *reinterpret_cast<uint4*>(cache + p.loc[base + i0 + j] * p.slot_bytes) = v[j];
+        }
+    }
+}
+
+}  // namespace msgl
+
+using namespace msgl;
+
+extern "C" size_t msgl_prepare_extend_workspace_bytes(int bs) { return bs > 0 ? (size_t)bs * sizeof(int4) : 0; }
+
+extern "C" int msgl_prepare_extend(const int32_t* req_pool_indices, const int32_t* prefix_lens, const int32_t* new_lens, const int32_t* alloc_lens,
+                                   const int32_t* free_pages, int32_t free_capacity, const int32_t* free_range, int32_t* req_to_token,
+                                   int64_t r2t_stride, int32_t table_rows, int32_t max_ctx, int32_t* req_to_page, int64_t r2p_stride,
+                                   const int32_t* parents, uint64_t* tree_mask, int mask_words, int32_t* positions, int32_t* out_cache_loc,
+                                   int32_t capacity, int32_t* cu_seqlens_q, int32_t* seq_lens, int32_t* alloc_out, int32_t* free_range_out,
+                                   int32_t* status, int bs, int page_size, void* workspace, size_t workspace_bytes, void* stream) {
+    MSGL_REQUIRE(bs >= 0 && page_size > 0 && free_capacity >= 0 && max_ctx > 0 && table_rows > 0 && capacity >= 0,
+                 "msgl_prepare_extend: bs=%d page_size=%d free_capacity=%d max_ctx=%d table_rows=%d capacity=%d", bs, page_size, free_capacity, max_ctx,
+                 table_rows, capacity);
+    if (bs == 0) return MSGL_OK;
+    MSGL_REQUIRE(max_ctx <= 0x7fffffff - page_size, "msgl_prepare_extend: max_ctx %d + page_size %d leaves 32 bits", max_ctx, page_size);
+    MSGL_REQUIRE(req_pool_indices && prefix_lens && new_lens && alloc_lens && free_pages && free_range && req_to_token && cu_seqlens_q && seq_lens &&
+                     alloc_out && free_range_out && status && (capacity == 0 || (positions && out_cache_loc)),
+                 "msgl_prepare_extend: null pointer argument");
+    MSGL_REQUIRE((parents == nullptr) == (tree_mask == nullptr), "msgl_prepare_extend: parents and tree_mask go together");
+    MSGL_REQUIRE(parents == nullptr || (mask_words >= 1 && mask_words <= MSGL_TREE_MAX_WORDS), "msgl_prepare_extend: mask_words %d outside 1..%d",
+                 mask_words, MSGL_TREE_MAX_WORDS);
+    MSGL_REQUIRE(r2t_stride >= max_ctx, "msgl_prepare_extend: r2t_stride %lld < max_ctx %d", (long long)r2t_stride, max_ctx);
+    MSGL_REQUIRE(req_to_page == nullptr || r2p_stride >= (max_ctx + page_size - 1) / page_size, "msgl_prepare_extend: r2p_stride %lld < pages of a row",
+                 (long long)r2p_stride);
+    MSGL_REQUIRE(seq_lens != prefix_lens && seq_lens != new_lens && seq_lens != alloc_lens && alloc_out != prefix_lens && alloc_out != new_lens,
+                 "msgl_prepare_extend: an output overwrites an input (only alloc_out may be alloc_lens, free_range_out free_range)");
+    if (workspace_bytes < msgl_prepare_extend_workspace_bytes(bs) || workspace == nullptr) {
+        set_error("msgl_prepare_extend: workspace %zu < %zu bytes", workspace_bytes, msgl_prepare_extend_workspace_bytes(bs));
+        return MSGL_E_WORKSPACE;
+    }
+    MSGL_REQUIRE(aligned16(workspace), "msgl_prepare_extend: workspace must be 16-byte aligned");
+    ExtendPrepParams p;
+    p.req_idx = req_pool_indices, p.prefix = prefix_lens, p.new_lens = new_lens, p.alloc = alloc_lens;
+    p.free_pages = free_pages, p.free_capacity = free_capacity, p.free_range = free_range;
+    p.r2t = req_to_token, p.r2t_stride = r2t_stride, p.r2p = req_to_page, p.r2p_stride = r2p_stride;
+    p.table_rows = table_rows, p.max_ctx = max_ctx;
+    p.parents = parents, p.positions = positions, p.out_loc = out_cache_loc, p.cu = cu_seqlens_q, p.seq_lens = seq_lens;
+    p.mask = tree_mask, p.alloc_out = alloc_out, p.free_range_out = free_range_out, p.status = status;
+    p.scratch = static_cast<int4*>(workspace);
+    p.capacity = capacity, p.words = parents ? mask_words : 0, p.bs = bs, p.ps = page_size;
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    hipLaunchKernelGGL(extend_prepare_scan_kernel, dim3(1), dim3(kScanThreads), 0, st, p);
+    if (parents) hipLaunchKernelGGL(extend_prepare_tree_kernel, dim3((unsigned)((bs + 3) / 4)), dim3(256), 0, st, p);
+    else if (capacity) hipLaunchKernelGGL(extend_prepare_fill_kernel, dim3((unsigned)((capacity + 255) / 256)), dim3(256), 0, st, p);
+    return check_launch("extend_prepare kernels");
+}
+
+extern "C" int msgl_accept_tree(const int32_t* draft_tokens, const int32_t* target_tokens, const int32_t* parents, const int32_t* cu_seqlens_q,
+                                const int32_t* prefix_lens, const int32_t* out_cache_loc, const uint64_t* kv_layers, int num_layers,
+                                int64_t cache_stride, int Hkv, int D, int32_t* accept_lens, int32_t* accept_rows, int32_t* accept_tokens,
+                                int32_t* next_tokens, int32_t* seq_lens, int bs, int max_accept, void* stream) {
+    MSGL_REQUIRE(bs >= 0 && bs <= 65535 * 16 && num_layers >= 0 && num_layers <= 4096 && max_accept >= 1 && max_accept <= 64 * MSGL_TREE_MAX_WORDS,
+                 "msgl_accept_tree: bs=%d num_layers=%d max_accept=%d", bs, num_layers, max_accept);
+    if (bs == 0) return MSGL_OK;
+    MSGL_REQUIRE(draft_tokens && target_tokens && parents && cu_seqlens_q && prefix_lens && out_cache_loc && accept_lens && accept_rows && accept_tokens &&
+                     next_tokens && seq_lens && (num_layers == 0 || kv_layers),
+                 "msgl_accept_tree: null pointer argument");
+    MSGL_REQUIRE(num_layers == 0 || (Hkv > 0 && D > 0 && (int64_t)Hkv * D % 8 == 0 && cache_stride >= (int64_t)Hkv * D && cache_stride % 8 == 0),
+                 "msgl_accept_tree: Hkv=%d D=%d cache_stride=%lld (rows must be whole 16-byte pieces)", Hkv, D, (long long)cache_stride);
+    AcceptParams p;
+    p.draft = draft_tokens, p.target = target_tokens, p.parents = parents, p.cu = cu_seqlens_q, p.prefix = prefix_lens, p.loc = out_cache_loc;
+    p.layers = kv_layers, p.slot_bytes = cache_stride * 2, p.row_chunks = num_layers ? (int32_t)((int64_t)Hkv * D / 8) : 0;
+    p.lens = accept_lens, p.rows = accept_rows, p.tokens = accept_tokens, p.next = next_tokens, p.seq_lens = seq_lens;
+    p.bs = bs, p.num_layers = num_layers, p.most = max_accept;
+    // enough groups for eight per compute unit, each repeating the walk: fewer layers per group beyond that only repeat it more often
+    const int64_t want = 8 * (int64_t)device_cus();
+    const int groups = (int)(bs >= want ? 1 : num_layers > 1 ? (want + bs - 1) / bs < num_layers ? (want + bs - 1) / bs : num_layers : 1);
+    p.layers_per_group = num_layers ? (num_layers + groups - 1) / groups : 0;
+    const unsigned gy = num_layers ? (unsigned)((num_layers + p.layers_per_group - 1) / p.layers_per_group) : 1u;
+    hipLaunchKernelGGL(accept_tree_kernel, dim3((unsigned)bs, gy), dim3(256), 0, static_cast<hipStream_t>(stream), p);
+    return check_launch("accept_tree_kernel");
+}

@@ -5,6 +5,7 @@ Every function here runs a HIP kernel; none has a torch or CPU fallback.
 """
 from __future__ import annotations
 
+from dataclasses import dataclass
 from typing import List, Optional, Tuple
 
 import torch
@@ -613,6 +614,229 @@ def prepare_decode(req_pool_indices: torch.Tensor, seq_lens: torch.Tensor, last_
         req_to_token.shape[1], positions.data_ptr(),
         out_cache_loc.data_ptr(), next_tokens.data_ptr() if next_tokens is not None else None,
         input_ids.data_ptr() if input_ids is not None else None, status.data_ptr(), bs, page_size, _stream()))
+
+
+# ----------------------------------------------------------------------------- speculative decoding with drafted trees
+TREE_MAX_WORDS = 16        # MSGL_TREE_MAX_WORDS: mask words of 64 nodes per request
+LOGPROBS_MAX_TOP = 32      # MSGL_LOGPROBS_MAX_TOP
+
+
+def _launch(dev: torch.device, entry, *args) -> None:
+    """entry(*args, stream) on dev's current stream, with dev the current device while the kernels are launched."""
+    if torch.cuda.current_device() == dev.index:
+        _check(entry(*args, torch.cuda.current_stream(dev).cuda_stream))
+    else:
+        with torch.cuda.device(dev):
+            _check(entry(*args, torch.cuda.current_stream(dev).cuda_stream))
+
+
+def _i32_on(dev: torch.device, n: int, **tensors) -> None:
+    """Every tensor is a dense 1-D int32 tensor of n entries on dev."""
+    for name, t in tensors.items():
+        if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or t.device != dev or (n > 1 and t.stride(0) != 1):
+            raise ValueError(f"{name} must be a contiguous 1-D int32 tensor of {n} entries on {dev} "
+                             f"(got {t.dtype} {tuple(t.shape)}, strides {t.stride()}, on {t.device})")
+
+
+def _table_on(dev: torch.device, t: torch.Tensor, name: str) -> None:
+    _need(t.device == dev and t.dtype == torch.int32 and t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= t.shape[1],
+          f"{name} must be an int32 [reqs, ctx] tensor with dense rows on {dev}")
+
+
+def _scratch(workspace: Optional[torch.Tensor], need: int, dev: torch.device) -> Optional[torch.Tensor]:
+    if workspace is None:
+        return torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    _need(workspace.device == dev and workspace.is_contiguous() and workspace.data_ptr() % 16 == 0,
+          f"workspace must be a contiguous 16-byte aligned tensor on {dev}")
+    return workspace
+
+
+def _bytes(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.numel() * t.element_size()
+
+
+def prepare_extend_workspace_bytes(bs: int) -> int:
+    return int(_lib.msgl_prepare_extend_workspace_bytes(int(bs)))
+
+
+def prepare_extend(req_pool_indices: torch.Tensor, prefix_lens: torch.Tensor, new_lens: torch.Tensor, alloc_lens: torch.Tensor,
+                   free_pages: torch.Tensor, free_range: torch.Tensor, req_to_token: torch.Tensor, positions: torch.Tensor,
+                   out_cache_loc: torch.Tensor, cu_seqlens_q: torch.Tensor, seq_lens: torch.Tensor, status: torch.Tensor, page_size: int, *,
+                   parents: Optional[torch.Tensor] = None, tree_mask: Optional[torch.Tensor] = None,
+                   req_to_page: Optional[torch.Tensor] = None, alloc_out: Optional[torch.Tensor] = None,
+                   free_range_out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> None:
+    """Slots, positions and page-table entries of an extend step, built on the device from the lengths (see
+    msgl_prepare_extend); with ``parents`` also the positions and ancestor masks of drafted trees.  Writes ``positions``,
+    ``out_cache_loc`` (and ``tree_mask``: int64 [capacity, words]) of any capacity, ``cu_seqlens_q``, ``seq_lens`` and the tables;
+    ``alloc_lens`` and ``free_range`` advance in place unless ``alloc_out`` / ``free_range_out`` are given.  ``status``
+    (int32[1]) becomes non-zero if the step was refused, and nothing but empty outputs is written then."""
+    dev = req_pool_indices.device
+    _need(dev.type == "cuda", f"req_pool_indices must live on the GPU (got {dev})")
+    bs, capacity = req_pool_indices.numel(), out_cache_loc.numel()
+    alloc_out = alloc_lens if alloc_out is None else alloc_out
+    free_range_out = free_range if free_range_out is None else free_range_out
+    _i32_on(dev, bs, req_pool_indices=req_pool_indices, prefix_lens=prefix_lens, new_lens=new_lens, alloc_lens=alloc_lens, seq_lens=seq_lens,
+            alloc_out=alloc_out)
+    _i32_on(dev, capacity, positions=positions, out_cache_loc=out_cache_loc)
+    _i32_on(dev, free_pages.numel(), free_pages=free_pages)
+    _i32_on(dev, 2, free_range=free_range, free_range_out=free_range_out)
+    _i32_on(dev, bs + 1, cu_seqlens_q=cu_seqlens_q)
+    _i32_on(dev, 1, status=status)
+    _table_on(dev, req_to_token, "req_to_token")
+    _need((parents is None) == (tree_mask is None), "parents and tree_mask go together")
+    words = 0
+    if parents is not None:
+        _i32_on(dev, capacity, parents=parents)
+        _need(tree_mask.device == dev and tree_mask.dtype == torch.int64 and tree_mask.dim() == 2 and tree_mask.is_contiguous()
+              and tree_mask.shape[0] == capacity and 1 <= tree_mask.shape[1] <= TREE_MAX_WORDS,
+              f"tree_mask must be a contiguous int64 [{capacity}, 1..{TREE_MAX_WORDS}] tensor on {dev}")
+        words = tree_mask.shape[1]
+    if req_to_page is not None:
+        _table_on(dev, req_to_page, "req_to_page")
+        _need(req_to_page.shape[0] == req_to_token.shape[0], "req_to_page needs a row per row of req_to_token")
+    if bs == 0:
+        return
+    ws = _scratch(workspace, 16 * bs, dev)
+    _launch(dev, _lib.msgl_prepare_extend, req_pool_indices.data_ptr(), prefix_lens.data_ptr(), new_lens.data_ptr(), alloc_lens.data_ptr(),
+            free_pages.data_ptr(), free_pages.numel(), free_range.data_ptr(), req_to_token.data_ptr(), req_to_token.stride(0),
+            req_to_token.shape[0], req_to_token.shape[1], req_to_page.data_ptr() if req_to_page is not None else None,
+            req_to_page.stride(0) if req_to_page is not None else 0, parents.data_ptr() if parents is not None else None,
+            tree_mask.data_ptr() if tree_mask is not None else None, words, positions.data_ptr(), out_cache_loc.data_ptr(), capacity,
+            cu_seqlens_q.data_ptr(), seq_lens.data_ptr(), alloc_out.data_ptr(), free_range_out.data_ptr(), status.data_ptr(), bs, int(page_size),
+            ws.data_ptr(), _bytes(ws))
+
+
+def tree_attention_splits(bs: int, max_seqlen_q: int, max_seqlen_k: int, Hq: int, Hkv: int, total_kv: int = 0) -> int:
+    """Runs of keys per request that tree_attention takes for these bounds when its workspace allows."""
+    return int(_lib.msgl_tree_attention_splits(int(bs), int(max_seqlen_q), int(max_seqlen_k), int(total_kv), int(Hq), int(Hkv)))
+
+
+def tree_attention_workspace_bytes(total_tokens: int, Hq: int, D: int, splits: int) -> int:
+    return int(_lib.msgl_tree_attention_workspace_bytes(int(total_tokens), int(Hq), int(D), int(splits)))
+
+
+def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, req_to_token: torch.Tensor, req_pool_indices: torch.Tensor,
+                   cu_seqlens_q: torch.Tensor, prefix_lens: torch.Tensor, tree_mask: torch.Tensor, max_seqlen_q: int, max_seqlen_k: int,
+                   scale: float, *, total_kv: int = 0, out: Optional[torch.Tensor] = None,
+                   workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of drafted-tree nodes q [T, Hq, D] (packed behind cu_seqlens_q) over the paged cache: node i of request b sees the first
+    prefix_lens[b] positions and the nodes its row of ``tree_mask`` (int64 [T, words], from prepare_extend) names; see
+    msgl_tree_attention.  ``max_seqlen_q``: most nodes of a request.  ``max_seqlen_k`` (longest prefix + nodes) and ``total_kv`` (their
+    sum over the batch, 0 = unknown) steer the cut of long contexts; ``workspace`` (tree_attention_workspace_bytes) is allocated here when
+    omitted."""
+    dev = q.device
+    _dev_bf16(q, "q")
+    _need(q.dim() == 3 and q.stride(2) == 1 and q.stride(1) == q.shape[2], "q must be [T, Hq, D] with dense heads")
+    T, Hq, D = q.shape
+    _need(k_cache.dim() == 3, "k_cache must be [slots, Hkv, D]")
+    Hkv = k_cache.shape[1]
+    cs = _cache_stride(k_cache, v_cache, Hkv, D)
+    _need(k_cache.device == dev and v_cache.device == dev, f"k_cache / v_cache must live on {dev}")
+    bs = req_pool_indices.numel()
+    _i32_on(dev, bs, req_pool_indices=req_pool_indices, prefix_lens=prefix_lens)
+    _i32_on(dev, bs + 1, cu_seqlens_q=cu_seqlens_q)
+    _table_on(dev, req_to_token, "req_to_token")
+    _need(tree_mask.device == dev and tree_mask.dtype == torch.int64 and tree_mask.dim() == 2 and tree_mask.is_contiguous()
+          and tree_mask.shape[0] == T and 1 <= tree_mask.shape[1] <= TREE_MAX_WORDS,
+          f"tree_mask must be a contiguous int64 [{T}, 1..{TREE_MAX_WORDS}] tensor on {dev}")
+    _need(0 < max_seqlen_q <= 64 * tree_mask.shape[1] or T == 0, f"max_seqlen_q {max_seqlen_q} needs {-(-max_seqlen_q // 64)} mask words")
+    if out is None:
+        out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=dev)
+    else:
+        _dev_bf16(out, "out")
+        _need(out.device == dev and out.shape == q.shape and out.stride(2) == 1 and out.stride(1) == D, "out must match q's layout")
+    if T == 0 or bs == 0:
+        return out
+    if workspace is None:
+        splits = _lib.msgl_tree_attention_splits(bs, max_seqlen_q, max_seqlen_k, total_kv, Hq, Hkv)
+        ws = torch.empty(4 * (D + 2) * T * Hq * splits, dtype=torch.uint8, device=dev) if splits > 1 else None
+    else:
+        ws = _scratch(workspace, 0, dev)
+    _launch(dev, _lib.msgl_tree_attention, q.data_ptr(), q.stride(0) if T > 1 else Hq * D, k_cache.data_ptr(), v_cache.data_ptr(), cs,
+            req_to_token.data_ptr(), req_to_token.stride(0), req_pool_indices.data_ptr(), cu_seqlens_q.data_ptr(), prefix_lens.data_ptr(),
+            tree_mask.data_ptr(), tree_mask.shape[1], out.data_ptr(), out.stride(0) if T > 1 else Hq * D, T, bs, int(max_seqlen_q),
+            int(max_seqlen_k), int(total_kv), Hq, Hkv, D, float(scale), ws.data_ptr() if ws is not None else None, _bytes(ws))
+    return out
+
+
+@dataclass
+class KvLayers:
+    """The K and V caches of every layer as one device table of addresses, for kernels that work on all layers at once (accept_tree).
+    Holds the caches: the addresses stay valid as long as this does."""
+    table: torch.Tensor
+    k: List[torch.Tensor]
+    v: List[torch.Tensor]
+    slot_stride: int
+
+
+def kv_layers(k_buffers: List[torch.Tensor], v_buffers: List[torch.Tensor]) -> KvLayers:
+    """k_buffers / v_buffers: one [slots, Hkv, D] cache (or strided view of a pool) per layer, all of one layout, as
+    ``MHAKVPool.k_buffer`` / ``v_buffer``."""
+    _need(len(k_buffers) == len(v_buffers) and len(k_buffers) >= 1, "one K and one V cache per layer")
+    first = k_buffers[0]
+    _need(first.dim() == 3, "caches must be [slots, Hkv, D]")
+    strides = {_cache_stride(k, v, first.shape[1], first.shape[2]) for k, v in zip(k_buffers, v_buffers)}
+    _need(len(strides) == 1 and all(t.shape == first.shape and t.device == first.device for t in [*k_buffers, *v_buffers]),
+          "every layer's caches must have one shape, one slot stride and one device")
+    _need(all(t.data_ptr() % 16 == 0 for t in [*k_buffers, *v_buffers]) and first.shape[1] * first.shape[2] % 8 == 0 and next(iter(strides)) % 8 == 0,
+          "cache rows must be 16-byte aligned")
+    table = torch.tensor([[k.data_ptr(), v.data_ptr()] for k, v in zip(k_buffers, v_buffers)], dtype=torch.int64).to(first.device)
+    return KvLayers(table, list(k_buffers), list(v_buffers), strides.pop())
+
+
+def accept_tree(draft_tokens: torch.Tensor, target_tokens: torch.Tensor, parents: torch.Tensor, cu_seqlens_q: torch.Tensor,
+                prefix_lens: torch.Tensor, out_cache_loc: torch.Tensor, layers: Optional[KvLayers], accept_lens: torch.Tensor,
+                accept_rows: torch.Tensor, accept_tokens: torch.Tensor, next_tokens: torch.Tensor, seq_lens: torch.Tensor) -> None:
+    """Greedy acceptance of drafted trees (see msgl_accept_tree): from every root along the nodes whose ``draft_tokens`` entry is the
+    model's ``target_tokens`` entry of the node before.  Writes accept_lens [bs], accept_rows and accept_tokens [bs, most] (-1 behind the
+    path), next_tokens [bs] and seq_lens [bs] = prefix_lens + accept_lens (may be prefix_lens itself), and moves the accepted nodes' K and V
+    rows to consecutive positions in every layer of ``layers`` (None: moves nothing)."""
+    dev = draft_tokens.device
+    _need(dev.type == "cuda", f"draft_tokens must live on the GPU (got {dev})")
+    T, bs = draft_tokens.numel(), prefix_lens.numel()
+    _i32_on(dev, T, draft_tokens=draft_tokens, target_tokens=target_tokens, parents=parents, out_cache_loc=out_cache_loc)
+    _i32_on(dev, bs + 1, cu_seqlens_q=cu_seqlens_q)
+    _i32_on(dev, bs, prefix_lens=prefix_lens, accept_lens=accept_lens, next_tokens=next_tokens, seq_lens=seq_lens)
+    _need(accept_rows.dim() == 2 and accept_rows.shape[0] == bs and 1 <= accept_rows.shape[1] <= 64 * TREE_MAX_WORDS
+          and accept_tokens.shape == accept_rows.shape, f"accept_rows and accept_tokens must be [{bs}, 1..{64 * TREE_MAX_WORDS}]")
+    for name, t in (("accept_rows", accept_rows), ("accept_tokens", accept_tokens)):
+        _need(t.device == dev and t.dtype == torch.int32 and t.is_contiguous(), f"{name} must be a contiguous int32 tensor on {dev}")
+    if bs == 0:
+        return
+    if layers is None:
+        table, count, stride, Hkv, D = None, 0, 0, 0, 0
+    else:
+        _need(layers.table.device == dev, f"the caches must live on {dev}")
+        table, count, stride = layers.table.data_ptr(), len(layers.k), layers.slot_stride
+        _, Hkv, D = layers.k[0].shape
+    _launch(dev, _lib.msgl_accept_tree, draft_tokens.data_ptr(), target_tokens.data_ptr(), parents.data_ptr(), cu_seqlens_q.data_ptr(),
+            prefix_lens.data_ptr(), out_cache_loc.data_ptr(), table, count, stride, Hkv, D, accept_lens.data_ptr(), accept_rows.data_ptr(),
+            accept_tokens.data_ptr(), next_tokens.data_ptr(), seq_lens.data_ptr(), bs, accept_rows.shape[1])
+
+
+def token_logprobs_workspace_bytes(rows: int, vocab: int, dtype: torch.dtype, top_k: int = 0) -> int:
+    return int(_lib.msgl_token_logprobs_workspace_bytes(int(rows), int(vocab), 4 if dtype == torch.float32 else 2, int(top_k)))
+
+
+def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, top_k: int = 0, *, workspace: Optional[torch.Tensor] = None):
+    """(logprobs [rows], entropy [rows], top_ids int32 [rows, top_k], top_logprobs [rows, top_k]) of logits [rows, vocab] (bf16 or fp32),
+    all but the ids fp32: log softmax at ``token_ids`` (NaN for an id outside the vocabulary), the rows' entropies in nats, and the
+    top_k most probable tokens, ties to the lower id; see msgl_token_logprobs."""
+    dev = logits.device
+    _need(logits.is_cuda and logits.dtype in (torch.bfloat16, torch.float32), "logits must be bf16 or fp32 on the GPU")
+    rows, vocab, rs = _rows_view(logits, "logits")
+    _i32_on(dev, rows, token_ids=token_ids)
+    _need(0 <= top_k <= min(vocab, LOGPROBS_MAX_TOP), f"top_k {top_k} outside 0..min(vocab, {LOGPROBS_MAX_TOP})")
+    stats = torch.empty((2, rows), dtype=torch.float32, device=dev)
+    ids = torch.empty((rows, top_k), dtype=torch.int32, device=dev)
+    top = torch.empty((rows, top_k), dtype=torch.float32, device=dev)
+    size = logits.element_size()
+    if rows:
+        ws = _scratch(workspace, _lib.msgl_token_logprobs_workspace_bytes(rows, vocab, size, top_k), dev)
+        _launch(dev, _lib.msgl_token_logprobs, logits.data_ptr(), rs, size, token_ids.data_ptr(), stats.data_ptr(),
+                stats.data_ptr() + 4 * rows, ids.data_ptr() if top_k else None, top.data_ptr() if top_k else None, rows, vocab, top_k,
+                ws.data_ptr(), _bytes(ws))
+    return stats[0], stats[1], ids, top
 
 
 def stream_read(buf: torch.Tensor, sink: torch.Tensor, unroll: int = 8, groups_per_cu: int = 16, span_kib: int = 0) -> None:
