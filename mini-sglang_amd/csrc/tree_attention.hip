@@ -17,6 +17,11 @@
 //   * The page table is read per token, also by LDS-DMA, four tiles ahead: any page size, no scalar path, nothing the compiler counts.
 //   * All these loads are inline asm and waited for by count; their order is K0 V0 t3 K1 V1 | t4 K2 V2 | t5 K3 V3 ... (t = table entries).
 // Long contexts are cut into runs of keys (one work group each) that leave (O, max, sum) in the workspace; a second kernel joins them.
+#include <stdlib.h>
+
+#include <type_traits>
+#include <utility>
+
 #include "msgl_common.h"
 #include "extend_common.h"
 
@@ -29,6 +34,7 @@ constexpr int kTreeRing = 4 * kTreeHalf;            // per wave: two K tiles, tw
 constexpr int kTreeSlotRing = 4 * 256;              // per wave: table entries of four tiles (64 words each)
 constexpr int kTreeLds = kTreeWaves * (kTreeRing + kTreeSlotRing);
 constexpr int kTreeMergeRow = kHD + 4;              // floats per row of the exchange at the end (spread over the banks)
+constexpr int merge_bytes(int waves, int rb) { return waves * 32 * rb * (kTreeMergeRow + 2) * 4; }
 constexpr float kRescaleAt = 8.f;                   // log2 units a row's maximum may outgrow its reference before O is rescaled
 
 struct TreeParams {
@@ -49,7 +55,7 @@ struct TreeParams {
     float* ws_o;   // [token][head][split][128]
     float* ws_ml;  // [token][head][split][2]
     int Hq, Hkv, group;
-    int row_tiles, splits, chunk;
+    int items, row_tiles, splits, chunk;
     int max_q;
     float scale_log2e;
 };
@@ -99,36 +105,308 @@ __device__ __forceinline__ uint32_t mask_bits(const uint64_t* row, int words, in
     return (uint32_t)v;
 }
 
-template <int RB, bool NT>
-__global__ __launch_bounds__(kTreeWaves * 64, 1) void tree_attention_kernel(TreeParams p) {
-    extern __shared__ __attribute__((aligned(1024))) char smem[];
-    // block -> (row tile, kv head, request, run of keys), row tile fastest
-    int id = blockIdx.x;
-    const int rt = id % p.row_tiles;
-    id /= p.row_tiles;
-    const int h = id % p.Hkv;
-    id /= p.Hkv;
-    const int split = id % p.splits;
-    const int b = id / p.splits;
-    const int base = p.cu[b];
-    const int n = min(p.cu[b + 1] - base, p.max_q);
-    const int G = p.group;
-    const int rows = n * G;
-    const int r0 = rt * 32 * RB;
-    if (r0 >= rows) return;
-    const int prefix = p.prefix[b];
-    const int S = prefix + n;
-    const int nsplit = min((S + p.chunk - 1) / p.chunk, p.splits);
-    if (split >= nsplit) return;
-    const int t0 = split * p.chunk;
-    const int t1 = split == p.splits - 1 ? S : min(S, t0 + p.chunk);
+// What a work group is asked for: one request's run of keys [t0, t1) against rows r0 .. of a kv head, as (node, head) pairs.
+struct TreeItem {
+    int b, base, n, rows, r0, prefix, t0, t1, split, nsplit;
+    bool none;
+};
+__device__ __forceinline__ TreeItem tree_item(const TreeParams& p, int b, int split, int r0) {
+    TreeItem it;
+    it.b = b, it.split = split, it.r0 = r0;
+    it.base = p.cu[b];
+    it.n = min(p.cu[b + 1] - it.base, p.max_q);
+    it.rows = it.n * p.group;
+    it.prefix = p.prefix[b];
+    const int S = it.prefix + it.n;
+    it.nsplit = min((S + p.chunk - 1) / p.chunk, p.splits);
+    it.none = r0 >= it.rows || split >= it.nsplit;
+    it.t0 = split * p.chunk;
+    it.t1 = split == p.splits - 1 ? S : min(S, it.t0 + p.chunk);
+    return it;
+}
 
+// A wave's running state for RB blocks of 32 rows: O^T (dims 32 mb + 8 (i >> 2) + 4 half + (i & 3) in register i of block mb, row lane & 31),
+// reference maximum in log2 units, this lane half's share of the sum.
+template <int RB>
+struct TreeState {
+    f32x16_t o[RB][4];
+    float m[RB], l[RB];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+#pragma unroll
+            for (int mb = 0; mb < 4; ++mb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[rb][mb][i] = 0.f;
+            m[rb] = kNegBigE, l[rb] = 0.f;
+        }
+    }
+};
+
+// f(integral_constant<int, 0>) ... f(integral_constant<int, N - 1>): register arrays indexed by constants before any optimisation runs
+template <int... I, typename F>
+__device__ __forceinline__ void each_of(F&& f, std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void each(F&& f) {
+    each_of(f, std::make_integer_sequence<int, N>{});
+}
+
+// Q^T fragments: lane (row lane & 31, half) holds dims 16 ks + 8 half .. + 8.  Rows behind the last one repeat it; they are never stored.
+template <int RB>
+__device__ __forceinline__ void load_queries(const TreeParams& p, const TreeItem& it, int row0, int h, int lane, bf16x8_t (&qf)[RB][8]) {
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+        const int r = min(row0 + rb * 32 + (lane & 31), it.rows - 1);
+        const int node = r / p.group;
+        const uint16_t* qp = p.q + (int64_t)(it.base + node) * p.q_stride + (h * p.group + r - node * p.group) * kHD + (lane >> 5) * 8;
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) qf[rb][ks] = as_bf16x8(*reinterpret_cast<const uint4*>(qp + ks * 16));
+    }
+    // in registers before any load that the compiler does not count is under way
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) asm volatile("" : "+v"(qf[rb][ks]));
+}
+
+// K fragments of a 32-key tile: row lane & 31, piece 2 ks + half (at that piece ^ (row & 15)).
+__device__ __forceinline__ void read_keys(const char* kt, int lane, bf16x8_t (&kf)[8]) {
+    const int col = lane & 31, half = lane >> 5;
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks) kf[ks] = as_bf16x8(*reinterpret_cast<const uint4*>(kt + col * 256 + (((2 * ks + half) ^ (col & 15)) << 4)));
+}
+
+// V^T fragments: the 16 lanes of a group name 4 rows x 32 bytes and receive one dim each of those 4 rows: rows 16 ks + 8 pair + 4 half +
+// (lane & 15 >> 2), dims 32 mb + 16 (lane >> 4 & 1) + (lane & 15); 16-byte piece c of row r lies at c ^ 4 (r & 3).
+__device__ __forceinline__ bf16x8_t read_values(const char* vt, int lane, int mb, int ks) {
+    const int q16 = lane & 15, row = 4 * (lane >> 5) + (q16 >> 2);
+    const int piece = (4 * mb + 2 * (lane >> 4 & 1) + ((q16 >> 1) & 1)) ^ (4 * (row & 3));
+    const char* at = vt + row * 256 + (piece << 4) + (q16 & 1) * 8;
+    short4_t x[2];
+#pragma unroll
+    for (int pair = 0; pair < 2; ++pair)
+        x[pair] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)(at + (16 * ks + 8 * pair) * 256));
+    return __builtin_bit_cast(bf16x8_t, (short8_t){x[0][0], x[0][1], x[0][2], x[0][3], x[1][0], x[1][1], x[1][2], x[1][3]});
+}
+
+template <int RB>
+__device__ __forceinline__ void tile_scores(const bf16x8_t (&kf)[8], const bf16x8_t (&qf)[RB][8], f32x16_t (&s)[RB]) {
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[rb][i] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) s[rb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[ks], qf[rb][ks], s[rb], 0, 0, 0);
+    }
+}
+
+// What a row sees of the tile that begins at key0: bit k for key k.
+__device__ __forceinline__ uint32_t row_sees(const TreeParams& p, const TreeItem& it, int row, int key0) {
+    const int rel = key0 - it.prefix;
+    const uint64_t* bits = p.mask + (int64_t)(it.base + min(row, it.rows - 1) / p.group) * p.words;
+    uint32_t see = rel >= 0 ? mask_bits(bits, p.words, rel) : rel <= -32 ? ~0u : (mask_bits(bits, p.words, 0) << -rel) | ((1u << -rel) - 1);
+    if (key0 + kTreeKeys > it.t1) see &= (1u << (it.t1 - key0)) - 1;
+    return see;
+}
+
+// Hides what the rows do not see of the tile that begins at key0.
+// s[rb][i]: key 8 (i >> 2) + 4 half + (i & 3) of the tile, row lane & 31 of the block.
+template <int RB>
+__device__ __forceinline__ void tile_mask(const TreeParams& p, const TreeItem& it, int row0, int key0, int lane, f32x16_t (&s)[RB]) {
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+        const uint32_t bits = row_sees(p, it, row0 + rb * 32 + (lane & 31), key0) >> (4 * (lane >> 5));
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (!(bits >> (8 * (i >> 2) + (i & 3)) & 1)) s[rb][i] = -INFINITY;
+    }
+}
+
+// The row's reference maximum follows the maximum of its scores (top, over this lane's keys) when that has outgrown it by 2^8 (or is the first):
+// probabilities up to 2^8 are as exact in bf16 and as harmless in the sums, and O is rescaled in the first tiles only.
+template <int RB>
+__device__ __forceinline__ void follow_maximum(float scale_log2e, float (&top)[RB], TreeState<RB>& st) {
+    bool grown = false;
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+        top[rb] = max_with_lane_xor32(top[rb]) * scale_log2e;
+        grown |= top[rb] > st.m[rb] + kRescaleAt;
+    }
+    if (__any(grown)) {
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+            const float mn = fmaxf(st.m[rb], top[rb]);
+            const float f = fast_exp2(st.m[rb] - mn);
+            st.m[rb] = mn;
+            st.l[rb] *= f;
+#pragma unroll
+            for (int mb = 0; mb < 4; ++mb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) st.o[rb][mb][i] *= f;
+        }
+    }
+}
+template <int RB>
+__device__ __forceinline__ void tile_reference(float scale_log2e, const f32x16_t (&s)[RB], TreeState<RB>& st) {
+    float top[RB];
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+        top[rb] = s[rb][0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) top[rb] = fmaxf(top[rb], s[rb][i]);
+    }
+    follow_maximum<RB>(scale_log2e, top, st);
+}
+
+// Scores to probabilities relative to the reference, their sum, and the second product's operand.
+template <int RB>
+__device__ __forceinline__ void tile_probabilities(float scale_log2e, f32x16_t (&s)[RB], TreeState<RB>& st, bf16x8_t (&pf)[RB][2]) {
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            s[rb][i] = fast_exp2(__builtin_fmaf(s[rb][i], scale_log2e, -st.m[rb]));
+            sum += s[rb][i];
+        }
+        st.l[rb] += sum;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+            pf[rb][ks] = as_bf16x8(make_uint4(pack_bf16(s[rb][8 * ks], s[rb][8 * ks + 1]), pack_bf16(s[rb][8 * ks + 2], s[rb][8 * ks + 3]),
+                                              pack_bf16(s[rb][8 * ks + 4], s[rb][8 * ks + 5]), pack_bf16(s[rb][8 * ks + 6], s[rb][8 * ks + 7])));
+    }
+}
+
+template <int RB>
+__device__ __forceinline__ void tile_values(const char* vt, int lane, const bf16x8_t (&pf)[RB][2], TreeState<RB>& st) {
+#pragma unroll
+    for (int mb = 0; mb < 4; ++mb)
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            const bf16x8_t vf = read_values(vt, lane, mb, ks);
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) st.o[rb][mb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[rb][ks], st.o[rb][mb], 0, 0, 0);
+        }
+}
+
+// In a tile with hidden keys a row must not touch what it does not see: 0 * NaN and 0 * inf are NaN.  There the product is taken of the finite
+// values; whether there were others (a branch of the tree that went wrong) is returned, and add_odd_values deals with them at the end.
+template <int RB>
+__device__ __forceinline__ bool tile_values_masked(const char* vt, int lane, const bf16x8_t (&pf)[RB][2], TreeState<RB>& st) {
+    bool odd = false;
+#pragma unroll
+    for (int mb = 0; mb < 4; ++mb)
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            const uint4 x = __builtin_bit_cast(uint4, read_values(vt, lane, mb, ks));
+            uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const bool lo = (w[i] & 0x7f80u) == 0x7f80u, hi = (w[i] & 0x7f800000u) == 0x7f800000u;
+                odd |= lo || hi;
+                w[i] &= (lo ? 0xffff0000u : ~0u) & (hi ? 0xffffu : ~0u);
+            }
+            const bf16x8_t vf = as_bf16x8(make_uint4(w[0], w[1], w[2], w[3]));
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) st.o[rb][mb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[rb][ks], st.o[rb][mb], 0, 0, 0);
+        }
+    return __any(odd);
+}
+
+// The values that are not finite, added to the rows that see them (a softmax weight is never 0, whatever 32 bits make of it).  o: this wave's rows in
+// LDS.  Runs only where a tile had such a value.
+__device__ __forceinline__ void add_odd_values(const TreeParams& p, const TreeItem& it, int row0, int rows, int h, int key0, int lane, float* o) {
+    const int32_t* table = p.r2t + (int64_t)p.req_idx[it.b] * p.r2t_stride;
+    for (int r = lane; r < rows; r += 64) {
+        const uint32_t see = row_sees(p, it, row0 + r, key0);
+        for (int k = 0; k < kTreeKeys && key0 + k < it.t1; ++k) {
+            const uint16_t* v = reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(p.vc) + (uint64_t)(uint32_t)table[key0 + k] * p.slot_bytes) + h * kHD;
+            for (int d = 0; d < kHD; ++d)
+                if ((v[d] & 0x7f80u) == 0x7f80u && (see >> k & 1)) o[r * kTreeMergeRow + d] += bf16_lo(v[d]);
+        }
+    }
+}
+
+// End of a work group: groups of WPH waves hold the same rows (different keys); their states are joined through LDS and written, as the final
+// rows if the request has this one run, else as the run's partial.  row0(g) / head(g): first row and kv head of wave group g; bit t of odd: this
+// wave's tile at odd_key0 + t * odd_step held values that are not finite.
+template <int RB, int WPH, int NW, typename Row0, typename Head>
+__device__ __forceinline__ void join_and_store(const TreeParams& p, const TreeItem& it, TreeState<RB>& st, char* smem, int wave, int lane, uint64_t odd, int odd_key0,
+                                               int odd_step, Row0 row0, Head head) {
+    constexpr int R = 32 * RB;
+    const int half = lane >> 5, col = lane & 31;
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) st.l[rb] += __shfl_xor(st.l[rb], 32);
+    __syncthreads();  // every wave is done with the tiles
+    float* lds_o = reinterpret_cast<float*>(smem);               // [wave][row][kTreeMergeRow]
+    float* lds_ml = lds_o + NW * R * kTreeMergeRow;      // [wave][row][2]
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+        float* dst = lds_o + (wave * R + rb * 32 + col) * kTreeMergeRow + 4 * half;
+#pragma unroll
+        for (int mb = 0; mb < 4; ++mb)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<float4*>(dst + 32 * mb + 8 * i) =
+                    make_float4(st.o[rb][mb][4 * i], st.o[rb][mb][4 * i + 1], st.o[rb][mb][4 * i + 2], st.o[rb][mb][4 * i + 3]);
+        if (half == 0) *reinterpret_cast<float2*>(lds_ml + (wave * R + rb * 32 + col) * 2) = make_float2(st.m[rb], st.l[rb]);
+    }
+    if (__syncthreads_or(odd != 0)) {
+        for (int t = 0; odd >> t; ++t)
+            if (odd >> t & 1)
+                add_odd_values(p, it, row0(wave / WPH), R, head(wave / WPH), odd_key0 + t * odd_step, lane, lds_o + wave * R * kTreeMergeRow);
+        __syncthreads();
+    }
+    for (int idx = threadIdx.x; idx < (NW / WPH) * R * 32; idx += NW * 64) {
+        const int g = idx / (R * 32), r = (idx >> 5) % R, d = (idx & 31) * 4;
+        const int row = row0(g) + r;
+        if (row >= it.rows) continue;
+        float M = kNegBigE;
+#pragma unroll
+        for (int w = 0; w < WPH; ++w) M = fmaxf(M, lds_ml[((g * WPH + w) * R + r) * 2]);
+        float L = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < WPH; ++w) {
+            const float2 ml = *reinterpret_cast<const float2*>(lds_ml + ((g * WPH + w) * R + r) * 2);
+            const float f = fast_exp2(ml.x - M);
+            L += f * ml.y;
+            const float4 x = *reinterpret_cast<const float4*>(lds_o + ((g * WPH + w) * R + r) * kTreeMergeRow + d);
+            acc.x += f * x.x, acc.y += f * x.y, acc.z += f * x.z, acc.w += f * x.w;
+        }
+        const int node = row / p.group;
+        const int hq = head(g) * p.group + row - node * p.group;
+        const int64_t tok = it.base + node;
+        if (it.nsplit == 1) {
+            const float inv = L == 0.f ? 0.f : 1.0f / L;  // L == 0: the row sees nothing
+            *reinterpret_cast<uint2*>(p.out + tok * p.out_stride + hq * kHD + d) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+        } else {
+            const int64_t at = (tok * p.Hq + hq) * p.splits + it.split;
+            *reinterpret_cast<float4*>(p.ws_o + at * kHD + d) = acc;
+            if (d == 0) *reinterpret_cast<float2*>(p.ws_ml + at * 2) = make_float2(M, L);
+        }
+    }
+}
+
+// HPB kv heads per work group, 4 / HPB waves per head.
+template <int RB, int HPB>
+__global__ __launch_bounds__(kTreeWaves * 64, 1) void tree_attention_kernel(TreeParams p) {
+    constexpr int WPH = kTreeWaves / HPB;
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    // block -> (group of heads, run of keys, request), heads fastest: the token rows' pieces are read at about the same time
+    const int hgroups = p.Hkv / HPB;
+    const int hg = blockIdx.x % (unsigned)hgroups;
+    const int id = blockIdx.x / (unsigned)hgroups;
+    const TreeItem it = tree_item(p, id / p.splits, id % p.splits, 0);
+    if (it.none) return;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int half = lane >> 5, col = lane & 31;
+    const int h = hg * HPB + wave / WPH, sub = wave % WPH;
     const int g4 = lane >> 4, q16 = lane & 15;
-    const int all_tiles = (t1 - t0 + kTreeKeys - 1) / kTreeKeys;
-    const int T = all_tiles > wave ? (all_tiles - wave + kTreeWaves - 1) / kTreeWaves : 0;  // own tiles: wave, wave + 4, ...
+    const int all_tiles = (it.t1 - it.t0 + kTreeKeys - 1) / kTreeKeys;
+    const int T = all_tiles > sub ? (all_tiles - sub + WPH - 1) / WPH : 0;  // own tiles: sub, sub + WPH, ...
 
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
     char* ring = smem + wave * kTreeRing;
@@ -136,265 +414,322 @@ __global__ __launch_bounds__(kTreeWaves * 64, 1) void tree_attention_kernel(Tree
     const uint32_t ring_at = lds0 + wave * kTreeRing;
     const uint32_t words_at = lds0 + kTreeWaves * kTreeRing + wave * kTreeSlotRing;
 
-    f32x16_t o[RB][4];
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-        for (int mb = 0; mb < 4; ++mb)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[rb][mb][i] = 0.f;
-    float m[RB], l[RB];
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) m[rb] = kNegBigE, l[rb] = 0.f;
-
+    TreeState<RB> st;
+    st.clear();
+    uint64_t odd = 0;  // tiles behind the plain ones that held a value that is not finite
+    const int plain = (max(0, (min(it.prefix, it.t1) - it.t0) / kTreeKeys - sub) + WPH - 1) / WPH;  // own tiles that every row sees whole
     if (T > 0) {
-        const int32_t* table = p.r2t + (int64_t)p.req_idx[b] * p.r2t_stride;
+        const int32_t* table = p.r2t + (int64_t)p.req_idx[it.b] * p.r2t_stride;
         // table entries of own tile j, lane (g4', i) <- key 4 i + g4' of the tile, so that a lane of the K/V loads finds its eight rows'
         // entries in 32 consecutive bytes.  Positions behind the run's last key repeat that key.
         const int word_key = 4 * (lane & 7) + ((lane >> 3) & 3);
         auto issue_words = [&](int j) {
-            const int pos = min(t0 + (wave + j * kTreeWaves) * kTreeKeys + word_key, t1 - 1);
+            const int pos = min(it.t0 + (sub + j * WPH) * kTreeKeys + word_key, it.t1 - 1);
             dma_words((uint64_t)(table + pos), words_at + (j & 3) * 256);
         };
         issue_words(0);
         issue_words(1);
         issue_words(2);
-        // Q^T fragments: lane (row col, half) holds dims 16 ks + 8 half .. + 8.  Rows behind the last one repeat it; they are not stored.
         bf16x8_t qf[RB][8];
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-            const int r = min(r0 + rb * 32 + col, rows - 1);
-            const int node = r / G;
-            const uint16_t* qp = p.q + (int64_t)(base + node) * p.q_stride + (h * G + r - node * G) * kHD + half * 8;
-#pragma unroll
-            for (int ks = 0; ks < 8; ++ks) qf[rb][ks] = as_bf16x8(*reinterpret_cast<const uint4*>(qp + ks * 16));
-        }
-        // everything so far has arrived, the query in registers: from here on the loads in flight are this kernel's to count
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-            for (int ks = 0; ks < 8; ++ks) asm volatile("" : "+v"(qf[rb][ks]));
-        wait_loads<0>();
+        load_queries<RB>(p, it, 0, h, lane, qf);
+        wait_loads<0>();  // from here on the loads in flight are this kernel's to count
 
-        // K rows: 16-byte piece c of row r lies at piece c ^ (r & 15); V rows: at piece c ^ 4 (r & 3).  A lane loads piece q16 of rows
-        // 4 i + g4, so it fetches the piece that belongs there.
+        // a lane loads piece q16 of rows 4 i + g4, so it fetches the piece that belongs there (read_keys, read_values)
         uint64_t kfrom[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) kfrom[i] = (uint64_t)(p.kc + h * kHD) + ((q16 ^ (4 * i + g4)) << 4);
         const uint64_t vfrom = (uint64_t)(p.vc + h * kHD) + ((q16 ^ (4 * g4)) << 4);
-        auto issue_k = [&](int j) {
+        auto issue_rows = [&](int j, bool values) {
             const int4 s0 = *reinterpret_cast<const int4*>(words + (j & 3) * 256 + g4 * 32), s1 = *reinterpret_cast<const int4*>(words + (j & 3) * 256 + g4 * 32 + 16);
             const uint32_t s[8] = {(uint32_t)s0.x, (uint32_t)s0.y, (uint32_t)s0.z, (uint32_t)s0.w, (uint32_t)s1.x, (uint32_t)s1.y, (uint32_t)s1.z, (uint32_t)s1.w};
             uint64_t a[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) a[i] = (uint64_t)s[i] * p.slot_bytes + kfrom[i & 3];
-            dma_tile<NT>(a, ring_at + (j & 1) * kTreeHalf);
+            for (int i = 0; i < 8; ++i) a[i] = (uint64_t)s[i] * p.slot_bytes + (values ? vfrom : kfrom[i & 3]);
+            dma_tile<true>(a, ring_at + ((values ? 2 : 0) + (j & 1)) * kTreeHalf);
         };
-        auto issue_v = [&](int j) {
-            const int4 s0 = *reinterpret_cast<const int4*>(words + (j & 3) * 256 + g4 * 32), s1 = *reinterpret_cast<const int4*>(words + (j & 3) * 256 + g4 * 32 + 16);
-            const uint32_t s[8] = {(uint32_t)s0.x, (uint32_t)s0.y, (uint32_t)s0.z, (uint32_t)s0.w, (uint32_t)s1.x, (uint32_t)s1.y, (uint32_t)s1.z, (uint32_t)s1.w};
-            uint64_t a[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) a[i] = (uint64_t)s[i] * p.slot_bytes + vfrom;
-            dma_tile<NT>(a, ring_at + (2 + (j & 1)) * kTreeHalf);
-        };
-        issue_k(0);
-        issue_v(0);
+        issue_rows(0, false);
+        issue_rows(0, true);
         if (T > 1) {
             issue_words(3);
-            issue_k(1);
-            issue_v(1);
+            issue_rows(1, false);
+            issue_rows(1, true);
         }
-        // LDS offsets of the fragment reads: K row col, piece (2 ks + half) ^ (col & 15); V^T: the 16 lanes of a group name 4 rows x 32
-        // bytes and receive one dim each of those 4 rows: rows 16 s + 8 pair + 4 half + (q16 >> 2), dims 32 mb + 16 (g4 & 1) + q16.
-        const uint32_t kread = (uint32_t)col * 256, kswz = (uint32_t)(col & 15);
-        const uint32_t vrow = 4 * half + (q16 >> 2);
-        const uint32_t vread = vrow * 256 + (q16 & 1) * 8;
-        const uint32_t vpiece = 2 * (g4 & 1) + ((q16 >> 1) & 1), vswz = 4 * (vrow & 3);
-
-        for (int j = 0; j < T; ++j) {
-            const bool more = j + 2 < T, next = j + 1 < T;
-            // outstanding behind K(j): V(j), and if there is a next tile t(j+3), K(j+1), V(j+1)
-            if (next) wait_loads<25>();
+        // outstanding behind K(j): V(j), and if there is a next tile t(j+3), K(j+1), V(j+1)
+        auto keys_of = [&](int j, f32x16_t (&s)[RB]) __attribute__((always_inline)) {
+            if (j + 1 < T) wait_loads<25>();
             else wait_loads<8>();
-            const char* kt = ring + (j & 1) * kTreeHalf;
             bf16x8_t kf[8];
-#pragma unroll
-            for (int ks = 0; ks < 8; ++ks) kf[ks] = as_bf16x8(*reinterpret_cast<const uint4*>(kt + kread + (((2 * ks + half) ^ kswz) << 4)));
-            if (more) {
+            read_keys(ring + (j & 1) * kTreeHalf, lane, kf);
+            if (j + 2 < T) {
                 issue_words(j + 4);
-                issue_k(j + 2);
+                issue_rows(j + 2, false);
             }
-            f32x16_t s[RB];
-#pragma unroll
-            for (int rb = 0; rb < RB; ++rb) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[rb][i] = 0.f;
-#pragma unroll
-                for (int ks = 0; ks < 8; ++ks) s[rb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[ks], qf[rb][ks], s[rb], 0, 0, 0);
-            }
-            // s[rb][i]: key 8 (i >> 2) + 4 half + (i & 3) of the tile, row col of the block
-            const int key0 = t0 + (wave + j * kTreeWaves) * kTreeKeys;
-            const bool masked = key0 + kTreeKeys > min(prefix, t1);
-            uint32_t see[RB];
-            if (masked) {
-                const int rel = key0 - prefix;
-#pragma unroll
-                for (int rb = 0; rb < RB; ++rb) {
-                    const int node = min(r0 + rb * 32 + col, rows - 1) / G;
-                    const uint64_t* row = p.mask + (int64_t)(base + node) * p.words;
-                    uint32_t bits = rel >= 0 ? mask_bits(row, p.words, rel) : rel <= -32 ? ~0u : (mask_bits(row, p.words, 0) << -rel) | ((1u << -rel) - 1);
-                    if (key0 + kTreeKeys > t1) bits &= (1u << (t1 - key0)) - 1;
-                    see[rb] = bits;
-                    bits >>= 4 * half;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (!(bits >> (8 * (i >> 2) + (i & 3)) & 1)) s[rb][i] = -INFINITY;
-                }
-            }
-            bf16x8_t pf[RB][2];
-            float pr[RB][16];
-#pragma unroll
-            for (int rb = 0; rb < RB; ++rb) {
-                float top = s[rb][0];
-#pragma unroll
-                for (int i = 1; i < 16; ++i) top = fmaxf(top, s[rb][i]);
-                top = fmaxf(top, __shfl_xor(top, 32)) * p.scale_log2e;
-                // the reference follows the maximum when that has outgrown it by 2^8, or is the first: probabilities up to 2^8 are as exact
-                if (__any(top > m[rb] + kRescaleAt)) {
-                    const float mn = fmaxf(m[rb], top);
-                    const float f = fast_exp2(m[rb] - mn);
-                    m[rb] = mn;
-                    l[rb] *= f;
-#pragma unroll
-                    for (int mb = 0; mb < 4; ++mb)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) o[rb][mb][i] *= f;
-                }
-                uint32_t w[8];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) pr[rb][i] = fast_exp2(__builtin_fmaf(s[rb][i], p.scale_log2e, -m[rb]));
-#pragma unroll
-                for (int i = 0; i < 16; ++i) l[rb] += pr[rb][i];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) w[i] = pack_bf16(pr[rb][2 * i], pr[rb][2 * i + 1]);
-                pf[rb][0] = as_bf16x8(make_uint4(w[0], w[1], w[2], w[3]));
-                pf[rb][1] = as_bf16x8(make_uint4(w[4], w[5], w[6], w[7]));
-            }
-            // outstanding behind V(j): t(j+3), K(j+1), V(j+1), t(j+4), K(j+2)
-            if (more) wait_loads<26>();
-            else if (next) wait_loads<17>();
+            tile_scores<RB>(kf, qf, s);
+        };
+        // outstanding behind V(j): t(j+3), K(j+1), V(j+1), t(j+4), K(j+2)
+        auto wait_values = [&](int j) __attribute__((always_inline)) {
+            if (j + 2 < T) wait_loads<26>();
+            else if (j + 1 < T) wait_loads<17>();
             else wait_loads<0>();
-            const char* vt = ring + (2 + (j & 1)) * kTreeHalf;
-            bf16x8_t vf[4][2];
-#pragma unroll
-            for (int mb = 0; mb < 4; ++mb)
-#pragma unroll
-                for (int ks = 0; ks < 2; ++ks) {
-                    short4_t x[2];
-#pragma unroll
-                    for (int pair = 0; pair < 2; ++pair)
-                        x[pair] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)(
-                            vt + (16 * ks + 8 * pair) * 256 + vread + (((4 * mb + vpiece) ^ vswz) << 4)));
-                    vf[mb][ks] = __builtin_bit_cast(bf16x8_t, (short8_t){x[0][0], x[0][1], x[0][2], x[0][3], x[1][0], x[1][1], x[1][2], x[1][3]});
-                }
-            // In a tile with hidden keys a row must not touch what it does not see: 0 * NaN and 0 * inf are NaN.  If such a value is in the
-            // tile (a branch of the tree that went wrong), its products are taken key by key, by those rows that see the key.
-            bool plain = true;
-            if (masked) {
-                bool odd = false;
-#pragma unroll
-                for (int mb = 0; mb < 4; ++mb)
-#pragma unroll
-                    for (int ks = 0; ks < 2; ++ks) {
-                        const uint4 x = __builtin_bit_cast(uint4, vf[mb][ks]);
-                        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) odd |= (w[i] & 0x7f80u) == 0x7f80u || (w[i] & 0x7f800000u) == 0x7f800000u;
-                    }
-                plain = !__any(odd);
-            }
-            if (plain) {
-                if (more) issue_v(j + 2);
-#pragma unroll
-                for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-                    for (int mb = 0; mb < 4; ++mb)
-#pragma unroll
-                        for (int ks = 0; ks < 2; ++ks) o[rb][mb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[mb][ks], pf[rb][ks], o[rb][mb], 0, 0, 0);
-            } else {
-#pragma unroll
-                for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-#pragma unroll 1
-                        for (int hh = 0; hh < 2; ++hh) {
-                            const int key = 8 * (i >> 2) + 4 * hh + (i & 3);
-                            const float pk = __shfl(pr[rb][i], col + 32 * hh);
-                            if (see[rb] >> key & 1) {
-                                const char* vr = vt + key * 256;
-#pragma unroll
-                                for (int mb = 0; mb < 4; ++mb)
-#pragma unroll
-                                    for (int d = 0; d < 16; ++d) {
-                                        const int dim = 32 * mb + 8 * (d >> 2) + 4 * half + (d & 3);
-                                        const uint16_t x = *reinterpret_cast<const uint16_t*>(vr + (((dim >> 3) ^ (4 * (key & 3))) << 4) + (dim & 7) * 2);
-                                        o[rb][mb][d] += pk * bf16_lo(x);
-                                    }
-                            }
-                        }
-                if (more) issue_v(j + 2);
-            }
+            return ring + (2 + (j & 1)) * kTreeHalf;
+        };
+        int j = 0;
+        for (; j < plain; ++j) {
+            f32x16_t s[RB];
+            bf16x8_t pf[RB][2];
+            keys_of(j, s);
+            tile_reference<RB>(p.scale_log2e, s, st);
+            tile_probabilities<RB>(p.scale_log2e, s, st, pf);
+            tile_values<RB>(wait_values(j), lane, pf, st);
+            if (j + 2 < T) issue_rows(j + 2, true);
+        }
+        for (; j < T; ++j) {
+            f32x16_t s[RB];
+            bf16x8_t pf[RB][2];
+            keys_of(j, s);
+            tile_mask<RB>(p, it, 0, it.t0 + (sub + j * WPH) * kTreeKeys, lane, s);
+            tile_reference<RB>(p.scale_log2e, s, st);
+            tile_probabilities<RB>(p.scale_log2e, s, st, pf);
+            if (tile_values_masked<RB>(wait_values(j), lane, pf, st)) odd |= 1ull << (j - plain);
+            if (j + 2 < T) issue_rows(j + 2, true);
         }
     }
     wait_loads<0>();
-    // the waves' states, joined: O^T has dims 32 mb + 8 (i >> 2) + 4 half + (i & 3) in register i of block mb
+    join_and_store<RB, WPH, kTreeWaves>(p, it, st, smem, wave, lane, odd, it.t0 + (sub + plain * WPH) * kTreeKeys, WPH * kTreeKeys, [](int) { return 0; },
+                            [&](int g) { return hg * HPB + g; });
+}
+
+// More than 64 rows per kv head: the NW waves hold 32 rows each and share the tiles, so that K and V are read once per 32 NW rows.  A tile is loaded by
+// all waves, 32 / NW keys each, SLOTS - 2 tiles ahead into a ring; a wave waits for its own loads of tile j, then the barrier says that everybody's
+// have landed and that everybody is done with tile j - 2, whose slot is filled anew.  Two waves per SIMD either way (NW = 8 and one work group
+// per compute unit, or NW = 4 and two): a wave issues an instruction about every eighth cycle, whatever it is, so one wave cannot keep
+// softmax and matrix products side by side (measured with 64 rows a wave, one wave per SIMD: 786 TFLOP/s with all keys in L2).
+template <int NW>
+struct TreeWide {
+    static constexpr int kSlots = NW == 8 ? 8 : 4;
+    static constexpr int kAhead = kSlots - 2;
+    static constexpr int kKeys = kTreeKeys / NW;              // a wave's keys of a tile
+    static constexpr int kLoads = kKeys / 4;                  // LDS-DMA loads of 4 rows for them, K and V each
+    static constexpr int kBlock = 64 / kKeys;                 // tiles whose table entries one load brings
+    static constexpr int kRing = kSlots * 2 * kTreeHalf;
+    static constexpr int kTiles = kRing + NW * 2 * 256;       // two blocks of table entries per wave
+    static constexpr int kLds = kTiles > merge_bytes(NW, 1) ? kTiles : merge_bytes(NW, 1);
+    static_assert(kAhead <= kBlock - 1, "a block of table entries is refilled once its last tile has been requested");
+};
+
+// 4 rows x 256 bytes of K to 1 KiB at LDS byte address dst, and of V to the same place in the V half of the tile.
+template <bool NT>
+__device__ __forceinline__ void dma_rows4(uint64_t k, uint64_t v, uint32_t dst) {
+    static_assert(kTreeHalf == 0x2000, "distance of the halves in the statement");
+    unsigned keep;
+    if (NT)
+        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off nt\n\ts_add_u32 m0, m0, 0x2000\n\ts_nop 0\n\t"
+                     "global_load_lds_dwordx4 %3, off nt\n\ts_mov_b32 m0, %0"
+                     : "=&s"(keep)
+                     : "s"(dst), "v"(k), "v"(v)
+                     : "memory", "scc");
+    else
+        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\ts_add_u32 m0, m0, 0x2000\n\ts_nop 0\n\t"
+                     "global_load_lds_dwordx4 %3, off\n\ts_mov_b32 m0, %0"
+                     : "=&s"(keep)
+                     : "s"(dst), "v"(k), "v"(v)
+                     : "memory", "scc");
+}
+
+template <int NW, bool NT>
+__global__ __launch_bounds__(NW * 64, 2) void tree_attention_wide_kernel(TreeParams p) {
+    using W = TreeWide<NW>;
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    // block -> item, row tile: the row tiles of an item run on the same XCD (block ids modulo 8), whose L2 then holds the keys for all of them
+    const int y = blockIdx.x >> 3;
+    const int rt = y % p.row_tiles;
+    const int item = (y / p.row_tiles) * 8 + (blockIdx.x & 7);
+    if (item >= p.items) return;
+    const int h = item % p.Hkv;
+    const int id = item / p.Hkv;
+    const TreeItem it = tree_item(p, id / p.splits, id % p.splits, rt * 32 * NW);
+    if (it.none) return;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g4 = lane >> 4, q16 = lane & 15;
+    const int row0 = it.r0 + wave * 32;
+    const int T = (it.t1 - it.t0 + kTreeKeys - 1) / kTreeKeys;
+
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
+    char* words = smem + W::kRing + wave * 512;
+    const uint32_t words_at = lds0 + W::kRing + wave * 512;
+    const int32_t* table = p.r2t + (int64_t)p.req_idx[it.b] * p.r2t_stride;
+    // entry kKeys t + kLoads g4' + i of a block: key kKeys wave + 4 i + g4' of the block's tile t
+    const int in_tile = lane % W::kKeys;
+    const int word_key = lane / W::kKeys * kTreeKeys + W::kKeys * wave + 4 * (in_tile % W::kLoads) + in_tile / W::kLoads;
+    auto issue_words = [&](int block) {
+        const int pos = min(it.t0 + block * W::kBlock * kTreeKeys + word_key, it.t1 - 1);
+        dma_words((uint64_t)(table + pos), words_at + (block & 1) * 256);
+    };
+    issue_words(0);
+    issue_words(1);
+    bf16x8_t qf[1][8];
+    load_queries<1>(p, it, row0, h, lane, qf);
+    wait_loads<0>();
+    uint64_t kfrom[W::kLoads];
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) l[rb] += __shfl_xor(l[rb], 32);
-    __syncthreads();  // every wave is done with its ring
-    float* lds_o = reinterpret_cast<float*>(smem);                              // [wave][row][kTreeMergeRow]
-    float* lds_ml = lds_o + kTreeWaves * 32 * RB * kTreeMergeRow;               // [wave][row][2]
+    for (int i = 0; i < W::kLoads; ++i) kfrom[i] = (uint64_t)(p.kc + h * kHD) + ((q16 ^ ((W::kKeys * wave + 4 * i + g4) & 15)) << 4);
+    const uint64_t vfrom = (uint64_t)(p.vc + h * kHD) + ((q16 ^ (4 * g4)) << 4);
+    auto issue_tile = [&](int j) __attribute__((always_inline)) {
+        const char* w = words + (j * W::kKeys * 4 & 511) + W::kLoads * g4 * 4;
+        const uint32_t dst = lds0 + (j % W::kSlots) * 2 * kTreeHalf + wave * (W::kKeys * 256);
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-        float* dst = lds_o + (wave * 32 * RB + rb * 32 + col) * kTreeMergeRow + 4 * half;
-#pragma unroll
-        for (int mb = 0; mb < 4; ++mb)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                *reinterpret_cast<float4*>(dst + 32 * mb + 8 * i) = make_float4(o[rb][mb][4 * i], o[rb][mb][4 * i + 1], o[rb][mb][4 * i + 2], o[rb][mb][4 * i + 3]);
-        if (half == 0) {
-            lds_ml[(wave * 32 * RB + rb * 32 + col) * 2] = m[rb];
-            lds_ml[(wave * 32 * RB + rb * 32 + col) * 2 + 1] = l[rb];
+        for (int i = 0; i < W::kLoads; ++i) {
+            const uint64_t o = (uint64_t)reinterpret_cast<const uint32_t*>(w)[i] * p.slot_bytes;
+            dma_rows4<NT>(kfrom[i] + o, vfrom + o, dst + i * 1024);
         }
+    };
+    for (int j = 0; j < W::kAhead; ++j) issue_tile(j);
+
+    TreeState<1> st;
+    st.clear();
+    uint64_t odd = 0;  // tiles behind the plain ones that held a value that is not finite
+    // Tile j can be read after this.  Every call requests one tile more, behind the run's end the last key over and over, so that the count is
+    // always the same (a table block among the loads only makes the wait stricter) and there is no branch.
+    auto arrive = [&](int j) __attribute__((always_inline)) {
+        wait_loads<2 * W::kLoads * (W::kAhead - 1)>();
+        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): what this wave has read of tile j - 2 is in registers
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");  // no read of the tile moves ahead of the barrier
+        issue_tile(j + W::kAhead);
+    };
+    // the block of table entries whose last tile arrive(j) has requested is filled anew
+    auto refill = [&](int j) __attribute__((always_inline)) {
+        if ((j + W::kAhead + 1) % W::kBlock == 0) issue_words((j + W::kAhead) / W::kBlock + 2);
+    };
+    auto tile_at = [&](int j) { return smem + (j % W::kSlots) * 2 * kTreeHalf; };
+    const int plain = max(0, min(it.prefix, it.t1) - it.t0) / kTreeKeys;  // tiles that every row sees whole
+    int j = 0;
+    if (row0 >= it.rows) {  // no rows for this wave: it loads and keeps the barriers
+        for (; j < T; ++j) arrive(j), refill(j);
+    } else if (plain > 2) {
+        // The steady state is one stream of 16 matrix instructions per tile, each a slice with its share of everything else:
+        //   slices 0 .. 7     S^T of tile j + 1 (its K fragments are in registers); V^T fragments of tile j are read
+        //   slices 8 .. 15    O^T of tile j; tile j + 2 arrives, its K fragments are read
+        // and beside them the exponentials of tile j, sixteen in eleven slices, each pair packed the slice after, and over the last quarter the
+        // maximum of the new scores.  A step is one basic block (a branch inside would let the compiler sink the exponentials behind it), and
+        // four steps are unrolled: a tile's place in a 64 KiB half of the ring is then an immediate of the reads.
+        f32x16_t sa[1], sb[1];
+        bf16x8_t kf[8], vf[4][2], pf[1][2];
+        float top[1];
+        arrive(0);
+        read_keys(tile_at(0), lane, kf);
+        tile_scores<1>(kf, qf, sa);
+        tile_reference<1>(p.scale_log2e, sa, st);
+        arrive(1);
+        refill(0), refill(1);
+        read_keys(tile_at(1), lane, kf);
+        typedef __attribute__((address_space(3))) char lds_char;
+        uint32_t kat[8], vat[4];  // LDS addresses of the fragment reads in the ring's current half
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) kat[ks] = lds0 + (lane & 31) * 256 + (((2 * ks + (lane >> 5)) ^ (lane & 15)) << 4);
+#pragma unroll
+        for (int mb = 0; mb < 4; ++mb) {
+            const int row = 4 * (lane >> 5) + (q16 >> 2);
+            vat[mb] = lds0 + kTreeHalf + row * 256 + (((4 * mb + 2 * (g4 & 1) + ((q16 >> 1) & 1)) ^ (4 * (row & 3))) << 4) + (q16 & 1) * 8;
+        }
+        auto step = [&](int j, auto C, f32x16_t& s, f32x16_t& next) __attribute__((always_inline)) {
+            constexpr uint32_t vimm = decltype(C)::value * 2 * kTreeHalf, kimm = ((decltype(C)::value + 2) & 3) * 2 * kTreeHalf;
+            uint32_t pk[8];
+            each<16>([&](auto K) __attribute__((always_inline)) {
+                constexpr int k = K;
+                if constexpr (k < 8) {
+                    f32x16_t c;
+                    if constexpr (k == 0) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) c[i] = 0.f;
+                    } else {
+                        c = next;
+                    }
+                    next = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[k], qf[0][k], c, 0, 0, 0);
+                    short4_t x[2];
+#pragma unroll
+                    for (int pair = 0; pair < 2; ++pair)
+                        x[pair] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (__attribute__((address_space(3))) short4_t*)((lds_char*)(uintptr_t)vat[k & 3] + (vimm + (16 * (k >> 2) + 8 * pair) * 256)));
+                    vf[k & 3][k >> 2] = __builtin_bit_cast(bf16x8_t, (short8_t){x[0][0], x[0][1], x[0][2], x[0][3], x[1][0], x[1][1], x[1][2], x[1][3]});
+                } else {
+                    constexpr int e = k - 8, ks = e / 4, mb = e % 4;
+                    if constexpr (e == 0) arrive(j + 2);
+                    st.o[0][mb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[mb][ks], pf[0][ks], st.o[0][mb], 0, 0, 0);
+                    kf[e] = __builtin_bit_cast(bf16x8_t, *(const __attribute__((address_space(3))) u32x4_t*)((lds_char*)(uintptr_t)kat[e] + kimm));
+                }
+                // exponential i in slice 11 i / 16
+                each<16>([&](auto U) __attribute__((always_inline)) {
+                    constexpr int i = U;
+                    if constexpr (i * 11 / 16 == k) s[i] = fast_exp2(__builtin_fmaf(s[i], p.scale_log2e, -st.m[0]));
+                    if constexpr (i * 11 / 16 == k - 1) {
+                        st.l[0] += s[i];
+                        if constexpr (i % 2 == 1) pk[i / 2] = pack_bf16(s[i - 1], s[i]);
+                        if constexpr (i == 7) pf[0][0] = as_bf16x8(make_uint4(pk[0], pk[1], pk[2], pk[3]));
+                        if constexpr (i == 15) pf[0][1] = as_bf16x8(make_uint4(pk[4], pk[5], pk[6], pk[7]));
+                    }
+                });
+                if constexpr (k >= 12) {  // (the last S^T instruction lies four matrix instructions back: its result is there)
+                    constexpr int at = (k - 12) * 4;
+                    top[0] = max3_raw(at == 0 ? next[0] : top[0], next[at], next[at + 1]);
+                    top[0] = max3_raw(top[0], next[at + 2], next[at + 3]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            });
+            follow_maximum<1>(p.scale_log2e, top, st);
+            refill(j + 2);
+            if constexpr (W::kSlots == 8 && decltype(C)::value == 1) {
+#pragma unroll
+                for (int ks = 0; ks < 8; ++ks) kat[ks] ^= 8 * kTreeHalf;
+            }
+            if constexpr (W::kSlots == 8 && decltype(C)::value == 3) {
+#pragma unroll
+                for (int mb = 0; mb < 4; ++mb) vat[mb] ^= 8 * kTreeHalf;
+            }
+        };
+        constexpr std::integral_constant<int, 0> c0{};
+        constexpr std::integral_constant<int, 1> c1{};
+        constexpr std::integral_constant<int, 2> c2{};
+        constexpr std::integral_constant<int, 3> c3{};
+        for (; j + 5 < plain; j += 4) {
+            step(j, c0, sa[0], sb[0]);
+            step(j + 1, c1, sb[0], sa[0]);
+            step(j + 2, c2, sa[0], sb[0]);
+            step(j + 3, c3, sb[0], sa[0]);
+        }
+        if (j + 2 < plain) {
+            step(j, c0, sa[0], sb[0]);
+            if (j + 3 < plain) {
+                step(j + 1, c1, sb[0], sa[0]);
+                if (j + 4 < plain) step(j + 2, c2, sa[0], sb[0]);
+            }
+        }
+        if ((plain - 2 - j) & 1) sa[0] = sb[0];
+        j = plain - 2;
+        tile_probabilities<1>(p.scale_log2e, sa, st, pf);
+        tile_values<1>(tile_at(j) + kTreeHalf, lane, pf, st);
+        tile_scores<1>(kf, qf, sa);
+        tile_reference<1>(p.scale_log2e, sa, st);
+        tile_probabilities<1>(p.scale_log2e, sa, st, pf);
+        tile_values<1>(tile_at(j + 1) + kTreeHalf, lane, pf, st);
+        j = plain;
     }
-    __syncthreads();
-    for (int idx = threadIdx.x; idx < 32 * RB * 32; idx += kTreeWaves * 64) {
-        const int r = idx >> 5, d = (idx & 31) * 4;
-        if (r0 + r >= rows) break;
-        float M = kNegBigE;
-#pragma unroll
-        for (int w = 0; w < kTreeWaves; ++w) M = fmaxf(M, lds_ml[(w * 32 * RB + r) * 2]);
-        float L = 0.f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int w = 0; w < kTreeWaves; ++w) {
-            const float f = fast_exp2(lds_ml[(w * 32 * RB + r) * 2] - M);
-            L += f * lds_ml[(w * 32 * RB + r) * 2 + 1];
-            const float4 x = *reinterpret_cast<const float4*>(lds_o + (w * 32 * RB + r) * kTreeMergeRow + d);
-            acc.x += f * x.x, acc.y += f * x.y, acc.z += f * x.z, acc.w += f * x.w;
-        }
-        const int node = (r0 + r) / G;
-        const int hq = h * G + (r0 + r) - node * G;
-        const int64_t tok = base + node;
-        if (nsplit == 1) {
-            const float inv = L == 0.f ? 0.f : 1.0f / L;  // L == 0: the row sees nothing
-            *reinterpret_cast<uint2*>(p.out + tok * p.out_stride + hq * kHD + d) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
-        } else {
-            const int64_t at = (tok * p.Hq + hq) * p.splits + split;
-            *reinterpret_cast<float4*>(p.ws_o + at * kHD + d) = acc;
-            if (d == 0) *reinterpret_cast<float2*>(p.ws_ml + at * 2) = make_float2(M, L);
-        }
+    for (; j < T; ++j) {
+        f32x16_t s[1];
+        bf16x8_t kf[8], pf[1][2];
+        arrive(j);
+        refill(j);
+        read_keys(tile_at(j), lane, kf);
+        tile_scores<1>(kf, qf, s);
+        if (j >= plain) tile_mask<1>(p, it, row0, it.t0 + j * kTreeKeys, lane, s);
+        tile_reference<1>(p.scale_log2e, s, st);
+        tile_probabilities<1>(p.scale_log2e, s, st, pf);
+        if (j < plain) tile_values<1>(tile_at(j) + kTreeHalf, lane, pf, st);
+        else if (tile_values_masked<1>(tile_at(j) + kTreeHalf, lane, pf, st)) odd |= 1ull << (j - plain);
     }
+    wait_loads<0>();
+    join_and_store<1, 1, NW>(p, it, st, smem, wave, lane, odd, it.t0 + plain * kTreeKeys, kTreeKeys, [&](int g) { return it.r0 + g * 32; }, [&](int) { return h; });
 }
 
 // Joins the runs of one (token, head) per wave: two dims per lane.
@@ -428,35 +763,53 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeParams p) {
     *reinterpret_cast<uint32_t*>(p.out + (int64_t)(base + node) * p.out_stride + hq * kHD + 2 * lane) = pack_bf16(o0 * inv, o1 * inv);
 }
 
-template <int RB, bool NT>
-static int launch_tree(const TreeParams& p, int64_t blocks, hipStream_t stream) {
-    constexpr int kMerge = kTreeWaves * 32 * RB * (kTreeMergeRow + 2) * 4;
-    constexpr int kLds = kTreeLds > kMerge ? kTreeLds : kMerge;
-    static PerDeviceOnce once;  // more than the 64 KiB a kernel gets by default
-    if (!once.ensure([] {
-            return hipFuncSetAttribute(reinterpret_cast<const void*>(tree_attention_kernel<RB, NT>), hipFuncAttributeMaxDynamicSharedMemorySize, kLds) ==
-                   hipSuccess;
-        })) {
-        set_error("msgl_tree_attention: cannot reserve %d bytes of LDS", kLds);
+// Kernels that need more than the 64 KiB of LDS a kernel gets by default.
+template <typename K>
+static int launch_tree(K kernel, PerDeviceOnce& once, int lds, int waves, const TreeParams& p, int64_t blocks, hipStream_t stream) {
+    if (!once.ensure([&] { return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds) == hipSuccess; })) {
+        set_error("msgl_tree_attention: cannot reserve %d bytes of LDS", lds);
         return MSGL_E_LAUNCH;
     }
-    hipLaunchKernelGGL((tree_attention_kernel<RB, NT>), dim3((unsigned)blocks), dim3(kTreeWaves * 64), kLds, stream, p);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(waves * 64), lds, stream, p);
     return check_launch("tree_attention_kernel");
+}
+template <int RB, int HPB>
+static int launch_narrow(const TreeParams& p, int64_t blocks, hipStream_t stream) {
+    static PerDeviceOnce once;
+    return launch_tree(&tree_attention_kernel<RB, HPB>, once, kTreeLds > merge_bytes(kTreeWaves, RB) ? kTreeLds : merge_bytes(kTreeWaves, RB), kTreeWaves, p,
+                       blocks, stream);
+}
+template <int NW, bool NT>
+static int launch_wide(const TreeParams& p, int64_t blocks, hipStream_t stream) {
+    static PerDeviceOnce once;
+    return launch_tree(&tree_attention_wide_kernel<NW, NT>, once, TreeWide<NW>::kLds, NW, p, blocks, stream);
 }
 
 constexpr int kMaxTreeSplits = 256;
 
-static int tree_row_tiles(int max_q, int group) {
-    const int rows = max_q * group;
-    return (rows + 63) / 64;  // blocks of 32 rows, two to a work group where there are two
+// How the rows of a kv head are dealt: up to 64 to waves that share them and take different keys, more to waves that hold 32 or 64 rows each and
+// share the keys.
+struct TreeShape {
+    int waves;  // 0: the narrow kernel
+    int rb, row_tiles, hpb;
+};
+static TreeShape tree_shape(int max_q, int Hq, int Hkv) {
+    const int64_t rows = (int64_t)max_q * (Hq / Hkv);
+    TreeShape s;
+    s.waves = rows <= 64 ? 0 : rows <= 128 ? 4 : 8;
+    s.rb = rows > 32 && rows <= 64 ? 2 : 1;
+    s.row_tiles = s.waves ? (int)((rows + 32 * s.waves - 1) / (32 * s.waves)) : 1;
+    s.hpb = 1; if (!s.waves && getenv("TREE_HPB")) { s.hpb = atoi(getenv("TREE_HPB")); if (s.hpb > Hkv) s.hpb = 1; }
+    return s;
 }
 
 // Runs of keys per request: enough work groups for the chip, each at least four tiles (one per wave) long.
 static int tree_splits(int bs, int max_q, int max_k, int64_t total_kv, int Hq, int Hkv) {
     if (bs <= 0 || max_q <= 0 || max_k <= 0 || Hkv <= 0 || Hq < Hkv) return 1;
+    const TreeShape sh = tree_shape(max_q, Hq, Hkv);
     const int64_t keys = total_kv > 0 && total_kv < (int64_t)bs * max_k ? total_kv : (int64_t)bs * max_k;
-    const int64_t per_key = (int64_t)Hkv * tree_row_tiles(max_q, Hq / Hkv);
-    const int64_t want = 2 * (int64_t)device_cus();
+    const int64_t per_key = (int64_t)(Hkv / sh.hpb) * sh.row_tiles;
+    const int64_t want = (sh.waves == 8 ? 1 : 2) * (int64_t)device_cus();
     int64_t chunk = (keys * per_key + want - 1) / want;
     if (chunk < kTreeKeys * kTreeWaves) chunk = kTreeKeys * kTreeWaves;
     int64_t splits = (max_k + chunk - 1) / chunk;
@@ -502,7 +855,8 @@ extern "C" int msgl_tree_attention(const void* q, int64_t q_stride, const void* 
     p.mask = tree_mask, p.words = mask_words;
     p.out = static_cast<uint16_t*>(out), p.out_stride = out_stride;
     p.Hq = Hq, p.Hkv = Hkv, p.group = Hq / Hkv, p.max_q = max_seqlen_q;
-    p.row_tiles = tree_row_tiles(max_seqlen_q, p.group);
+    const TreeShape sh = tree_shape(max_seqlen_q, Hq, Hkv);
+    p.row_tiles = sh.row_tiles;
     p.scale_log2e = scale * 1.44269504088896340736f;
     int splits = tree_splits(bs, max_seqlen_q, max_seqlen_k, total_kv, Hq, Hkv);
     // as many runs as the workspace has room for
@@ -514,13 +868,21 @@ extern "C" int msgl_tree_attention(const void* q, int64_t q_stride, const void* 
     p.ws_o = static_cast<float*>(workspace);
     p.ws_ml = p.ws_o + (splits > 1 ? (size_t)total_tokens * Hq * splits * kHD : 0);
     MSGL_REQUIRE(splits == 1 || aligned16(workspace), "msgl_tree_attention: workspace must be 16-byte aligned");
-    const int64_t blocks = (int64_t)bs * splits * Hkv * p.row_tiles;
+    const int64_t items = (int64_t)bs * splits * (Hkv / sh.hpb);
+    const int64_t blocks = sh.waves ? (items + 7) / 8 * 8 * p.row_tiles : items;
     MSGL_REQUIRE(blocks <= 0x7fffffff, "msgl_tree_attention: %lld work groups", (long long)blocks);
+    p.items = (int)items;
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    const bool once = p.row_tiles == 1;  // K and V are read by one work group: past the caches
     int rc;
-    if (max_seqlen_q * p.group <= 32) rc = launch_tree<1, true>(p, blocks, st);
-    else rc = once ? launch_tree<2, true>(p, blocks, st) : launch_tree<2, false>(p, blocks, st);
+    if (sh.waves) {
+        const bool once = p.row_tiles == 1;  // K and V are read by one work group: past the caches
+        if (sh.waves == 4) rc = once ? launch_wide<4, true>(p, blocks, st) : launch_wide<4, false>(p, blocks, st);
+        else rc = once ? launch_wide<8, true>(p, blocks, st) : launch_wide<8, false>(p, blocks, st);
+    } else if (sh.rb == 1) {
+        rc = sh.hpb == 4 ? launch_narrow<1, 4>(p, blocks, st) : sh.hpb == 2 ? launch_narrow<1, 2>(p, blocks, st) : launch_narrow<1, 1>(p, blocks, st);
+    } else {
+        rc = sh.hpb == 4 ? launch_narrow<2, 4>(p, blocks, st) : sh.hpb == 2 ? launch_narrow<2, 2>(p, blocks, st) : launch_narrow<2, 1>(p, blocks, st);
+    }
     if (rc != MSGL_OK || splits == 1) return rc;
     const int64_t waves = (int64_t)bs * max_seqlen_q * Hq;
     hipLaunchKernelGGL(tree_merge_kernel, dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, st, p);
