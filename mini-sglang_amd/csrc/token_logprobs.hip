@@ -2,20 +2,25 @@
 //
 //   logprob = x_t - m - ln Z,  H = ln Z - (sum e_i (x_i - m)) / Z,  e_i = exp(x_i - m),  Z = sum e_i,  m = max x_i
 //
-// One read of the logits.  A work group takes a segment of a row (2048 pieces of 16 bytes, eight per thread, all requested before
-// the first is used, and kept in registers) and leaves (m, Z, sum e (x - m)) and the segment's k best (value, index) pairs in the
-// workspace; a second kernel folds a row's segments.
+// One read of the logits.  A work group takes a segment of a row (LOADS pieces of 16 bytes per thread, all requested before the first is used,
+// and kept in registers) and leaves (reference, Z, sum e (x - reference)) and the segment's k best (value, index) pairs in the workspace; a second
+// kernel folds a row's segments.
 //
 // Order of the alternatives: by value, ties to the lower index, NaN above everything (as msgl_argmax).  Value and index are one
 // 64-bit key: the float's bits mapped to an unsigned number that rises with the value, then the index's complement.
+// The k best of a segment: the k-th largest of a wave's 64 lane maxima is no larger than the segment's k-th largest value, so the few values
+// that reach it (in every wave's view: the largest of the four) are all that has to be ranked.  The k-th largest lane maximum comes from
+// bisecting its bits with ballots.  Segments where that leaves too many (long ties that are not a fill from the segment's start on, NaN,
+// infinities) are taken apart winner by winner instead.
+#include "extend_common.h"
 #include "msgl_common.h"
 
 namespace msgl {
 
 constexpr int kLpThreads = 256;
-constexpr int kLpLoads = 8;                        // 16-byte pieces per thread
-constexpr int kLpPieces = kLpThreads * kLpLoads;   // pieces per segment
-constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int kLpWaves = kLpThreads / 64;
+constexpr int kLpCandidates = 1024;
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
 
 struct SegmentStats {
     double ref;  // natural units: e = exp(x - ref)
@@ -42,6 +47,7 @@ __device__ __forceinline__ uint32_t order_key(float x) {
     const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.0f);  // -0 -> +0: equal values, equal keys
     return b ^ ((int32_t)b < 0 ? 0xffffffffu : 0x80000000u);
 }
+constexpr uint32_t kLowestKey = 0x007fffffu;  // of -inf
 __device__ __forceinline__ float key_value(uint32_t k) {
     if (k == kNanKey) return __builtin_nanf("");
     return __builtin_bit_cast(float, k & 0x80000000u ? k ^ 0x80000000u : ~k);
@@ -68,8 +74,30 @@ __device__ __forceinline__ uint64_t block_max_key(uint64_t x, uint64_t* lds) {
     __syncthreads();
     x = lds[0];
 #pragma unroll
-    for (int w = 1; w < kLpThreads / 64; ++w) x = lds[w] > x ? lds[w] : x;
+    for (int w = 1; w < kLpWaves; ++w) x = lds[w] > x ? lds[w] : x;
     return x;
+}
+
+// The k-th largest of the wave's 64 keys, as far as its upper `bits` bits go (the others 0); 0 if k > 64.
+__device__ __forceinline__ uint32_t wave_kth(uint32_t key, int k, int bits) {
+    uint32_t t = 0;
+    for (int b = 31; b > 31 - bits; --b) {
+        const uint32_t with = t | 1u << b;
+        if (__popcll(__ballot(key >= with)) >= k) t = with;
+    }
+    return t;
+}
+
+// Ranks `count` distinct keys and hands the `top` largest to put(rank, key); the places behind the last one get 0.
+template <typename Put>
+__device__ __forceinline__ void rank_keys(const uint64_t* keys, int count, int top, Put put) {
+    for (int i = threadIdx.x; i < count; i += kLpThreads) {
+        const uint64_t mine = keys[i];
+        int rank = 0;
+        for (int j = 0; j < count; ++j) rank += keys[j] > mine;
+        if (rank < top) put(rank, mine);
+    }
+    for (int i = count + threadIdx.x; i < top; i += kLpThreads) put(i, 0);
 }
 
 // element e of a 16-byte piece
@@ -80,98 +108,168 @@ __device__ __forceinline__ float piece_value(const uint4& v, int e) {
     return e & 1 ? bf16_hi(w[e >> 1]) : bf16_lo(w[e >> 1]);
 }
 
-template <int BYTES>
+template <int BYTES, int LOADS>
 __global__ __launch_bounds__(kLpThreads) void logprob_segment_kernel(LogprobParams p) {
-    constexpr int E = 16 / BYTES;  // elements per piece
-    __shared__ float lds_f[kLpThreads / 64][2];
-    __shared__ uint64_t lds_k[kLpThreads / 64];
+    constexpr int E = 16 / BYTES;                     // elements per piece
+    constexpr int kPieces = kLpThreads * LOADS;       // pieces per segment
+    __shared__ float lds_f[kLpWaves][2];
+    __shared__ uint32_t lds_t[kLpWaves];
+    __shared__ uint64_t lds_k[kLpCandidates];
+    __shared__ int lds_n[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t row = blockIdx.x / (unsigned)p.segments;
     const int seg = blockIdx.x - (unsigned)row * (unsigned)p.segments;
     // rows may start anywhere: whole aligned pieces are read (a piece with one of the row's elements in it is the row's own memory or
-    // its allocation's), and what lies outside the row is left out
+    // its allocation's), and what lies outside the row counts as -inf
     const char* first = p.logits + row * p.row_bytes;
     const int lead = (int)((uintptr_t)first & 15) / BYTES;
     const char* base = first - lead * BYTES;
     const int pieces = (int)(((int64_t)lead + p.vocab + E - 1) / E);
-    uint4 v[kLpLoads];
+    auto index = [&](int j, int e) { return (seg * kPieces + j * kLpThreads + tid) * E + e - lead; };
+    auto inside = [&](int j, int e) { return (unsigned)index(j, e) < (unsigned)p.vocab; };
+    uint4 v[LOADS];
 #pragma unroll
-    for (int j = 0; j < kLpLoads; ++j) {
-        const int g = seg * kLpPieces + j * kLpThreads + tid;
+    for (int j = 0; j < LOADS; ++j) {
+        const int g = seg * kPieces + j * kLpThreads + tid;
         constexpr uint32_t none = BYTES == 4 ? 0xff800000u : 0xff80ff80u;  // -inf
         v[j] = make_uint4(none, none, none, none);
         if (g < pieces) v[j] = *reinterpret_cast<const uint4*>(base + (int64_t)g * 16);
     }
-    auto index = [&](int j, int e) { return (seg * kLpPieces + j * kLpThreads + tid) * E + e - lead; };
-    auto inside = [&](int j, int e) { return (unsigned)index(j, e) < (unsigned)p.vocab; };
-    float m = -INFINITY;
+    if (tid < 2) lds_n[tid] = 0;
 #pragma unroll
-    for (int j = 0; j < kLpLoads; ++j)
+    for (int j = 0; j < LOADS; ++j) {  // the row's first and last piece
+        if (inside(j, 0) && inside(j, E - 1)) continue;
+        uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
 #pragma unroll
         for (int e = 0; e < E; ++e)
-            if (inside(j, e)) m = fmaxf(m, piece_value<BYTES>(v[j], e));
-    m = wave_max(m);
-    if (lane == 0) lds_f[wave][0] = m;
-    __syncthreads();
+            if (!inside(j, e)) {
+                if (BYTES == 4) w[e & 3] = 0xff800000u;
+                else w[e >> 1 & 3] = e & 1 ? (w[e >> 1 & 3] & 0xffffu) | 0xff800000u : (w[e >> 1 & 3] & 0xffff0000u) | 0xff80u;
+            }
+        v[j] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    float best[LOADS], mine = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kLpThreads / 64; ++w) m = fmaxf(m, lds_f[w][0]);
+    for (int j = 0; j < LOADS; ++j) {
+        best[j] = piece_value<BYTES>(v[j], 0);
+#pragma unroll
+        for (int e = 2; e < E; e += 2) best[j] = max3_raw(best[j], piece_value<BYTES>(v[j], e - 1), piece_value<BYTES>(v[j], e));
+        best[j] = fmaxf(best[j], piece_value<BYTES>(v[j], E - 1));
+        mine = fmaxf(mine, best[j]);
+    }
+    const float top_wave = wave_max(mine);
+    // 16 bits of the threshold are enough to leave few candidates
+    const uint32_t bar_wave = p.top ? wave_kth(order_key(mine), p.top, 16) : 0;
+    if (lane == 0) lds_f[wave][0] = top_wave, lds_t[wave] = bar_wave;
+    __syncthreads();
+    float m = lds_f[0][0];
+    uint32_t bar = max(lds_t[0], kLowestKey);
+#pragma unroll
+    for (int w = 1; w < kLpWaves; ++w) m = fmaxf(m, lds_f[w][0]), bar = max(bar, lds_t[w]);
     const float ref = m == -INFINITY ? 0.f : m;  // nothing but -inf here: every e is 0 (or NaN)
     float z = 0.f, t = 0.f;
 #pragma unroll
-    for (int j = 0; j < kLpLoads; ++j)
+    for (int j = 0; j < LOADS; ++j)
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-            if (inside(j, e)) {
-                const float d = piece_value<BYTES>(v[j], e) - ref;
-                const float x = fast_exp2(d * kLog2e);
-                z += x;
-                t += x * fmaxf(d, -200.f);  // e^-200 is 0 in 32 bits: -inf and the like add 0, not 0 * inf
-            }
+        for (int e = 0; e < E; ++e) {
+            const float d = (piece_value<BYTES>(v[j], e) - ref) * kLog2e;
+            const float x = fast_exp2(d);
+            z += x;
+            t += x * fmaxf(d, -200.f);  // 2^-200 is 0 in 32 bits: -inf and the like add 0, not 0 * inf
+        }
     z = wave_sum(z), t = wave_sum(t);
     __syncthreads();
     if (lane == 0) lds_f[wave][0] = z, lds_f[wave][1] = t;
     __syncthreads();
-    if (tid == 0) {
-        z = t = 0.f;
+    z = t = 0.f;
 #pragma unroll
-        for (int w = 0; w < kLpThreads / 64; ++w) z += lds_f[w][0], t += lds_f[w][1];
-        p.stats[row * p.segments + seg] = SegmentStats{(double)ref, z, t};
+    for (int w = 0; w < kLpWaves; ++w) z += lds_f[w][0], t += lds_f[w][1];
+    if (tid == 0) p.stats[row * p.segments + seg] = SegmentStats{(double)ref, z, t * kLn2};
+    if (p.top == 0) return;
+
+    uint64_t* out = p.keys + (row * p.segments + seg) * p.top;
+    auto put = [&](int rank, uint64_t key) { out[rank] = key; };
+    bool few = z == z;  // (NaN or infinities in the segment: no sum, and no plain order)
+    if (few) {
+        // candidates: values at or above the bar; with `ties` only values above it, and of those at it the ones within the first pieces
+        auto gather = [&](float at, bool ties) {
+#pragma unroll
+            for (int j = 0; j < LOADS; ++j) {
+                if (!__any(best[j] >= at)) continue;
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const float x = piece_value<BYTES>(v[j], e);
+                    const bool tie = x == at;
+                    if (inside(j, e) && (ties ? x > at || (tie && j == 0 && tid <= p.top) : x >= at)) {
+                        const int n = atomicAdd(&lds_n[0], 1);
+                        if (n < kLpCandidates) lds_k[n] = pair_key(x, index(j, e));
+                        if (ties && tie) atomicAdd(&lds_n[1], 1);
+                    }
+                }
+            }
+            __syncthreads();
+        };
+        gather(key_value(bar), false);
+        int n = lds_n[0];
+        if (n > kLpCandidates) {  // the whole threshold, and ties at it by their place: a masked or constant segment
+            const uint32_t full = wave_kth(order_key(mine), p.top, 32);
+            __syncthreads();
+            if (lane == 0) lds_t[wave] = full;
+            if (tid < 2) lds_n[tid] = 0;
+            __syncthreads();
+            bar = max(lds_t[0], kLowestKey);
+#pragma unroll
+            for (int w = 1; w < kLpWaves; ++w) bar = max(bar, lds_t[w]);
+            gather(key_value(bar), true);
+            n = lds_n[0];
+            few = n <= kLpCandidates && lds_n[1] >= p.top;
+        }
+        if (few) rank_keys(lds_k, n, p.top, put);
     }
-    // the k best: every thread offers the best of its elements that are below the last winner
-    uint64_t last = ~0ull, mine = 0;
+    if (few) return;
+    // winner by winner: every thread offers the best of its elements that are below the last winner
+    uint64_t last = ~0ull, offer = 0;
     bool stale = true;
+    __syncthreads();
     for (int k = 0; k < p.top; ++k) {
         if (stale) {
-            mine = 0;
+            offer = 0;
 #pragma unroll
-            for (int j = 0; j < kLpLoads; ++j)
+            for (int j = 0; j < LOADS; ++j)
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     const uint64_t key = pair_key(piece_value<BYTES>(v[j], e), index(j, e));
-                    if (inside(j, e) && key < last && key > mine) mine = key;
+                    if (inside(j, e) && key < last && key > offer) offer = key;
                 }
         }
-        last = block_max_key(mine, lds_k);
-        stale = mine == last;
-        if (tid == 0) p.keys[(row * p.segments + seg) * p.top + k] = last;  // 0: the segment has fewer elements
+        last = block_max_key(offer, lds_k);
+        stale = offer == last;
+        if (tid == 0) out[k] = last;  // 0: the segment has fewer elements
     }
 }
 
 __global__ __launch_bounds__(kLpThreads) void logprob_row_kernel(LogprobParams p, int bytes) {
-    __shared__ uint64_t lds_k[kLpThreads / 64];
+    __shared__ uint64_t lds_k[kLpCandidates];
+    __shared__ uint32_t lds_t;
+    __shared__ int lds_n;
     const int64_t row = blockIdx.x;
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63;
     const SegmentStats* st = p.stats + row * p.segments;
+    // every wave folds the sums for itself, a segment per lane
     double ref = -INFINITY;
-    for (int s = 0; s < p.segments; ++s) ref = st[s].z > 0.f && st[s].ref > ref ? st[s].ref : ref;
+    for (int s = lane; s < p.segments; s += 64) ref = st[s].z > 0.f && st[s].ref > ref ? st[s].ref : ref;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) ref = fmax(ref, __shfl_xor(ref, d));
     float z = 0.f, t = 0.f;
-    for (int s = 0; s < p.segments; ++s) {
-        if (st[s].z == 0.f) continue;
-        const float d = (float)(st[s].ref - ref);
+    for (int s = lane; s < p.segments; s += 64) {
+        const SegmentStats e = st[s];
+        if (e.z == 0.f) continue;
+        const float d = (float)(e.ref - ref);
         const float f = fast_exp2(d * kLog2e);
-        z += f * st[s].z;
-        t += f * (st[s].t + fmaxf(d, -200.f) * st[s].z);
+        z += f * e.z;
+        t += f * (e.t + fmaxf(d, -200.f) * e.z);
     }
+    z = wave_sum(z), t = wave_sum(t);
     if (z == 0.f) z = __builtin_nanf("");  // no element above -inf
     const double lnz = (double)logf(z);
     if (tid == 0) {
@@ -184,24 +282,53 @@ __global__ __launch_bounds__(kLpThreads) void logprob_row_kernel(LogprobParams p
         p.logprobs[row] = (float)(((double)x - ref) - lnz);
         p.entropy[row] = logf(z) - t / z;
     }
+    if (p.top == 0) return;
     const uint64_t* keys = p.keys + row * p.segments * p.top;
-    uint64_t last = ~0ull;
+    auto put = [&](int rank, uint64_t key) {
+        p.top_ids[row * p.top + rank] = (int32_t)~(uint32_t)key;
+        p.top_logprobs[row * p.top + rank] = (float)(((double)key_value((uint32_t)(key >> 32)) - ref) - lnz);
+    };
+    // the k-th largest of the segments' best keys bounds the k-th largest of all from below (fewer segments than k: no bound)
+    if (tid < 64) {
+        uint32_t best = 0;
+        for (int s = lane; s < p.segments; s += 64) best = max(best, (uint32_t)(keys[(int64_t)s * p.top] >> 32));
+        const uint32_t bar = wave_kth(best, p.top, 32);
+        if (lane == 0) lds_t = bar, lds_n = 0;
+    }
+    __syncthreads();
+    const uint32_t bar = lds_t;
+    for (int i = tid; i < p.segments * p.top; i += kLpThreads) {
+        const uint64_t key = keys[i];
+        if (key != 0 && (uint32_t)(key >> 32) >= bar) {
+            const int n = atomicAdd(&lds_n, 1);
+            if (n < kLpCandidates) lds_k[n] = key;
+        }
+    }
+    __syncthreads();
+    if (lds_n <= kLpCandidates) {
+        rank_keys(lds_k, lds_n, p.top, put);
+        return;
+    }
+    __syncthreads();
+    uint64_t last = ~0ull;  // very long rows of ties: winner by winner
     for (int k = 0; k < p.top; ++k) {
-        uint64_t mine = 0;
+        uint64_t offer = 0;
         for (int i = tid; i < p.segments * p.top; i += kLpThreads) {
             const uint64_t key = keys[i];
-            if (key < last && key > mine) mine = key;
+            if (key < last && key > offer) offer = key;
         }
-        last = block_max_key(mine, lds_k);
-        if (tid == 0) {
-            p.top_ids[row * p.top + k] = (int32_t)~(uint32_t)last;
-            p.top_logprobs[row * p.top + k] = (float)(((double)key_value((uint32_t)(last >> 32)) - ref) - lnz);
-        }
+        last = block_max_key(offer, lds_k);
+        if (tid == 0) put(k, last);
     }
 }
 
-static int logprob_segments(int vocab, int bytes) {
-    const int64_t per = (int64_t)kLpPieces * (16 / bytes);
+// Pieces per thread: eight keep the most bytes in flight per group; two where eight would leave compute units without a segment.
+static int logprob_loads(int rows, int vocab, int bytes) {
+    const int64_t pieces = ((int64_t)vocab * bytes + 15) / 16;
+    return (int64_t)rows * ((pieces + 8 * kLpThreads - 1) / (8 * kLpThreads)) < device_cus() ? 2 : 8;
+}
+static int logprob_segments(int rows, int vocab, int bytes) {
+    const int64_t per = (int64_t)kLpThreads * logprob_loads(rows, vocab, bytes) * (16 / bytes);
     return (int)(((int64_t)vocab + 16 / bytes - 1 + per - 1) / per);  // (a row's first piece may begin up to E - 1 elements early)
 }
 
@@ -211,7 +338,7 @@ using namespace msgl;
 
 extern "C" size_t msgl_token_logprobs_workspace_bytes(int rows, int vocab, int elem_bytes, int top) {
     if (rows <= 0 || vocab <= 0 || (elem_bytes != 2 && elem_bytes != 4) || top < 0) return 0;
-    return (size_t)rows * logprob_segments(vocab, elem_bytes) * (sizeof(SegmentStats) + (size_t)top * sizeof(uint64_t));
+    return (size_t)rows * logprob_segments(rows, vocab, elem_bytes) * (sizeof(SegmentStats) + (size_t)top * sizeof(uint64_t));
 }
 
 extern "C" int msgl_token_logprobs(const void* logits, int64_t row_stride, int elem_bytes, const int32_t* token_ids, float* logprobs,
@@ -226,7 +353,7 @@ extern "C" int msgl_token_logprobs(const void* logits, int64_t row_stride, int e
     MSGL_REQUIRE(((uintptr_t)logits & (elem_bytes - 1)) == 0 && row_stride >= 0, "msgl_token_logprobs: misaligned logits or row_stride %lld",
                  (long long)row_stride);
     LogprobParams p;
-    p.segments = logprob_segments(vocab, elem_bytes);
+    p.segments = logprob_segments(rows, vocab, elem_bytes);
     MSGL_REQUIRE((int64_t)rows * p.segments <= 0x7fffffff, "msgl_token_logprobs: %d rows x %d segments", rows, p.segments);
     const size_t need = msgl_token_logprobs_workspace_bytes(rows, vocab, elem_bytes, top);
     if (workspace == nullptr || workspace_bytes < need) {
@@ -241,8 +368,11 @@ extern "C" int msgl_token_logprobs(const void* logits, int64_t row_stride, int e
     p.vocab = vocab, p.top = top;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const dim3 grid((unsigned)(rows * p.segments));
-    if (elem_bytes == 2) hipLaunchKernelGGL(logprob_segment_kernel<2>, grid, dim3(kLpThreads), 0, st, p);
-    else hipLaunchKernelGGL(logprob_segment_kernel<4>, grid, dim3(kLpThreads), 0, st, p);
+    const bool eight = logprob_loads(rows, vocab, elem_bytes) == 8;
+    if (elem_bytes == 2 && eight) hipLaunchKernelGGL((logprob_segment_kernel<2, 8>), grid, dim3(kLpThreads), 0, st, p);
+    else if (elem_bytes == 2) hipLaunchKernelGGL((logprob_segment_kernel<2, 2>), grid, dim3(kLpThreads), 0, st, p);
+    else if (eight) hipLaunchKernelGGL((logprob_segment_kernel<4, 8>), grid, dim3(kLpThreads), 0, st, p);
+    else hipLaunchKernelGGL((logprob_segment_kernel<4, 2>), grid, dim3(kLpThreads), 0, st, p);
     hipLaunchKernelGGL(logprob_row_kernel, dim3((unsigned)rows), dim3(kLpThreads), 0, st, p, elem_bytes);
     return check_launch("token_logprobs kernels");
 }

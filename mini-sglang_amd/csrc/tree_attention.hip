@@ -17,8 +17,6 @@
 //   * The page table is read per token, also by LDS-DMA, four tiles ahead: any page size, no scalar path, nothing the compiler counts.
 //   * All these loads are inline asm and waited for by count; their order is K0 V0 t3 K1 V1 | t4 K2 V2 | t5 K3 V3 ... (t = table entries).
 // Long contexts are cut into runs of keys (one work group each) that leave (O, max, sum) in the workspace; a second kernel joins them.
-#include <stdlib.h>
-
 #include <type_traits>
 #include <utility>
 
@@ -32,7 +30,6 @@ constexpr int kTreeKeys = 32;                       // keys per tile
 constexpr int kTreeHalf = kTreeKeys * kHD * 2;      // bytes of a K or V tile
 constexpr int kTreeRing = 4 * kTreeHalf;            // per wave: two K tiles, two V tiles
 constexpr int kTreeSlotRing = 4 * 256;              // per wave: table entries of four tiles (64 words each)
-constexpr int kTreeLds = kTreeWaves * (kTreeRing + kTreeSlotRing);
 constexpr int kTreeMergeRow = kHD + 4;              // floats per row of the exchange at the end (spread over the banks)
 constexpr int merge_bytes(int waves, int rb) { return waves * 32 * rb * (kTreeMergeRow + 2) * 4; }
 constexpr float kRescaleAt = 8.f;                   // log2 units a row's maximum may outgrow its reference before O is rescaled
@@ -54,7 +51,7 @@ struct TreeParams {
     int64_t out_stride;
     float* ws_o;   // [token][head][split][128]
     float* ws_ml;  // [token][head][split][2]
-    int Hq, Hkv, group;
+    int bs, Hq, Hkv, group;
     int items, row_tiles, splits, chunk;
     int max_q;
     float scale_log2e;
@@ -390,23 +387,19 @@ __device__ __forceinline__ void join_and_store(const TreeParams& p, const TreeIt
     }
 }
 
-// HPB kv heads per work group, 4 / HPB waves per head.
-template <int RB, int HPB>
+template <int RB>
 __global__ __launch_bounds__(kTreeWaves * 64, 1) void tree_attention_kernel(TreeParams p) {
-    constexpr int WPH = kTreeWaves / HPB;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
-    // block -> (group of heads, run of keys, request), heads fastest: the token rows' pieces are read at about the same time
-    const int hgroups = p.Hkv / HPB;
-    const int hg = blockIdx.x % (unsigned)hgroups;
-    const int id = blockIdx.x / (unsigned)hgroups;
+    // block -> (kv head, run of keys, request), heads fastest: a token row's pieces are read at about the same time
+    const int h = blockIdx.x % (unsigned)p.Hkv;
+    const int id = blockIdx.x / (unsigned)p.Hkv;
     const TreeItem it = tree_item(p, id / p.splits, id % p.splits, 0);
     if (it.none) return;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int h = hg * HPB + wave / WPH, sub = wave % WPH;
     const int g4 = lane >> 4, q16 = lane & 15;
     const int all_tiles = (it.t1 - it.t0 + kTreeKeys - 1) / kTreeKeys;
-    const int T = all_tiles > sub ? (all_tiles - sub + WPH - 1) / WPH : 0;  // own tiles: sub, sub + WPH, ...
+    const int T = all_tiles > wave ? (all_tiles - wave + kTreeWaves - 1) / kTreeWaves : 0;  // own tiles: wave, wave + kTreeWaves, ...
 
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
     char* ring = smem + wave * kTreeRing;
@@ -417,14 +410,14 @@ __global__ __launch_bounds__(kTreeWaves * 64, 1) void tree_attention_kernel(Tree
     TreeState<RB> st;
     st.clear();
     uint64_t odd = 0;  // tiles behind the plain ones that held a value that is not finite
-    const int plain = (max(0, (min(it.prefix, it.t1) - it.t0) / kTreeKeys - sub) + WPH - 1) / WPH;  // own tiles that every row sees whole
+    const int plain = (max(0, (min(it.prefix, it.t1) - it.t0) / kTreeKeys - wave) + kTreeWaves - 1) / kTreeWaves;  // own tiles that every row sees whole
     if (T > 0) {
         const int32_t* table = p.r2t + (int64_t)p.req_idx[it.b] * p.r2t_stride;
         // table entries of own tile j, lane (g4', i) <- key 4 i + g4' of the tile, so that a lane of the K/V loads finds its eight rows'
         // entries in 32 consecutive bytes.  Positions behind the run's last key repeat that key.
         const int word_key = 4 * (lane & 7) + ((lane >> 3) & 3);
         auto issue_words = [&](int j) {
-            const int pos = min(it.t0 + (sub + j * WPH) * kTreeKeys + word_key, it.t1 - 1);
+            const int pos = min(it.t0 + (wave + j * kTreeWaves) * kTreeKeys + word_key, it.t1 - 1);
             dma_words((uint64_t)(table + pos), words_at + (j & 3) * 256);
         };
         issue_words(0);
@@ -487,7 +480,7 @@ __global__ __launch_bounds__(kTreeWaves * 64, 1) void tree_attention_kernel(Tree
             f32x16_t s[RB];
             bf16x8_t pf[RB][2];
             keys_of(j, s);
-            tile_mask<RB>(p, it, 0, it.t0 + (sub + j * WPH) * kTreeKeys, lane, s);
+            tile_mask<RB>(p, it, 0, it.t0 + (wave + j * kTreeWaves) * kTreeKeys, lane, s);
             tile_reference<RB>(p.scale_log2e, s, st);
             tile_probabilities<RB>(p.scale_log2e, s, st, pf);
             if (tile_values_masked<RB>(wait_values(j), lane, pf, st)) odd |= 1ull << (j - plain);
@@ -495,8 +488,8 @@ __global__ __launch_bounds__(kTreeWaves * 64, 1) void tree_attention_kernel(Tree
         }
     }
     wait_loads<0>();
-    join_and_store<RB, WPH, kTreeWaves>(p, it, st, smem, wave, lane, odd, it.t0 + (sub + plain * WPH) * kTreeKeys, WPH * kTreeKeys, [](int) { return 0; },
-                            [&](int g) { return hg * HPB + g; });
+    join_and_store<RB, kTreeWaves, kTreeWaves>(p, it, st, smem, wave, lane, odd, it.t0 + (wave + plain * kTreeWaves) * kTreeKeys, kTreeWaves * kTreeKeys, [](int) { return 0; },
+                            [&](int) { return h; });
 }
 
 // More than 64 rows per kv head: the NW waves hold 32 rows each and share the tiles, so that K and V are read once per 32 NW rows.  A tile is loaded by
@@ -732,35 +725,74 @@ __global__ __launch_bounds__(NW * 64, 2) void tree_attention_wide_kernel(TreePar
     join_and_store<1, 1, NW>(p, it, st, smem, wave, lane, odd, it.t0 + plain * kTreeKeys, kTreeKeys, [&](int g) { return it.r0 + g * 32; }, [&](int) { return h; });
 }
 
-// Joins the runs of one (token, head) per wave: two dims per lane.
+// Joins the runs of a (token, head): GROUPS half-waves per row take every GROUPS-th run, four dims per lane, and meet in LDS.
+template <int GROUPS>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeParams p) {
-    const int lane = threadIdx.x & 63;
+    __shared__ float lds[8][kHD + 2];
+    const int lane = threadIdx.x & 31, hw = threadIdx.x >> 5;
+    const int g = hw % GROUPS;
     const int per = p.max_q * p.Hq;  // (node, head) pairs of a request
-    const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int64_t id = (int64_t)blockIdx.x * (8 / GROUPS) + hw / GROUPS;
     const int b = (int)(id / per);
     const int r = (int)(id - (int64_t)b * per);
-    const int base = p.cu[b];
-    const int n = min(p.cu[b + 1] - base, p.max_q);
-    const int node = r / p.Hq, hq = r - node * p.Hq;
-    if (node >= n) return;
-    const int S = p.prefix[b] + n;
-    const int nsplit = min((S + p.chunk - 1) / p.chunk, p.splits);
-    if (nsplit <= 1) return;  // written by the first kernel
-    const int64_t at = ((int64_t)(base + node) * p.Hq + hq) * p.splits;
-    float M = kNegBigE;
-    for (int s = lane; s < nsplit; s += 64) M = fmaxf(M, p.ws_ml[(at + s) * 2]);
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) M = fmaxf(M, __shfl_xor(M, d));
-    float L = 0.f, o0 = 0.f, o1 = 0.f;
-    for (int s = 0; s < nsplit; ++s) {
-        const float2 ml = *reinterpret_cast<const float2*>(p.ws_ml + (at + s) * 2);
-        const float2 o = *reinterpret_cast<const float2*>(p.ws_o + (at + s) * kHD + 2 * lane);
-        const float f = fast_exp2(ml.x - M);
-        L += f * ml.y;
-        o0 += f * o.x, o1 += f * o.y;
+    int base = 0, n = 0, nsplit = 0;
+    if (b < p.bs) {
+        base = p.cu[b];
+        n = min(p.cu[b + 1] - base, p.max_q);
+        nsplit = min((p.prefix[b] + n + p.chunk - 1) / p.chunk, p.splits);
     }
+    const int node = r / p.Hq, hq = r - node * p.Hq;
+    const bool live = node < n && nsplit > 1;  // (one run: written by the first kernel)
+    const int64_t at = ((int64_t)(base + node) * p.Hq + hq) * p.splits;
+    float M = kNegBigE, L = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (live) {
+        for (int s0 = g; s0 < nsplit; s0 += 4 * GROUPS) {  // four runs' loads under way at a time
+            float2 ml[4];
+            float4 o[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int s = min(s0 + k * GROUPS, nsplit - 1);
+                ml[k] = *reinterpret_cast<const float2*>(p.ws_ml + (at + s) * 2);
+                o[k] = *reinterpret_cast<const float4*>(p.ws_o + (at + s) * kHD + 4 * lane);
+            }
+            float top = M;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) top = fmaxf(top, ml[k].x);
+            const float f0 = fast_exp2(M - top);
+            M = top;
+            L *= f0, acc.x *= f0, acc.y *= f0, acc.z *= f0, acc.w *= f0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float f = s0 + k * GROUPS < nsplit ? fast_exp2(ml[k].x - M) : 0.f;
+                L += f * ml[k].y;
+                if (f != 0.f) acc.x += f * o[k].x, acc.y += f * o[k].y, acc.z += f * o[k].z, acc.w += f * o[k].w;
+            }
+        }
+    }
+    if (GROUPS > 1) {
+        *reinterpret_cast<float2*>(&lds[hw][4 * lane]) = make_float2(acc.x, acc.y);
+        *reinterpret_cast<float2*>(&lds[hw][4 * lane + 2]) = make_float2(acc.z, acc.w);
+        if (lane == 0) lds[hw][kHD] = M, lds[hw][kHD + 1] = L;
+        __syncthreads();
+        if (g != 0) return;
+        float top = kNegBigE;
+#pragma unroll
+        for (int k = 0; k < GROUPS; ++k) top = fmaxf(top, lds[hw + k][kHD]);
+        L = 0.f;
+        acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < GROUPS; ++k) {
+            const float f = fast_exp2(lds[hw + k][kHD] - top);
+            L += f * lds[hw + k][kHD + 1];
+            acc.x += f * lds[hw + k][4 * lane], acc.y += f * lds[hw + k][4 * lane + 1];
+            acc.z += f * lds[hw + k][4 * lane + 2], acc.w += f * lds[hw + k][4 * lane + 3];
+        }
+    }
+    if (!live) return;
     const float inv = L == 0.f ? 0.f : 1.0f / L;
-    *reinterpret_cast<uint32_t*>(p.out + (int64_t)(base + node) * p.out_stride + hq * kHD + 2 * lane) = pack_bf16(o0 * inv, o1 * inv);
+    *reinterpret_cast<uint2*>(p.out + (int64_t)(base + node) * p.out_stride + hq * kHD + 4 * lane) =
+        make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
 }
 
 // Kernels that need more than the 64 KiB of LDS a kernel gets by default.
@@ -773,11 +805,11 @@ static int launch_tree(K kernel, PerDeviceOnce& once, int lds, int waves, const 
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(waves * 64), lds, stream, p);
     return check_launch("tree_attention_kernel");
 }
-template <int RB, int HPB>
+template <int RB>
 static int launch_narrow(const TreeParams& p, int64_t blocks, hipStream_t stream) {
+    constexpr int kTiles = kTreeWaves * (kTreeRing + kTreeSlotRing), kJoin = merge_bytes(kTreeWaves, RB);
     static PerDeviceOnce once;
-    return launch_tree(&tree_attention_kernel<RB, HPB>, once, kTreeLds > merge_bytes(kTreeWaves, RB) ? kTreeLds : merge_bytes(kTreeWaves, RB), kTreeWaves, p,
-                       blocks, stream);
+    return launch_tree(&tree_attention_kernel<RB>, once, kTiles > kJoin ? kTiles : kJoin, kTreeWaves, p, blocks, stream);
 }
 template <int NW, bool NT>
 static int launch_wide(const TreeParams& p, int64_t blocks, hipStream_t stream) {
@@ -791,7 +823,7 @@ constexpr int kMaxTreeSplits = 256;
 // share the keys.
 struct TreeShape {
     int waves;  // 0: the narrow kernel
-    int rb, row_tiles, hpb;
+    int rb, row_tiles;
 };
 static TreeShape tree_shape(int max_q, int Hq, int Hkv) {
     const int64_t rows = (int64_t)max_q * (Hq / Hkv);
@@ -799,17 +831,18 @@ static TreeShape tree_shape(int max_q, int Hq, int Hkv) {
     s.waves = rows <= 64 ? 0 : rows <= 128 ? 4 : 8;
     s.rb = rows > 32 && rows <= 64 ? 2 : 1;
     s.row_tiles = s.waves ? (int)((rows + 32 * s.waves - 1) / (32 * s.waves)) : 1;
-    s.hpb = 1; if (!s.waves && getenv("TREE_HPB")) { s.hpb = atoi(getenv("TREE_HPB")); if (s.hpb > Hkv) s.hpb = 1; }
     return s;
 }
 
-// Runs of keys per request: enough work groups for the chip, each at least four tiles (one per wave) long.
+// Runs of keys per request: about one work group per compute unit in all, each run at least four tiles long.  More runs even out unequal requests
+// but cost partial results: measured with 16 requests of 2000 to 4000 tokens x 16 nodes (32 / 8 heads) 61, 67, 84, 111 us at one, two, four and eight
+// groups per unit, 64 requests of 4096 to 8192 x 8 nodes 285, 308, 315, 339 us, 2 x 32 nodes x 130001 tokens (8 / 1 heads) 60, 87 us at one and two.
 static int tree_splits(int bs, int max_q, int max_k, int64_t total_kv, int Hq, int Hkv) {
     if (bs <= 0 || max_q <= 0 || max_k <= 0 || Hkv <= 0 || Hq < Hkv) return 1;
     const TreeShape sh = tree_shape(max_q, Hq, Hkv);
     const int64_t keys = total_kv > 0 && total_kv < (int64_t)bs * max_k ? total_kv : (int64_t)bs * max_k;
-    const int64_t per_key = (int64_t)(Hkv / sh.hpb) * sh.row_tiles;
-    const int64_t want = (sh.waves == 8 ? 1 : 2) * (int64_t)device_cus();
+    const int64_t per_key = (int64_t)Hkv * sh.row_tiles;
+    const int64_t want = device_cus();
     int64_t chunk = (keys * per_key + want - 1) / want;
     if (chunk < kTreeKeys * kTreeWaves) chunk = kTreeKeys * kTreeWaves;
     int64_t splits = (max_k + chunk - 1) / chunk;
@@ -854,7 +887,7 @@ extern "C" int msgl_tree_attention(const void* q, int64_t q_stride, const void* 
     p.r2t = req_to_token, p.r2t_stride = r2t_stride, p.req_idx = req_pool_indices, p.cu = cu_seqlens_q, p.prefix = prefix_lens;
     p.mask = tree_mask, p.words = mask_words;
     p.out = static_cast<uint16_t*>(out), p.out_stride = out_stride;
-    p.Hq = Hq, p.Hkv = Hkv, p.group = Hq / Hkv, p.max_q = max_seqlen_q;
+    p.bs = bs, p.Hq = Hq, p.Hkv = Hkv, p.group = Hq / Hkv, p.max_q = max_seqlen_q;
     const TreeShape sh = tree_shape(max_seqlen_q, Hq, Hkv);
     p.row_tiles = sh.row_tiles;
     p.scale_log2e = scale * 1.44269504088896340736f;
@@ -868,7 +901,7 @@ extern "C" int msgl_tree_attention(const void* q, int64_t q_stride, const void* 
     p.ws_o = static_cast<float*>(workspace);
     p.ws_ml = p.ws_o + (splits > 1 ? (size_t)total_tokens * Hq * splits * kHD : 0);
     MSGL_REQUIRE(splits == 1 || aligned16(workspace), "msgl_tree_attention: workspace must be 16-byte aligned");
-    const int64_t items = (int64_t)bs * splits * (Hkv / sh.hpb);
+    const int64_t items = (int64_t)bs * splits * Hkv;
     const int64_t blocks = sh.waves ? (items + 7) / 8 * 8 * p.row_tiles : items;
     MSGL_REQUIRE(blocks <= 0x7fffffff, "msgl_tree_attention: %lld work groups", (long long)blocks);
     p.items = (int)items;
@@ -878,13 +911,14 @@ extern "C" int msgl_tree_attention(const void* q, int64_t q_stride, const void* 
         const bool once = p.row_tiles == 1;  // K and V are read by one work group: past the caches
         if (sh.waves == 4) rc = once ? launch_wide<4, true>(p, blocks, st) : launch_wide<4, false>(p, blocks, st);
         else rc = once ? launch_wide<8, true>(p, blocks, st) : launch_wide<8, false>(p, blocks, st);
-    } else if (sh.rb == 1) {
-        rc = sh.hpb == 4 ? launch_narrow<1, 4>(p, blocks, st) : sh.hpb == 2 ? launch_narrow<1, 2>(p, blocks, st) : launch_narrow<1, 1>(p, blocks, st);
     } else {
-        rc = sh.hpb == 4 ? launch_narrow<2, 4>(p, blocks, st) : sh.hpb == 2 ? launch_narrow<2, 2>(p, blocks, st) : launch_narrow<2, 1>(p, blocks, st);
+        rc = sh.rb == 1 ? launch_narrow<1>(p, blocks, st) : launch_narrow<2>(p, blocks, st);
     }
     if (rc != MSGL_OK || splits == 1) return rc;
-    const int64_t waves = (int64_t)bs * max_seqlen_q * Hq;
-    hipLaunchKernelGGL(tree_merge_kernel, dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, st, p);
+    // half-waves per row: as many as there are runs for, up to eight
+    const int64_t rows = (int64_t)bs * max_seqlen_q * Hq;
+    if (splits <= 8) hipLaunchKernelGGL(tree_merge_kernel<1>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, p);
+    else if (splits <= 32) hipLaunchKernelGGL(tree_merge_kernel<4>, dim3((unsigned)((rows + 1) / 2)), dim3(256), 0, st, p);
+    else hipLaunchKernelGGL(tree_merge_kernel<8>, dim3((unsigned)rows), dim3(256), 0, st, p);
     return check_launch("tree_merge_kernel");
 }
