@@ -12,6 +12,8 @@
 // that reach it (in every wave's view: the largest of the four) are all that has to be ranked.  The k-th largest lane maximum comes from
 // bisecting its bits with ballots.  Segments where that leaves too many (long ties that are not a fill from the segment's start on, NaN,
 // infinities) are taken apart winner by winner instead.
+#include <type_traits>
+
 #include "extend_common.h"
 #include "msgl_common.h"
 
@@ -19,8 +21,9 @@ namespace msgl {
 
 constexpr int kLpThreads = 256;
 constexpr int kLpWaves = kLpThreads / 64;
-constexpr int kLpCandidates = 1024;
+constexpr int kLpCandidates = 256;  // per wave
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
+constexpr double kLn2d = 0.693147180559945309417;
 
 struct SegmentStats {
     double ref;  // natural units: e = exp(x - ref)
@@ -88,17 +91,55 @@ __device__ __forceinline__ uint32_t wave_kth(uint32_t key, int k, int bits) {
     return t;
 }
 
-// Ranks `count` distinct keys and hands the `top` largest to put(rank, key); the places behind the last one get 0.
-template <typename Put>
-__device__ __forceinline__ void rank_keys(const uint64_t* keys, int count, int top, Put put) {
-    for (int i = threadIdx.x; i < count; i += kLpThreads) {
-        const uint64_t mine = keys[i];
-        int rank = 0;
-        for (int j = 0; j < count; ++j) rank += keys[j] > mine;
-        if (rank < top) put(rank, mine);
+// Candidates: a list per wave, zeros behind its end up to the next eight.
+struct Candidates {
+    uint64_t key[kLpWaves][kLpCandidates + 8];
+    int count[kLpWaves];
+    // Appends the lanes' keys where `take`, in lane order; n: the wave's count so far.  What does not fit is counted only.
+    __device__ __forceinline__ void append(int& n, bool take, uint64_t k) {
+        const uint64_t who = __ballot(take);
+        const int place = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+        if (take && place < kLpCandidates) key[threadIdx.x >> 6][place] = k;
+        n += __popcll(who);
     }
-    for (int i = count + threadIdx.x; i < top; i += kLpThreads) put(i, 0);
-}
+    // Ends the wave's list; true if every wave's list fits.
+    __device__ __forceinline__ bool close(int n) {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        if (lane < 8 && n <= kLpCandidates) key[wave][n + lane] = 0;
+        if (lane == 0) count[wave] = n;
+        __syncthreads();
+        int most = 0;
+#pragma unroll
+        for (int w = 0; w < kLpWaves; ++w) most = max(most, count[w]);
+        return most <= kLpCandidates;
+    }
+    // Hands the `top` largest (all distinct) to put(rank, key); the places behind the last one get 0.  Four lanes count for a key, a list each.
+    template <typename Put>
+    __device__ __forceinline__ void rank(int top, Put put) {
+        static_assert(kLpWaves == 4, "a lane of four per list");
+        int n[kLpWaves], total = 0;
+#pragma unroll
+        for (int w = 0; w < kLpWaves; ++w) n[w] = count[w], total += n[w];
+        const int list = threadIdx.x & 3;
+        const uint64_t* mine = key[list];
+        const int length = n[list];
+        for (int i = threadIdx.x >> 2; i < total; i += kLpThreads / 4) {
+            int at = i, w = 0;
+#pragma unroll
+            for (int k = 0; k < kLpWaves - 1; ++k)
+                if (w == k && at >= n[k]) at -= n[k], w = k + 1;
+            const uint64_t x = key[w][at];
+            int above = 0;
+            for (int j = 0; j < length; j += 8)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) above += mine[j + k] > x;
+            above += __shfl_xor(above, 1);
+            above += __shfl_xor(above, 2);
+            if (list == 0 && above < top) put(above, x);
+        }
+        for (int i = total + threadIdx.x; i < top; i += kLpThreads) put(i, 0);
+    }
+};
 
 // element e of a 16-byte piece
 template <int BYTES>
@@ -114,8 +155,8 @@ __global__ __launch_bounds__(kLpThreads) void logprob_segment_kernel(LogprobPara
     constexpr int kPieces = kLpThreads * LOADS;       // pieces per segment
     __shared__ float lds_f[kLpWaves][2];
     __shared__ uint32_t lds_t[kLpWaves];
-    __shared__ uint64_t lds_k[kLpCandidates];
-    __shared__ int lds_n[2];
+    __shared__ Candidates found;
+    __shared__ int lds_ties[kLpWaves];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t row = blockIdx.x / (unsigned)p.segments;
     const int seg = blockIdx.x - (unsigned)row * (unsigned)p.segments;
@@ -135,7 +176,6 @@ __global__ __launch_bounds__(kLpThreads) void logprob_segment_kernel(LogprobPara
         v[j] = make_uint4(none, none, none, none);
         if (g < pieces) v[j] = *reinterpret_cast<const uint4*>(base + (int64_t)g * 16);
     }
-    if (tid < 2) lds_n[tid] = 0;
 #pragma unroll
     for (int j = 0; j < LOADS; ++j) {  // the row's first and last piece
         if (inside(j, 0) && inside(j, E - 1)) continue;
@@ -168,15 +208,23 @@ __global__ __launch_bounds__(kLpThreads) void logprob_segment_kernel(LogprobPara
     for (int w = 1; w < kLpWaves; ++w) m = fmaxf(m, lds_f[w][0]), bar = max(bar, lds_t[w]);
     const float ref = m == -INFINITY ? 0.f : m;  // nothing but -inf here: every e is 0 (or NaN)
     float z = 0.f, t = 0.f;
+    auto add = [&](auto log2_of) {
 #pragma unroll
-    for (int j = 0; j < LOADS; ++j)
+        for (int j = 0; j < LOADS; ++j)
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const float d = (piece_value<BYTES>(v[j], e) - ref) * kLog2e;
-            const float x = fast_exp2(d);
-            z += x;
-            t += x * fmaxf(d, -200.f);  // 2^-200 is 0 in 32 bits: -inf and the like add 0, not 0 * inf
-        }
+            for (int e = 0; e < E; ++e) {
+                const float d = log2_of(piece_value<BYTES>(v[j], e));
+                const float x = fast_exp2(d);
+                z += x;
+                t += x * fmaxf(d, -200.f);  // 2^-200 is 0 in 32 bits: -inf and the like add 0, not 0 * inf
+            }
+    };
+    // (x - ref) log2 e as one multiply-add against a whole number near ref log2 e, itself the reference then; huge values (a mask's lowest value
+    // in every place) do not survive the multiplication and are subtracted first
+    const bool tame = fabsf(ref) < 1e5f;
+    const float ref2 = rintf(ref * kLog2e);
+    if (tame) add([&](float x) { return __builtin_fmaf(x, kLog2e, -ref2); });
+    else add([&](float x) { return (x - ref) * kLog2e; });
     z = wave_sum(z), t = wave_sum(t);
     __syncthreads();
     if (lane == 0) lds_f[wave][0] = z, lds_f[wave][1] = t;
@@ -184,7 +232,7 @@ __global__ __launch_bounds__(kLpThreads) void logprob_segment_kernel(LogprobPara
     z = t = 0.f;
 #pragma unroll
     for (int w = 0; w < kLpWaves; ++w) z += lds_f[w][0], t += lds_f[w][1];
-    if (tid == 0) p.stats[row * p.segments + seg] = SegmentStats{(double)ref, z, t * kLn2};
+    if (tid == 0) p.stats[row * p.segments + seg] = SegmentStats{tame ? (double)ref2 * kLn2d : (double)ref, z, t * kLn2};
     if (p.top == 0) return;
 
     uint64_t* out = p.keys + (row * p.segments + seg) * p.top;
@@ -192,39 +240,58 @@ __global__ __launch_bounds__(kLpThreads) void logprob_segment_kernel(LogprobPara
     bool few = z == z;  // (NaN or infinities in the segment: no sum, and no plain order)
     if (few) {
         // candidates: values at or above the bar; with `ties` only values above it, and of those at it the ones within the first pieces
-        auto gather = [&](float at, bool ties) {
+        auto gather = [&](float at, auto ties) {
+            int n = 0, tied = 0;  // of this wave
+            // bit j E + e: this lane's element e of piece j is one; taken lane by lane, a bit per turn, so that the key's arithmetic is paid for as
+            // often as the lane with the most has some, and not for every place in the pieces
+            uint32_t hits = 0;
 #pragma unroll
-            for (int j = 0; j < LOADS; ++j) {
-                if (!__any(best[j] >= at)) continue;
+            for (int j = LOADS - 1; j >= 0; --j)
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const float x = piece_value<BYTES>(v[j], e);
-                    const bool tie = x == at;
-                    if (inside(j, e) && (ties ? x > at || (tie && j == 0 && tid <= p.top) : x >= at)) {
-                        const int n = atomicAdd(&lds_n[0], 1);
-                        if (n < kLpCandidates) lds_k[n] = pair_key(x, index(j, e));
-                        if (ties && tie) atomicAdd(&lds_n[1], 1);
-                    }
+                for (int e = E - 1; e >= 0; --e) hits = hits << 1 | (piece_value<BYTES>(v[j], e) >= at ? 1u : 0u);
+            while (__any(hits != 0)) {
+                const int at_bit = hits ? __ffs(hits) - 1 : 0;
+                const bool one = hits != 0;
+                hits &= hits - 1;
+                const int j = at_bit / E, e = at_bit % E;
+                uint32_t w[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    w[c] = 0;
+#pragma unroll
+                    for (int k = 0; k < LOADS; ++k) w[c] = j == k ? (c == 0 ? v[k].x : c == 1 ? v[k].y : c == 2 ? v[k].z : v[k].w) : w[c];
                 }
+                const int c = BYTES == 4 ? e : e >> 1;
+                const uint32_t word = c == 0 ? w[0] : c == 1 ? w[1] : c == 2 ? w[2] : w[3];
+                const float x = BYTES == 4 ? __builtin_bit_cast(float, word) : e & 1 ? bf16_hi(word) : bf16_lo(word);
+                const int idx = (seg * kPieces + j * kLpThreads + tid) * E + e - lead;
+                bool take = one && (unsigned)idx < (unsigned)p.vocab;
+                if (ties) {
+                    const bool tie = x == at;
+                    take = take && (!tie || (j == 0 && tid <= p.top));
+                    tied += __popcll(__ballot(take && tie));
+                }
+                found.append(n, take, pair_key(x, idx));
             }
-            __syncthreads();
+            if (lane == 0) lds_ties[wave] = tied;
+            return found.close(n);
         };
-        gather(key_value(bar), false);
-        int n = lds_n[0];
-        if (n > kLpCandidates) {  // the whole threshold, and ties at it by their place: a masked or constant segment
+        few = gather(key_value(bar), std::false_type{});
+        if (!few) {  // the whole threshold, and ties at it by their place: a masked or constant segment
             const uint32_t full = wave_kth(order_key(mine), p.top, 32);
             __syncthreads();
             if (lane == 0) lds_t[wave] = full;
-            if (tid < 2) lds_n[tid] = 0;
             __syncthreads();
             bar = max(lds_t[0], kLowestKey);
 #pragma unroll
             for (int w = 1; w < kLpWaves; ++w) bar = max(bar, lds_t[w]);
-            gather(key_value(bar), true);
-            n = lds_n[0];
-            few = n <= kLpCandidates && lds_n[1] >= p.top;
+            few = gather(key_value(bar), std::true_type{});
+            int tied = 0;
+#pragma unroll
+            for (int w = 0; w < kLpWaves; ++w) tied += lds_ties[w];
+            few = few && tied >= p.top;
         }
-        if (few) rank_keys(lds_k, n, p.top, put);
+        if (few) found.rank(p.top, put);
     }
     if (few) return;
     // winner by winner: every thread offers the best of its elements that are below the last winner
@@ -242,16 +309,15 @@ __global__ __launch_bounds__(kLpThreads) void logprob_segment_kernel(LogprobPara
                     if (inside(j, e) && key < last && key > offer) offer = key;
                 }
         }
-        last = block_max_key(offer, lds_k);
+        last = block_max_key(offer, found.key[0]);
         stale = offer == last;
         if (tid == 0) out[k] = last;  // 0: the segment has fewer elements
     }
 }
 
 __global__ __launch_bounds__(kLpThreads) void logprob_row_kernel(LogprobParams p, int bytes) {
-    __shared__ uint64_t lds_k[kLpCandidates];
+    __shared__ Candidates found;
     __shared__ uint32_t lds_t;
-    __shared__ int lds_n;
     const int64_t row = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63;
     const SegmentStats* st = p.stats + row * p.segments;
@@ -288,25 +354,25 @@ __global__ __launch_bounds__(kLpThreads) void logprob_row_kernel(LogprobParams p
         p.top_ids[row * p.top + rank] = (int32_t)~(uint32_t)key;
         p.top_logprobs[row * p.top + rank] = (float)(((double)key_value((uint32_t)(key >> 32)) - ref) - lnz);
     };
-    // the k-th largest of the segments' best keys bounds the k-th largest of all from below (fewer segments than k: no bound)
+    // the k-th largest of some k or more of the keys bounds the k-th largest of all from below: of the segments' best ones, as many per
+    // segment as it takes
     if (tid < 64) {
+        const int per = (p.top + p.segments - 1) / p.segments;
         uint32_t best = 0;
-        for (int s = lane; s < p.segments; s += 64) best = max(best, (uint32_t)(keys[(int64_t)s * p.top] >> 32));
+        for (int i = lane; i < p.segments * per; i += 64) best = max(best, (uint32_t)(keys[(int64_t)(i / per) * p.top + i % per] >> 32));
         const uint32_t bar = wave_kth(best, p.top, 32);
-        if (lane == 0) lds_t = bar, lds_n = 0;
+        if (lane == 0) lds_t = bar;
     }
     __syncthreads();
     const uint32_t bar = lds_t;
-    for (int i = tid; i < p.segments * p.top; i += kLpThreads) {
-        const uint64_t key = keys[i];
-        if (key != 0 && (uint32_t)(key >> 32) >= bar) {
-            const int n = atomicAdd(&lds_n, 1);
-            if (n < kLpCandidates) lds_k[n] = key;
-        }
+    int n = 0;
+    for (int i0 = 0; i0 < p.segments * p.top; i0 += kLpThreads) {
+        const int i = i0 + tid;
+        const uint64_t key = i < p.segments * p.top ? keys[i] : 0;
+        found.append(n, key != 0 && (uint32_t)(key >> 32) >= bar, key);
     }
-    __syncthreads();
-    if (lds_n <= kLpCandidates) {
-        rank_keys(lds_k, lds_n, p.top, put);
+    if (found.close(n)) {
+        found.rank(p.top, put);
         return;
     }
     __syncthreads();
@@ -317,19 +383,21 @@ __global__ __launch_bounds__(kLpThreads) void logprob_row_kernel(LogprobParams p
             const uint64_t key = keys[i];
             if (key < last && key > offer) offer = key;
         }
-        last = block_max_key(offer, lds_k);
+        last = block_max_key(offer, found.key[0]);
         if (tid == 0) put(k, last);
     }
 }
 
-// Pieces per thread: eight keep the most bytes in flight per group; two where eight would leave compute units without a segment.
-static int logprob_loads(int rows, int vocab, int bytes) {
-    const int64_t pieces = ((int64_t)vocab * bytes + 15) / 16;
-    return (int64_t)rows * ((pieces + 8 * kLpThreads - 1) / (8 * kLpThreads)) < device_cus() ? 2 : 8;
+// Elements per thread: 32, or 16 where that would be fewer than four groups per compute unit.  Measured on a vocabulary of 151936 with five
+// alternatives, us with 16 / 32 / 64 elements per thread: one bf16 row 8.3 / 9.4 / 10.1, 32 rows 10.6 / 11.2 / 12.2, 64 rows 14.2 / 13.5 / 15.1, 1000 rows
+// 94 / 87 / 91; fp32 with 8 / 16 / 32: one row 8.8 / 8.7 / 8.9, 32 rows 13.9 / 11.8 / 12.1, 64 rows 18.3 / 16.1 / 15.6, 1000 rows 153 / 114 / 105.
+static int logprob_elements(int rows, int vocab) {
+    const int64_t segments = ((int64_t)vocab + 32 * kLpThreads - 1) / (32 * kLpThreads);
+    return rows * segments < 4 * (int64_t)device_cus() ? 16 : 32;
 }
 static int logprob_segments(int rows, int vocab, int bytes) {
-    const int64_t per = (int64_t)kLpThreads * logprob_loads(rows, vocab, bytes) * (16 / bytes);
-    return (int)(((int64_t)vocab + 16 / bytes - 1 + per - 1) / per);  // (a row's first piece may begin up to E - 1 elements early)
+    const int64_t per = (int64_t)kLpThreads * logprob_elements(rows, vocab);
+    return (int)(((int64_t)vocab + 16 / bytes - 1 + per - 1) / per);  // (a row's first piece may begin up to 16 / bytes - 1 elements early)
 }
 
 }  // namespace msgl
@@ -368,11 +436,11 @@ extern "C" int msgl_token_logprobs(const void* logits, int64_t row_stride, int e
     p.vocab = vocab, p.top = top;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const dim3 grid((unsigned)(rows * p.segments));
-    const bool eight = logprob_loads(rows, vocab, elem_bytes) == 8;
-    if (elem_bytes == 2 && eight) hipLaunchKernelGGL((logprob_segment_kernel<2, 8>), grid, dim3(kLpThreads), 0, st, p);
+    const bool most = logprob_elements(rows, vocab) == 32;
+    if (elem_bytes == 2 && most) hipLaunchKernelGGL((logprob_segment_kernel<2, 4>), grid, dim3(kLpThreads), 0, st, p);
     else if (elem_bytes == 2) hipLaunchKernelGGL((logprob_segment_kernel<2, 2>), grid, dim3(kLpThreads), 0, st, p);
-    else if (eight) hipLaunchKernelGGL((logprob_segment_kernel<4, 8>), grid, dim3(kLpThreads), 0, st, p);
-    else hipLaunchKernelGGL((logprob_segment_kernel<4, 2>), grid, dim3(kLpThreads), 0, st, p);
+    else if (most) hipLaunchKernelGGL((logprob_segment_kernel<4, 8>), grid, dim3(kLpThreads), 0, st, p);
+    else hipLaunchKernelGGL((logprob_segment_kernel<4, 4>), grid, dim3(kLpThreads), 0, st, p);
     hipLaunchKernelGGL(logprob_row_kernel, dim3((unsigned)rows), dim3(kLpThreads), 0, st, p, elem_bytes);
     return check_launch("token_logprobs kernels");
 }
