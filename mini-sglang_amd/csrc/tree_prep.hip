@@ -12,6 +12,8 @@
 
 namespace msgl {
 
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+
 struct ExtendPrepParams {
     const int32_t* req_idx;
     const int32_t* prefix;    // [bs] cached tokens
@@ -155,34 +157,26 @@ __global__ __launch_bounds__(256) void extend_prepare_fill_kernel(ExtendPrepPara
     p.out_loc[t] = place_token(p, rq, pos);
 }
 
-// Phase 2, trees: a wave per request; nodes in chunks of 64, a node per lane.  Inside a chunk the ancestors are collected by pointer
+// One request's tree, by one wave: nodes in chunks of 64, a node per lane.  Inside a chunk the ancestors are collected by pointer
 // doubling (a lane's pointer jumps to its pointer's pointer, collecting the nodes jumped over), so a chunk costs log2(depth) steps;
 // what lies in earlier chunks is the finished mask row of the first ancestor there.
-__global__ __launch_bounds__(256) void extend_prepare_tree_kernel(ExtendPrepParams p) {
+__device__ __forceinline__ void place_tree(const ExtendPrepParams& p, const int4 rq, int base, int n) {
     const int lane = threadIdx.x & 63;
-    const int b = blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int total = p.cu[p.bs];
-    for (int t = total + (blockIdx.x * 256 + threadIdx.x); t < p.capacity; t += gridDim.x * 256) {  // behind the last request
-        p.positions[t] = 0;
-        p.out_loc[t] = 0;
-        for (int w = 0; w < p.words; ++w) p.mask[(int64_t)t * p.words + w] = 0;
-    }
-    if (b >= p.bs) return;
-    const int base = p.cu[b];
-    const int n = min(p.cu[b + 1] - base, p.words * 64);
-    const int4 rq = p.scratch[b];
     for (int c = 0; c * 64 < n; ++c) {
         const int node = c * 64 + lane;
         const bool live = node < n;
         int par = live ? p.parents[base + node] : 0;
+        const int32_t slot = live ? place_token(p, rq, rq.x + node) : 0;
         if (par < 0 || par >= node) par = 0;  // anything but an earlier node hangs off the root
         const bool local = live && node > 0 && par >= c * 64;
         int ptr = local ? par - c * 64 : lane;
         const int outer = (live && node > 0 && !local) ? par : -1;
         uint64_t m = local ? 1ull << lane : 0;
-        while (__any(__shfl(ptr, ptr) != ptr)) {
+        while (true) {
+            const int next = __shfl(ptr, ptr);
+            if (!__any(next != ptr)) break;
             m |= __shfl(m, ptr);
-            ptr = __shfl(ptr, ptr);
+            ptr = next;
         }
         m |= (1ull << ptr) | (1ull << lane);
         const int up = __shfl(outer, ptr);
@@ -194,12 +188,113 @@ __global__ __launch_bounds__(256) void extend_prepare_tree_kernel(ExtendPrepPara
                 if (w < c && up >= 0) v = p.mask[(int64_t)(base + up) * p.words + w], depth += __popcll(v);
                 row[w] = v;
             }
-            const int pos = rq.x + node;
             p.positions[base + node] = rq.x + depth;
-            p.out_loc[base + node] = place_token(p, rq, pos);
+            p.out_loc[base + node] = slot;
         }
-        __threadfence_block();  // the next chunk reads these mask rows from other lanes of this wave
+        if (n > 64) __threadfence_block();  // the next chunk reads these mask rows from other lanes of this wave
         __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// Entries behind the last request: position 0, the dummy slot, an empty mask.
+__device__ __forceinline__ void clear_behind(const ExtendPrepParams& p, int total, int first, int step) {
+    for (int t = total + first; t < p.capacity; t += step) {
+        p.positions[t] = 0;
+        p.out_loc[t] = 0;
+        for (int w = 0; w < p.words; ++w) p.mask[(int64_t)t * p.words + w] = 0;
+    }
+}
+
+// Phase 2, trees: a wave per request.
+__global__ __launch_bounds__(256) void extend_prepare_tree_kernel(ExtendPrepParams p) {
+    const int b = blockIdx.x * 4 + (threadIdx.x >> 6);
+    clear_behind(p, p.cu[p.bs], blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
+    if (b >= p.bs) return;
+    const int base = p.cu[b];
+    place_tree(p, p.scratch[b], base, min(p.cu[b + 1] - base, p.words * 64));
+}
+
+// Both phases in one work group, for steps of a few thousand tokens: what bounds such a step is latency, and one launch with one barrier has
+// the least of it (4 requests of 8 nodes: 4.9 + 2.4 us as two launches).  Counts fit 32 bits (msgl_prepare_extend sees to it).
+constexpr int kSmallRequests = 1024, kSmallTokens = 4096;
+__global__ __launch_bounds__(kScanThreads) void extend_prepare_small_kernel(ExtendPrepParams p) {
+    __shared__ int4 req[kSmallRequests];           // prefix, alloc, page offset inside the wave's requests, table row
+    __shared__ int start[kSmallRequests];          // first token inside the wave's requests
+    __shared__ int sums[kScanThreads / 64][3];     // tokens, pages, refusals seen
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int head = p.free_range[0], valid_end = p.free_range[1], earlier = *p.status;
+    int L = 0, n = 0, A = 0, row = 0;
+    if (tid < p.bs) L = p.prefix[tid], n = p.new_lens[tid], A = p.alloc[tid], row = p.req_idx[tid];
+    const bool wrong = L < 0 || n < 0 || A < L || A > p.max_ctx || row < 0 || row >= p.table_rows;
+    const bool longer = !wrong && (int64_t)L + n > p.max_ctx;
+    const bool wide = !wrong && ((p.words && n > p.words * 64) || n > p.capacity);
+    const int counted = wrong || longer || wide ? 0 : n;
+    const int have = (A + p.ps - 1) / p.ps;
+    const int need = counted ? max(0, (L + counted + p.ps - 1) / p.ps - have) : 0;
+    int tokens = counted, pages = need;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int u = __shfl_up(tokens, d), v = __shfl_up(pages, d);
+        if (lane >= d) tokens += u, pages += v;
+    }
+    const int seen = (__any(wrong) ? 4 : 0) | (__any(longer) ? 2 : 0) | (__any(wide) ? 1 : 0);
+    if (lane == 63) sums[wave][0] = tokens, sums[wave][1] = pages, sums[wave][2] = seen;
+    if (tid < p.bs) {
+        req[tid] = make_int4(L, A, pages - need - have, row);
+        start[tid] = tokens - counted;
+    }
+    __syncthreads();
+    // every wave has read the state now; the waves' totals and, for a wave's requests, what lies before them
+    int total = 0, taken = 0, any = 0;
+    auto before = [&](int w, int what) {
+        int r = 0;
+#pragma unroll
+        for (int k = 0; k < kScanThreads / 64; ++k) r += k < w ? sums[k][what] : 0;
+        return r;
+    };
+#pragma unroll
+    for (int k = 0; k < kScanThreads / 64; ++k) total += sums[k][0], taken += sums[k][1], any |= sums[k][2];
+    int refuse = earlier;
+    if (!refuse)
+        refuse = any & 4 ? 3 : any & 2 ? 2 : ((any & 1) || total > p.capacity) ? 4 : (head < 0 || taken > (int64_t)min(valid_end, p.free_capacity) - head) ? 1 : 0;
+    if (tid < p.bs) {
+        p.cu[tid] = refuse ? 0 : tokens - counted + before(wave, 0);
+        p.seq_lens[tid] = refuse ? L : L + n;
+        if (!refuse || p.alloc_out != p.alloc) p.alloc_out[tid] = refuse ? A : max(A, L + n);
+    }
+    if (tid == 0) {
+        p.cu[p.bs] = refuse ? 0 : total;
+        if (refuse) *p.status = refuse;
+        if (!refuse || p.free_range_out != p.free_range) p.free_range_out[0] = refuse ? head : head + taken, p.free_range_out[1] = valid_end;
+    }
+    clear_behind(p, refuse ? 0 : total, tid, kScanThreads);
+    if (refuse) return;
+    if (p.parents) {
+        for (int b = wave; b < p.bs; b += kScanThreads / 64) {
+            const int4 rq = req[b];
+            const int w = b >> 6, base = start[b] + before(w, 0);
+            const int end = b + 1 < p.bs ? start[b + 1] + before((b + 1) >> 6, 0) : total;
+            place_tree(p, make_int4(rq.x, rq.y, rq.z + head + before(w, 1), rq.w), base, end - base);
+        }
+    } else {
+        for (int t = tid; t < total; t += kScanThreads) {
+            int w = 0, base = 0;  // the last wave whose requests start at or before t, then the last request among them
+#pragma unroll
+            for (int k = 0, at = 0; k < kScanThreads / 64 - 1; ++k) {
+                at += sums[k][0];
+                if (at <= t && (k + 1) * 64 < p.bs) w = k + 1, base = at;
+            }
+            int lo = w * 64, hi = min(p.bs, lo + 64) - 1;
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if (base + start[mid] <= t) lo = mid;
+                else hi = mid - 1;
+            }
+            const int4 rq = req[lo];
+            const int pos = rq.x + t - (base + start[lo]);
+            p.positions[t] = pos;
+            p.out_loc[t] = place_token(p, make_int4(rq.x, rq.y, rq.z + head + before(w, 1), rq.w), pos);
+        }
     }
 }
 
@@ -223,74 +318,83 @@ struct AcceptParams {
 };
 
 constexpr int kMoveBatch = 8;
+constexpr int kMostAccepted = 64 * MSGL_TREE_MAX_WORDS;
 
-// Work group = one request and a run of layers.  Every wave walks the tree by itself (no exchange needed): a node's child is the first
-// later node that hangs off it and drafted the token the model put after it.  Path indices rise, and row i of the path goes to node
-// i's slot with i <= path[i]; the source of a later row is therefore never an earlier row's destination, and a thread that carries
-// the same 16 bytes of every row may load a batch of rows before it stores them.
+// Work group = one request and a run of layers.  Its first wave walks the tree: a node's child is the first later node that hangs off it and
+// drafted the token the model put after it; the first 64 nodes are in registers, a node per lane, so a step is a ballot.  Then all threads move
+// rows, each the same 16 bytes of every row.  Path indices rise, and row i of the path goes to node i's slot with i <= path[i]: the source of a
+// later row is never an earlier row's destination, so a thread may load a batch of rows before it stores them.  What bounds this is latency
+// (lengths -> tree -> rows); every group repeats the walk rather than wait for a launch of its own.
 __global__ __launch_bounds__(256) void accept_tree_kernel(AcceptParams p) {
-    __shared__ int32_t path_lds[4][1024];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __shared__ int2 moves[kMostAccepted];  // slots: from, to
+    __shared__ int moved;
+    const int lane = threadIdx.x & 63;
     const int b = blockIdx.x;
-    const int base = p.cu[b];
-    const int n = p.cu[b + 1] - base;
-    const bool writer = blockIdx.y == 0 && wave == 0;
-    int32_t* path = path_lds[wave];
-    int len = 0;
-    if (n > 0) {
-        int par0 = lane < n ? p.parents[base + lane] : -1;
-        const int tok0 = lane < n ? p.draft[base + lane] : 0;
-        const int tgt0 = lane < n ? p.target[base + lane] : 0;
-        if (lane < n && (par0 < 0 || par0 >= lane)) par0 = 0;
-        int cur = 0;
-        while (true) {
-            const int want = cur < 64 ? __shfl(tgt0, cur) : p.target[base + cur];
-            if (lane == 0) path[len] = cur;
-            if (writer && lane == 0) p.rows[(int64_t)b * p.most + len] = base + cur, p.tokens[(int64_t)b * p.most + len] = want;
-            ++len;
-            if (writer && lane == 0) p.next[b] = want;
-            if (len == p.most) break;
-            int child = -1;
-            if (cur < 63) {
-                const uint64_t hit = __ballot(lane < n && lane > cur && par0 == cur && tok0 == want);
-                if (hit) child = __ffsll((unsigned long long)hit) - 1;
-            }
-            for (int c = max(64, (cur + 1) & ~63); child < 0 && c < n; c += 64) {
-                const int node = c + lane;
-                bool is = false;
-                if (node < n && node > cur) {
-                    int par = p.parents[base + node];
-                    if (par < 0 || par >= node) par = 0;
-                    is = par == cur && p.draft[base + node] == want;
+    if (threadIdx.x < 64) {
+        const bool writer = blockIdx.y == 0;
+        const int base = p.cu[b];
+        const int n = p.cu[b + 1] - base;
+        int len = 0, count = 0;
+        if (n > 0) {
+            int par0 = -1, tok0 = 0, tgt0 = 0, loc0 = 0;
+            if (lane < n) par0 = p.parents[base + lane], tok0 = p.draft[base + lane], tgt0 = p.target[base + lane], loc0 = p.loc[base + lane];
+            if (lane < n && (par0 < 0 || par0 >= lane)) par0 = 0;
+            int cur = 0, want = 0;
+            while (true) {
+                want = cur < 64 ? __shfl(tgt0, cur) : p.target[base + cur];
+                if (cur != len) {
+                    const int from = cur < 64 ? __shfl(loc0, cur) : p.loc[base + cur], to = len < 64 ? __shfl(loc0, len) : p.loc[base + len];
+                    if (lane == 0) moves[count] = make_int2(from, to);
+                    ++count;
                 }
-                const uint64_t hit = __ballot(is);
-                if (hit) child = c + __ffsll((unsigned long long)hit) - 1;
+                if (writer && lane == 0) p.rows[(int64_t)b * p.most + len] = base + cur, p.tokens[(int64_t)b * p.most + len] = want;
+                if (++len == p.most) break;
+                int child = -1;
+                if (cur < 63) {
+                    const uint64_t hit = __ballot(lane < n && lane > cur && par0 == cur && tok0 == want);
+                    if (hit) child = __ffsll((unsigned long long)hit) - 1;
+                }
+                for (int c = max(64, (cur + 1) & ~63); child < 0 && c < n; c += 64) {
+                    const int node = c + lane;
+                    bool is = false;
+                    if (node < n && node > cur) {
+                        int par = p.parents[base + node];
+                        if (par < 0 || par >= node) par = 0;
+                        is = par == cur && p.draft[base + node] == want;
+                    }
+                    const uint64_t hit = __ballot(is);
+                    if (hit) child = c + __ffsll((unsigned long long)hit) - 1;
+                }
+                if (child < 0) break;
+                cur = child;
             }
-            if (child < 0) break;
-            cur = child;
+            if (writer && lane == 0) p.next[b] = want;
         }
-    }
-    if (writer) {
-        for (int i = len + lane; i < p.most; i += 64) p.rows[(int64_t)b * p.most + i] = -1, p.tokens[(int64_t)b * p.most + i] = -1;
-        if (lane == 0) {
-            p.lens[b] = len;
-            p.seq_lens[b] = p.prefix[b] + len;
+        if (writer) {
+            for (int i = len + lane; i < p.most; i += 64) p.rows[(int64_t)b * p.most + i] = -1, p.tokens[(int64_t)b * p.most + i] = -1;
+            if (lane == 0) {
+                p.lens[b] = len;
+                p.seq_lens[b] = p.prefix[b] + len;
+            }
         }
+        if (lane == 0) moved = count;
     }
-    __builtin_amdgcn_wave_barrier();
-    __threadfence_block();
+    __syncthreads();
+    const int count = moved;
     const int l0 = blockIdx.y * p.layers_per_group, layers = min(p.num_layers - l0, p.layers_per_group);
     for (int e = threadIdx.x; e < layers * 2 * p.row_chunks; e += 256) {  // K chunks, then V chunks, layer after layer
         const int half = e / p.row_chunks;
         char* cache = reinterpret_cast<char*>(p.layers[2 * l0 + half]) + (int64_t)(e - half * p.row_chunks) * 16;
-        for (int i0 = 1; i0 < len; i0 += kMoveBatch) {
-            uint4 v[kMoveBatch];
-            const int count = min(kMoveBatch, len - i0);
+        for (int i0 = 0; i0 < count; i0 += kMoveBatch) {
+            u32x4 v[kMoveBatch];
 #pragma unroll
-            for (int j = 0; j < kMoveBatch; ++j) v[j] = *reinterpret_cast<const uint4*>(cache + p.loc[base + path[i0 + min(j, count - 1)]] * p.slot_bytes);
+            for (int j = 0; j < kMoveBatch; ++j) {
+                v[j] = u32x4{0, 0, 0, 0};
+                if (i0 + j < count) v[j] = *reinterpret_cast<const u32x4*>(cache + moves[i0 + j].x * p.slot_bytes);
+            }
 #pragma unroll
             for (int j = 0; j < kMoveBatch; ++j)
-                if (j < count) *reinterpret_cast<uint4*>(cache + p.loc[base + i0 + j] * p.slot_bytes) = v[j];
+                if (i0 + j < count) *reinterpret_cast<u32x4*>(cache + moves[i0 + j].y * p.slot_bytes) = v[j];
         }
     }
 }
@@ -299,7 +403,11 @@ __global__ __launch_bounds__(256) void accept_tree_kernel(AcceptParams p) {
 
 using namespace msgl;
 
-extern "C" size_t msgl_prepare_extend_workspace_bytes(int bs) { return bs > 0 ? (size_t)bs * sizeof(int4) : 0; }
+// (the largest sums of the one-group kernel: 1024 requests of at most `capacity` tokens and max_ctx pages)
+extern "C" size_t msgl_prepare_extend_workspace_bytes(int bs, int32_t capacity, int32_t max_ctx) {
+    if (bs <= 0 || (bs <= kSmallRequests && capacity <= kSmallTokens && max_ctx <= 1 << 20)) return 0;
+    return (size_t)bs * sizeof(int4);
+}
 
 extern "C" int msgl_prepare_extend(const int32_t* req_pool_indices, const int32_t* prefix_lens, const int32_t* new_lens, const int32_t* alloc_lens,
                                    const int32_t* free_pages, int32_t free_capacity, const int32_t* free_range, int32_t* req_to_token,
@@ -323,8 +431,9 @@ extern "C" int msgl_prepare_extend(const int32_t* req_pool_indices, const int32_
                  (long long)r2p_stride);
     MSGL_REQUIRE(seq_lens != prefix_lens && seq_lens != new_lens && seq_lens != alloc_lens && alloc_out != prefix_lens && alloc_out != new_lens,
                  "msgl_prepare_extend: an output overwrites an input (only alloc_out may be alloc_lens, free_range_out free_range)");
-    if (workspace_bytes < msgl_prepare_extend_workspace_bytes(bs) || workspace == nullptr) {
-        set_error("msgl_prepare_extend: workspace %zu < %zu bytes", workspace_bytes, msgl_prepare_extend_workspace_bytes(bs));
+    const size_t need = msgl_prepare_extend_workspace_bytes(bs, capacity, max_ctx);
+    if (need && (workspace_bytes < need || workspace == nullptr)) {
+        set_error("msgl_prepare_extend: workspace %zu < %zu bytes", workspace ? workspace_bytes : (size_t)0, need);
         return MSGL_E_WORKSPACE;
     }
     MSGL_REQUIRE(aligned16(workspace), "msgl_prepare_extend: workspace must be 16-byte aligned");
@@ -338,6 +447,10 @@ extern "C" int msgl_prepare_extend(const int32_t* req_pool_indices, const int32_
     p.scratch = static_cast<int4*>(workspace);
     p.capacity = capacity, p.words = parents ? mask_words : 0, p.bs = bs, p.ps = page_size;
     const hipStream_t st = static_cast<hipStream_t>(stream);
+    if (need == 0) {
+        hipLaunchKernelGGL(extend_prepare_small_kernel, dim3(1), dim3(kScanThreads), 0, st, p);
+        return check_launch("extend_prepare_small_kernel");
+    }
     hipLaunchKernelGGL(extend_prepare_scan_kernel, dim3(1), dim3(kScanThreads), 0, st, p);
     if (parents) hipLaunchKernelGGL(extend_prepare_tree_kernel, dim3((unsigned)((bs + 3) / 4)), dim3(256), 0, st, p);
     else if (capacity) hipLaunchKernelGGL(extend_prepare_fill_kernel, dim3((unsigned)((capacity + 255) / 256)), dim3(256), 0, st, p);
@@ -348,7 +461,7 @@ extern "C" int msgl_accept_tree(const int32_t* draft_tokens, const int32_t* targ
                                 const int32_t* prefix_lens, const int32_t* out_cache_loc, const uint64_t* kv_layers, int num_layers,
                                 int64_t cache_stride, int Hkv, int D, int32_t* accept_lens, int32_t* accept_rows, int32_t* accept_tokens,
                                 int32_t* next_tokens, int32_t* seq_lens, int bs, int max_accept, void* stream) {
-    MSGL_REQUIRE(bs >= 0 && bs <= 65535 * 16 && num_layers >= 0 && num_layers <= 4096 && max_accept >= 1 && max_accept <= 64 * MSGL_TREE_MAX_WORDS,
+    MSGL_REQUIRE(bs >= 0 && bs <= 65535 * 16 && num_layers >= 0 && num_layers <= 4096 && max_accept >= 1 && max_accept <= kMostAccepted,
                  "msgl_accept_tree: bs=%d num_layers=%d max_accept=%d", bs, num_layers, max_accept);
     if (bs == 0) return MSGL_OK;
     MSGL_REQUIRE(draft_tokens && target_tokens && parents && cu_seqlens_q && prefix_lens && out_cache_loc && accept_lens && accept_rows && accept_tokens &&
@@ -361,10 +474,10 @@ extern "C" int msgl_accept_tree(const int32_t* draft_tokens, const int32_t* targ
     p.layers = kv_layers, p.slot_bytes = cache_stride * 2, p.row_chunks = num_layers ? (int32_t)((int64_t)Hkv * D / 8) : 0;
     p.lens = accept_lens, p.rows = accept_rows, p.tokens = accept_tokens, p.next = next_tokens, p.seq_lens = seq_lens;
     p.bs = bs, p.num_layers = num_layers, p.most = max_accept;
-    // enough groups for eight per compute unit, each repeating the walk: fewer layers per group beyond that only repeat it more often
+    // enough groups for eight per compute unit, each repeating the walk: more would only repeat it more often
     const int64_t want = 8 * (int64_t)device_cus();
-    const int groups = (int)(bs >= want ? 1 : num_layers > 1 ? (want + bs - 1) / bs < num_layers ? (want + bs - 1) / bs : num_layers : 1);
-    p.layers_per_group = num_layers ? (num_layers + groups - 1) / groups : 0;
+    const int groups = (int)((want + bs - 1) / bs);
+    p.layers_per_group = (num_layers + groups - 1) / groups;
     const unsigned gy = num_layers ? (unsigned)((num_layers + p.layers_per_group - 1) / p.layers_per_group) : 1u;
     hipLaunchKernelGGL(accept_tree_kernel, dim3((unsigned)bs, gy), dim3(256), 0, static_cast<hipStream_t>(stream), p);
     return check_launch("accept_tree_kernel");

@@ -621,42 +621,65 @@ TREE_MAX_WORDS = 16        # MSGL_TREE_MAX_WORDS: mask words of 64 nodes per req
 LOGPROBS_MAX_TOP = 32      # MSGL_LOGPROBS_MAX_TOP
 
 
-def _launch(dev: torch.device, entry, *args) -> None:
-    """entry(*args, stream) on dev's current stream, with dev the current device while the kernels are launched."""
-    if torch.cuda.current_device() == dev.index:
-        _check(entry(*args, torch.cuda.current_stream(dev).cuda_stream))
+# These wrappers sit in a decode step's critical path at a handful of microseconds of kernel each: they test first and word the complaint only when
+# there is one.
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _launch(index: int, entry, *args) -> None:
+    """entry(*args, stream) on the device's current stream, with that device current while the kernels are launched."""
+    if torch.cuda.current_device() == index:
+        status = entry(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(dev):
-            _check(entry(*args, torch.cuda.current_stream(dev).cuda_stream))
+        with torch.cuda.device(index):
+            status = entry(*args, _raw_stream(index))
+    if status:
+        _check(status)
 
 
-def _i32_on(dev: torch.device, n: int, **tensors) -> None:
-    """Every tensor is a dense 1-D int32 tensor of n entries on dev."""
-    for name, t in tensors.items():
-        if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or t.device != dev or (n > 1 and t.stride(0) != 1):
-            raise ValueError(f"{name} must be a contiguous 1-D int32 tensor of {n} entries on {dev} "
+def _gpu_index(t: torch.Tensor, name: str) -> int:
+    if not t.is_cuda:
+        raise ValueError(f"{name} must live on the GPU (got {t.device})")
+    return t.get_device()
+
+
+def _i32_on(index: int, n: int, names: str, *tensors: torch.Tensor) -> None:
+    """Every tensor is a dense 1-D int32 tensor of n entries on device `index`; `names`, space separated, for the complaint."""
+    for t in tensors:
+        if t.dtype is not torch.int32 or t.numel() != n or t.get_device() != index or t.dim() != 1 or not t.is_contiguous():
+            name = names.split()[[x is t for x in tensors].index(True)]
+            raise ValueError(f"{name} must be a contiguous 1-D int32 tensor of {n} entries on the same GPU as the others "
                              f"(got {t.dtype} {tuple(t.shape)}, strides {t.stride()}, on {t.device})")
 
 
-def _table_on(dev: torch.device, t: torch.Tensor, name: str) -> None:
-    _need(t.device == dev and t.dtype == torch.int32 and t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= t.shape[1],
-          f"{name} must be an int32 [reqs, ctx] tensor with dense rows on {dev}")
+def _table_on(index: int, t: torch.Tensor, name: str) -> None:
+    if t.get_device() != index or t.dtype is not torch.int32 or t.dim() != 2 or t.stride(1) != 1 or t.stride(0) < t.shape[1]:
+        raise ValueError(f"{name} must be an int32 [reqs, ctx] tensor with dense rows on the same GPU as the others")
 
 
-def _scratch(workspace: Optional[torch.Tensor], need: int, dev: torch.device) -> Optional[torch.Tensor]:
+def _mask_on(index: int, t: torch.Tensor, rows: int) -> int:
+    """Words per row of a tree mask."""
+    if t.get_device() != index or t.dtype is not torch.int64 or t.dim() != 2 or t.shape[0] != rows or not t.is_contiguous() \
+            or not 1 <= t.shape[1] <= TREE_MAX_WORDS:
+        raise ValueError(f"tree_mask must be a contiguous int64 [{rows}, 1..{TREE_MAX_WORDS}] tensor on the same GPU as the others")
+    return t.shape[1]
+
+
+def _scratch(workspace: Optional[torch.Tensor], need: int, index: int) -> Tuple[Optional[torch.Tensor], Optional[int], int]:
+    """(the tensor to hold on to, address, bytes) of a caller's workspace, or of one of `need` bytes made here."""
     if workspace is None:
-        return torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _need(workspace.device == dev and workspace.is_contiguous() and workspace.data_ptr() % 16 == 0,
-          f"workspace must be a contiguous 16-byte aligned tensor on {dev}")
-    return workspace
+        if not need:
+            return None, None, 0
+        workspace = torch.empty(need, dtype=torch.uint8, device=index)
+        return workspace, workspace.data_ptr(), need
+    if workspace.get_device() != index or not workspace.is_contiguous() or workspace.data_ptr() % 16:
+        raise ValueError("workspace must be a contiguous 16-byte aligned tensor on the same GPU as the others")
+    return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
-def _bytes(t: Optional[torch.Tensor]) -> int:
-    return 0 if t is None else t.numel() * t.element_size()
-
-
-def prepare_extend_workspace_bytes(bs: int) -> int:
-    return int(_lib.msgl_prepare_extend_workspace_bytes(int(bs)))
+def prepare_extend_workspace_bytes(bs: int, capacity: int, max_ctx: int) -> int:
+    return int(_lib.msgl_prepare_extend_workspace_bytes(int(bs), int(capacity), int(max_ctx)))
 
 
 def prepare_extend(req_pool_indices: torch.Tensor, prefix_lens: torch.Tensor, new_lens: torch.Tensor, alloc_lens: torch.Tensor,
@@ -670,40 +693,42 @@ def prepare_extend(req_pool_indices: torch.Tensor, prefix_lens: torch.Tensor, ne
     ``out_cache_loc`` (and ``tree_mask``: int64 [capacity, words]) of any capacity, ``cu_seqlens_q``, ``seq_lens`` and the tables;
     ``alloc_lens`` and ``free_range`` advance in place unless ``alloc_out`` / ``free_range_out`` are given.  ``status``
     (int32[1]) becomes non-zero if the step was refused, and nothing but empty outputs is written then."""
-    dev = req_pool_indices.device
-    _need(dev.type == "cuda", f"req_pool_indices must live on the GPU (got {dev})")
+    index = _gpu_index(req_pool_indices, "req_pool_indices")
     bs, capacity = req_pool_indices.numel(), out_cache_loc.numel()
-    alloc_out = alloc_lens if alloc_out is None else alloc_out
-    free_range_out = free_range if free_range_out is None else free_range_out
-    _i32_on(dev, bs, req_pool_indices=req_pool_indices, prefix_lens=prefix_lens, new_lens=new_lens, alloc_lens=alloc_lens, seq_lens=seq_lens,
-            alloc_out=alloc_out)
-    _i32_on(dev, capacity, positions=positions, out_cache_loc=out_cache_loc)
-    _i32_on(dev, free_pages.numel(), free_pages=free_pages)
-    _i32_on(dev, 2, free_range=free_range, free_range_out=free_range_out)
-    _i32_on(dev, bs + 1, cu_seqlens_q=cu_seqlens_q)
-    _i32_on(dev, 1, status=status)
-    _table_on(dev, req_to_token, "req_to_token")
-    _need((parents is None) == (tree_mask is None), "parents and tree_mask go together")
-    words = 0
+    if alloc_out is None:
+        alloc_out = alloc_lens
+    if free_range_out is None:
+        free_range_out = free_range
+    _i32_on(index, bs, "req_pool_indices prefix_lens new_lens alloc_lens seq_lens alloc_out", req_pool_indices, prefix_lens, new_lens, alloc_lens, seq_lens,
+            alloc_out)
+    _i32_on(index, capacity, "positions out_cache_loc", positions, out_cache_loc)
+    _i32_on(index, free_pages.numel(), "free_pages", free_pages)
+    _i32_on(index, 2, "free_range free_range_out", free_range, free_range_out)
+    _i32_on(index, bs + 1, "cu_seqlens_q", cu_seqlens_q)
+    _i32_on(index, 1, "status", status)
+    _table_on(index, req_to_token, "req_to_token")
+    if (parents is None) != (tree_mask is None):
+        raise ValueError("parents and tree_mask go together")
+    parents_at = mask_at = page_at = None
+    words = page_stride = 0
     if parents is not None:
-        _i32_on(dev, capacity, parents=parents)
-        _need(tree_mask.device == dev and tree_mask.dtype == torch.int64 and tree_mask.dim() == 2 and tree_mask.is_contiguous()
-              and tree_mask.shape[0] == capacity and 1 <= tree_mask.shape[1] <= TREE_MAX_WORDS,
-              f"tree_mask must be a contiguous int64 [{capacity}, 1..{TREE_MAX_WORDS}] tensor on {dev}")
-        words = tree_mask.shape[1]
+        _i32_on(index, capacity, "parents", parents)
+        words = _mask_on(index, tree_mask, capacity)
+        parents_at, mask_at = parents.data_ptr(), tree_mask.data_ptr()
+    rows, max_ctx = req_to_token.shape
     if req_to_page is not None:
-        _table_on(dev, req_to_page, "req_to_page")
-        _need(req_to_page.shape[0] == req_to_token.shape[0], "req_to_page needs a row per row of req_to_token")
+        _table_on(index, req_to_page, "req_to_page")
+        if req_to_page.shape[0] != rows:
+            raise ValueError("req_to_page needs a row per row of req_to_token")
+        page_at, page_stride = req_to_page.data_ptr(), req_to_page.stride(0)
     if bs == 0:
         return
-    ws = _scratch(workspace, 16 * bs, dev)
-    _launch(dev, _lib.msgl_prepare_extend, req_pool_indices.data_ptr(), prefix_lens.data_ptr(), new_lens.data_ptr(), alloc_lens.data_ptr(),
-            free_pages.data_ptr(), free_pages.numel(), free_range.data_ptr(), req_to_token.data_ptr(), req_to_token.stride(0),
-            req_to_token.shape[0], req_to_token.shape[1], req_to_page.data_ptr() if req_to_page is not None else None,
-            req_to_page.stride(0) if req_to_page is not None else 0, parents.data_ptr() if parents is not None else None,
-            tree_mask.data_ptr() if tree_mask is not None else None, words, positions.data_ptr(), out_cache_loc.data_ptr(), capacity,
-            cu_seqlens_q.data_ptr(), seq_lens.data_ptr(), alloc_out.data_ptr(), free_range_out.data_ptr(), status.data_ptr(), bs, int(page_size),
-            ws.data_ptr(), _bytes(ws))
+    small = bs <= 1024 and capacity <= 4096 and max_ctx <= 1 << 20  # (no workspace for steps of this size)
+    ws, ws_at, ws_bytes = _scratch(workspace, 0 if small else prepare_extend_workspace_bytes(bs, capacity, max_ctx), index)
+    _launch(index, _lib.msgl_prepare_extend, req_pool_indices.data_ptr(), prefix_lens.data_ptr(), new_lens.data_ptr(), alloc_lens.data_ptr(),
+            free_pages.data_ptr(), free_pages.numel(), free_range.data_ptr(), req_to_token.data_ptr(), req_to_token.stride(0), rows, max_ctx,
+            page_at, page_stride, parents_at, mask_at, words, positions.data_ptr(), out_cache_loc.data_ptr(), capacity, cu_seqlens_q.data_ptr(),
+            seq_lens.data_ptr(), alloc_out.data_ptr(), free_range_out.data_ptr(), status.data_ptr(), bs, page_size, ws_at, ws_bytes)
 
 
 def tree_attention_splits(bs: int, max_seqlen_q: int, max_seqlen_k: int, Hq: int, Hkv: int, total_kv: int = 0) -> int:
@@ -724,39 +749,45 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     msgl_tree_attention.  ``max_seqlen_q``: most nodes of a request.  ``max_seqlen_k`` (longest prefix + nodes) and ``total_kv`` (their
     sum over the batch, 0 = unknown) steer the cut of long contexts; ``workspace`` (tree_attention_workspace_bytes) is allocated here when
     omitted."""
-    dev = q.device
-    _dev_bf16(q, "q")
-    _need(q.dim() == 3 and q.stride(2) == 1 and q.stride(1) == q.shape[2], "q must be [T, Hq, D] with dense heads")
+    index = _gpu_index(q, "q")
+    if q.dtype is not torch.bfloat16 or q.dim() != 3 or q.stride()[1:] != (q.shape[2], 1):
+        raise ValueError("q must be bfloat16 [T, Hq, D] with dense heads")
     T, Hq, D = q.shape
-    _need(k_cache.dim() == 3, "k_cache must be [slots, Hkv, D]")
-    Hkv = k_cache.shape[1]
-    cs = _cache_stride(k_cache, v_cache, Hkv, D)
-    _need(k_cache.device == dev and v_cache.device == dev, f"k_cache / v_cache must live on {dev}")
+    slots, Hkv, cs = _cache_on(index, k_cache, v_cache, D)
     bs = req_pool_indices.numel()
-    _i32_on(dev, bs, req_pool_indices=req_pool_indices, prefix_lens=prefix_lens)
-    _i32_on(dev, bs + 1, cu_seqlens_q=cu_seqlens_q)
-    _table_on(dev, req_to_token, "req_to_token")
-    _need(tree_mask.device == dev and tree_mask.dtype == torch.int64 and tree_mask.dim() == 2 and tree_mask.is_contiguous()
-          and tree_mask.shape[0] == T and 1 <= tree_mask.shape[1] <= TREE_MAX_WORDS,
-          f"tree_mask must be a contiguous int64 [{T}, 1..{TREE_MAX_WORDS}] tensor on {dev}")
-    _need(0 < max_seqlen_q <= 64 * tree_mask.shape[1] or T == 0, f"max_seqlen_q {max_seqlen_q} needs {-(-max_seqlen_q // 64)} mask words")
+    _i32_on(index, bs, "req_pool_indices prefix_lens", req_pool_indices, prefix_lens)
+    _i32_on(index, bs + 1, "cu_seqlens_q", cu_seqlens_q)
+    _table_on(index, req_to_token, "req_to_token")
+    words = _mask_on(index, tree_mask, T)
+    if T and not 0 < max_seqlen_q <= 64 * words:
+        raise ValueError(f"max_seqlen_q {max_seqlen_q} outside 1..{64 * words} (64 nodes per mask word)")
     if out is None:
-        out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=dev)
+        out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=index)
+        out_stride = Hq * D
     else:
-        _dev_bf16(out, "out")
-        _need(out.device == dev and out.shape == q.shape and out.stride(2) == 1 and out.stride(1) == D, "out must match q's layout")
+        if out.get_device() != index or out.dtype is not torch.bfloat16 or out.shape != q.shape or out.stride()[1:] != (D, 1):
+            raise ValueError("out must match q's layout")
+        out_stride = out.stride(0) if T > 1 else Hq * D
     if T == 0 or bs == 0:
         return out
+    need = 0
     if workspace is None:
         splits = _lib.msgl_tree_attention_splits(bs, max_seqlen_q, max_seqlen_k, total_kv, Hq, Hkv)
-        ws = torch.empty(4 * (D + 2) * T * Hq * splits, dtype=torch.uint8, device=dev) if splits > 1 else None
-    else:
-        ws = _scratch(workspace, 0, dev)
-    _launch(dev, _lib.msgl_tree_attention, q.data_ptr(), q.stride(0) if T > 1 else Hq * D, k_cache.data_ptr(), v_cache.data_ptr(), cs,
+        need = 4 * (D + 2) * T * Hq * splits if splits > 1 else 0
+    ws, ws_at, ws_bytes = _scratch(workspace, need, index)
+    _launch(index, _lib.msgl_tree_attention, q.data_ptr(), q.stride(0) if T > 1 else Hq * D, k_cache.data_ptr(), v_cache.data_ptr(), cs,
             req_to_token.data_ptr(), req_to_token.stride(0), req_pool_indices.data_ptr(), cu_seqlens_q.data_ptr(), prefix_lens.data_ptr(),
-            tree_mask.data_ptr(), tree_mask.shape[1], out.data_ptr(), out.stride(0) if T > 1 else Hq * D, T, bs, int(max_seqlen_q),
-            int(max_seqlen_k), int(total_kv), Hq, Hkv, D, float(scale), ws.data_ptr() if ws is not None else None, _bytes(ws))
+            tree_mask.data_ptr(), words, out.data_ptr(), out_stride, T, bs, max_seqlen_q, max_seqlen_k, total_kv, Hq, Hkv, D, scale, ws_at, ws_bytes)
     return out
+
+
+def _cache_on(index: int, k: torch.Tensor, v: torch.Tensor, D: int) -> Tuple[int, int, int]:
+    """(slots, Hkv, slot stride) of a [slots, Hkv, D] K/V pair on device `index`, heads dense per slot."""
+    stride = k.stride()
+    if k.dtype is not torch.bfloat16 or v.dtype is not torch.bfloat16 or k.get_device() != index or v.get_device() != index or k.dim() != 3 \
+            or k.shape != v.shape or k.shape[2] != D or stride != v.stride() or stride[1:] != (D, 1) or stride[0] < k.shape[1] * D:
+        raise ValueError(f"k_cache / v_cache must be bfloat16 [slots, Hkv, {D}] of one slot stride on the same GPU as the others, [Hkv, D] dense per slot")
+    return k.shape[0], k.shape[1], stride[0]
 
 
 @dataclass
@@ -791,25 +822,25 @@ def accept_tree(draft_tokens: torch.Tensor, target_tokens: torch.Tensor, parents
     model's ``target_tokens`` entry of the node before.  Writes accept_lens [bs], accept_rows and accept_tokens [bs, most] (-1 behind the
     path), next_tokens [bs] and seq_lens [bs] = prefix_lens + accept_lens (may be prefix_lens itself), and moves the accepted nodes' K and V
     rows to consecutive positions in every layer of ``layers`` (None: moves nothing)."""
-    dev = draft_tokens.device
-    _need(dev.type == "cuda", f"draft_tokens must live on the GPU (got {dev})")
+    index = _gpu_index(draft_tokens, "draft_tokens")
     T, bs = draft_tokens.numel(), prefix_lens.numel()
-    _i32_on(dev, T, draft_tokens=draft_tokens, target_tokens=target_tokens, parents=parents, out_cache_loc=out_cache_loc)
-    _i32_on(dev, bs + 1, cu_seqlens_q=cu_seqlens_q)
-    _i32_on(dev, bs, prefix_lens=prefix_lens, accept_lens=accept_lens, next_tokens=next_tokens, seq_lens=seq_lens)
-    _need(accept_rows.dim() == 2 and accept_rows.shape[0] == bs and 1 <= accept_rows.shape[1] <= 64 * TREE_MAX_WORDS
-          and accept_tokens.shape == accept_rows.shape, f"accept_rows and accept_tokens must be [{bs}, 1..{64 * TREE_MAX_WORDS}]")
-    for name, t in (("accept_rows", accept_rows), ("accept_tokens", accept_tokens)):
-        _need(t.device == dev and t.dtype == torch.int32 and t.is_contiguous(), f"{name} must be a contiguous int32 tensor on {dev}")
+    _i32_on(index, T, "draft_tokens target_tokens parents out_cache_loc", draft_tokens, target_tokens, parents, out_cache_loc)
+    _i32_on(index, bs + 1, "cu_seqlens_q", cu_seqlens_q)
+    _i32_on(index, bs, "prefix_lens accept_lens next_tokens seq_lens", prefix_lens, accept_lens, next_tokens, seq_lens)
+    for t in (accept_rows, accept_tokens):
+        if t.get_device() != index or t.dtype is not torch.int32 or t.dim() != 2 or t.shape != accept_rows.shape or t.shape[0] != bs \
+                or not 1 <= t.shape[1] <= 64 * TREE_MAX_WORDS or not t.is_contiguous():
+            raise ValueError(f"accept_rows and accept_tokens must be contiguous int32 [{bs}, 1..{64 * TREE_MAX_WORDS}] tensors on the same GPU as the others")
     if bs == 0:
         return
     if layers is None:
         table, count, stride, Hkv, D = None, 0, 0, 0, 0
     else:
-        _need(layers.table.device == dev, f"the caches must live on {dev}")
+        if layers.table.get_device() != index:
+            raise ValueError("the caches must live on the same GPU as the others")
         table, count, stride = layers.table.data_ptr(), len(layers.k), layers.slot_stride
         _, Hkv, D = layers.k[0].shape
-    _launch(dev, _lib.msgl_accept_tree, draft_tokens.data_ptr(), target_tokens.data_ptr(), parents.data_ptr(), cu_seqlens_q.data_ptr(),
+    _launch(index, _lib.msgl_accept_tree, draft_tokens.data_ptr(), target_tokens.data_ptr(), parents.data_ptr(), cu_seqlens_q.data_ptr(),
             prefix_lens.data_ptr(), out_cache_loc.data_ptr(), table, count, stride, Hkv, D, accept_lens.data_ptr(), accept_rows.data_ptr(),
             accept_tokens.data_ptr(), next_tokens.data_ptr(), seq_lens.data_ptr(), bs, accept_rows.shape[1])
 
@@ -822,21 +853,23 @@ def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, top_k: int = 0
     """(logprobs [rows], entropy [rows], top_ids int32 [rows, top_k], top_logprobs [rows, top_k]) of logits [rows, vocab] (bf16 or fp32),
     all but the ids fp32: log softmax at ``token_ids`` (NaN for an id outside the vocabulary), the rows' entropies in nats, and the
     top_k most probable tokens, ties to the lower id; see msgl_token_logprobs."""
-    dev = logits.device
-    _need(logits.is_cuda and logits.dtype in (torch.bfloat16, torch.float32), "logits must be bf16 or fp32 on the GPU")
+    index = _gpu_index(logits, "logits")
+    if logits.dtype is not torch.bfloat16 and logits.dtype is not torch.float32:
+        raise ValueError(f"logits must be bf16 or fp32 (got {logits.dtype})")
     rows, vocab, rs = _rows_view(logits, "logits")
-    _i32_on(dev, rows, token_ids=token_ids)
-    _need(0 <= top_k <= min(vocab, LOGPROBS_MAX_TOP), f"top_k {top_k} outside 0..min(vocab, {LOGPROBS_MAX_TOP})")
-    stats = torch.empty((2, rows), dtype=torch.float32, device=dev)
-    ids = torch.empty((rows, top_k), dtype=torch.int32, device=dev)
-    top = torch.empty((rows, top_k), dtype=torch.float32, device=dev)
-    size = logits.element_size()
+    _i32_on(index, rows, "token_ids", token_ids)
+    if not 0 <= top_k <= min(vocab, LOGPROBS_MAX_TOP):
+        raise ValueError(f"top_k {top_k} outside 0..min(vocab, {LOGPROBS_MAX_TOP})")
+    logprobs, entropy = torch.empty((2, rows), dtype=torch.float32, device=index).unbind(0)
+    ids = torch.empty((rows, top_k), dtype=torch.int32, device=index)
+    top = torch.empty((rows, top_k), dtype=torch.float32, device=index)
     if rows:
-        ws = _scratch(workspace, _lib.msgl_token_logprobs_workspace_bytes(rows, vocab, size, top_k), dev)
-        _launch(dev, _lib.msgl_token_logprobs, logits.data_ptr(), rs, size, token_ids.data_ptr(), stats.data_ptr(),
-                stats.data_ptr() + 4 * rows, ids.data_ptr() if top_k else None, top.data_ptr() if top_k else None, rows, vocab, top_k,
-                ws.data_ptr(), _bytes(ws))
-    return stats[0], stats[1], ids, top
+        size = 2 if logits.dtype is torch.bfloat16 else 4
+        need = _lib.msgl_token_logprobs_workspace_bytes(rows, vocab, size, top_k) if workspace is None else 0
+        ws, ws_at, ws_bytes = _scratch(workspace, need, index)
+        _launch(index, _lib.msgl_token_logprobs, logits.data_ptr(), rs, size, token_ids.data_ptr(), logprobs.data_ptr(), entropy.data_ptr(),
+                ids.data_ptr() if top_k else None, top.data_ptr() if top_k else None, rows, vocab, top_k, ws_at, ws_bytes)
+    return logprobs, entropy, ids, top
 
 
 def stream_read(buf: torch.Tensor, sink: torch.Tensor, unroll: int = 8, groups_per_cu: int = 16, span_kib: int = 0) -> None:
