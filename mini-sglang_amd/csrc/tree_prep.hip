@@ -474,8 +474,9 @@ extern "C" int msgl_accept_tree(const int32_t* draft_tokens, const int32_t* targ
     p.layers = kv_layers, p.slot_bytes = cache_stride * 2, p.row_chunks = num_layers ? (int32_t)((int64_t)Hkv * D / 8) : 0;
     p.lens = accept_lens, p.rows = accept_rows, p.tokens = accept_tokens, p.next = next_tokens, p.seq_lens = seq_lens;
     p.bs = bs, p.num_layers = num_layers, p.most = max_accept;
-    // enough groups for eight per compute unit, each repeating the walk: more would only repeat it more often
-    const int64_t want = 8 * (int64_t)device_cus();
+    // up to sixteen groups per compute unit, each repeating the walk (128 requests x 36 layers: 32, 22, 19, 17, 14, 13 us at 1, 2, 4, 8, 16, 32 groups
+    // per unit; with one kv head, where a group moves little, 11, 9, 8, 8, 8, 11)
+    const int64_t want = 16 * (int64_t)device_cus();
     const int groups = (int)((want + bs - 1) / bs);
     p.layers_per_group = (num_layers + groups - 1) / groups;
     const unsigned gy = num_layers ? (unsigned)((num_layers + p.layers_per_group - 1) / p.layers_per_group) : 1u;
