@@ -36,7 +36,13 @@ class AttentionBackend(ABC):
 
     def forward(self, q, k, v, layer, batch, save_kv_cache: bool = True, **kwargs):
         """Route one layer's call by the batch's forward mode."""
-        run = self.forward_decode if batch.forward_mode.is_decode() else self.forward_extend
+        mode = batch.forward_mode
+        if mode.is_decode():
+            run = self.forward_decode
+        elif getattr(mode, "is_verify", None) is not None and mode.is_verify():
+            run = self.forward_verify
+        else:
+            run = self.forward_extend
         return run(q, k, v, layer, batch, save_kv_cache=save_kv_cache, **kwargs)
 
     def forward_decode(self, q, k, v, layer, batch, save_kv_cache: bool = True):
@@ -46,6 +52,11 @@ class AttentionBackend(ABC):
     def forward_extend(self, q, k, v, layer, batch, save_kv_cache: bool = True):
         """Runs of new tokens per request, causal among themselves, on top of a cached prefix."""
         raise self._not_provided("forward_extend")
+
+    def forward_verify(self, q, k, v, layer, batch, save_kv_cache: bool = True):
+        """Every node of a drafted token tree per request, each seeing the cached prefix and its ancestors.  Not part of the reference's
+        interface: only callers that draft (runtime/tree_decode.py) set a mode that leads here."""
+        raise self._not_provided("forward_verify")
 
     # ------------------------------------------------------------------ graph capture and replay
     def init_cuda_graph_state(self, max_bs: int):

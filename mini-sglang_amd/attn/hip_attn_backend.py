@@ -42,6 +42,10 @@ class HipAttnMetadata:
     max_seqlen_q: int = 0
     max_seqlen_k: int = 0
     extend_plan: Optional[torch.Tensor] = None  # launch order of the (request, query tile) items, longest first
+    # verify (drafted trees): bounds that may be captured, and buffers of their own so that a captured step keeps its addresses
+    total_kv: int = 0
+    verify_out: Optional[torch.Tensor] = None        # rows behind the last node stay 0
+    verify_workspace: Optional[torch.Tensor] = None
     # metadata of a captured batch size: its launches use the workspace that was sized before the first capture
     static: bool = False
 
@@ -157,6 +161,14 @@ class HipAttnBackend(AttentionBackend):
             md.reuse_lens = getattr(batch, "shared_prefix_lens", None)
             if ragged and md.max_splits > 1:
                 md.decode_plan = ops.decode_plan(batch.seq_lens, md.max_splits, md.chunk_tokens)
+        elif getattr(batch.forward_mode, "is_verify", None) is not None and batch.forward_mode.is_verify():
+            md.max_seqlen_q, md.max_seqlen_k, md.total_kv = int(batch.input_seq_lens_max), int(batch.max_seq_len), int(batch.total_kv)
+            md.cu_seqlens_q = batch.cu_seqlens_q
+            rows = batch.tree_mask.shape[0]
+            md.verify_out = torch.zeros((rows, self.num_heads, self.head_dim), dtype=torch.bfloat16, device=self.device)
+            splits = ops.tree_attention_splits(bs, md.max_seqlen_q, md.max_seqlen_k, self.num_heads, self.num_kv_heads, md.total_kv)
+            need = ops.tree_attention_workspace_bytes(rows, self.num_heads, self.head_dim, splits)
+            md.verify_workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=self.device)
         else:
             md.max_seqlen_q = int(batch.input_seq_lens_max)
             md.max_seqlen_k = int(batch.seq_lens_cpu.max())
@@ -228,6 +240,17 @@ class HipAttnBackend(AttentionBackend):
             kv_stream=self.kv_stream, reuse_lens=md.reuse_lens, plan=md.decode_plan,
             start_lens=sh["start"] if sh is not None else None, extra_splits=sh["extra"] if sh is not None else None)
         return o.view(bs, layer.num_heads * layer.head_dim)
+
+    def forward_verify(self, q, k, v, layer, batch, save_kv_cache: bool = True):
+        if save_kv_cache:
+            self.kv_cache_pool.set_kv_buffer(layer, batch.out_cache_loc, k, v)
+        md = self.forward_metadata
+        k_cache, v_cache = self.kv_cache_pool.get_kv_buffer(layer.layer_id)
+        o = ops.tree_attention(
+            _as_heads(q, layer.num_heads, layer.head_dim), k_cache, v_cache, self.req_to_token_pool.req_to_token, batch.req_pool_indices,
+            md.cu_seqlens_q, batch.prefix_seq_lens, batch.tree_mask, md.max_seqlen_q, md.max_seqlen_k, layer.scale, total_kv=md.total_kv,
+            out=md.verify_out, workspace=md.verify_workspace)
+        return o.view(q.shape[0], layer.num_heads * layer.head_dim)
 
     # ------------------------------------------------------------------ graph hooks
     def init_cuda_graph_state(self, max_bs: int):

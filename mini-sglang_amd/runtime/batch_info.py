@@ -22,12 +22,16 @@ import torch
 class ForwardMode(IntEnum):
     EXTEND = auto()
     DECODE = auto()
+    VERIFY = auto()  # the drafted tree of every request at once (no counterpart in the reference)
 
     def is_extend(self) -> bool:
         return self == ForwardMode.EXTEND
 
     def is_decode(self) -> bool:
         return self == ForwardMode.DECODE
+
+    def is_verify(self) -> bool:
+        return self == ForwardMode.VERIFY
 
 
 @dataclasses.dataclass
@@ -85,6 +89,11 @@ class BatchInfo:
     # int32 [bs]: leading positions whose slots came from the prefix cache, i.e. may be shared with other requests
     # (a cache-policy hint for decode attention; None = unknown / nothing shared)
     shared_prefix_lens: torch.Tensor = None
+    # verify steps (runtime/tree_decode.py): packed nodes of request b are rows cu_seqlens_q[b] .. cu_seqlens_q[b + 1] - 1
+    cu_seqlens_q: torch.Tensor = None       # int32 [bs + 1]
+    tree_mask: torch.Tensor = None          # int64 [rows, words]: ancestors of every node, itself included
+    max_seq_len: int = 0                    # bounds of the step: longest prefix + nodes,
+    total_kv: int = 0                       # and their sum over the batch (input_seq_lens_max: most nodes of a request)
     req_to_token_pool: object = None
     page_allocator: object = None
     kv_cache_pool: object = None
