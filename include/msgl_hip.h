@@ -416,7 +416,8 @@ int msgl_prepare_decode_paged(const int32_t* req_pool_indices, int32_t* seq_lens
  * positions / out_cache_loc / tree_mask have `capacity` rows; rows behind the last token are set
  * to position 0, the dummy slot 0 and an empty mask, so that a captured step of fixed size writes
  * nothing that belongs to a request.  alloc_out may be alloc_lens and free_range_out may be
- * free_range (in place); no other output may be an input.
+ * free_range (in place); no other output may be an input.  A table row belongs to one request of the step: a row given
+ * twice gets both requests' entries in no set order.
  * All or nothing: *status (left as it is on success, sticky like msgl_prepare_decode's) becomes
  * 1 (free list exhausted), 2 (a request outgrows its table row of max_ctx entries), 3 (a negative
  * length, alloc_lens outside prefix_lens .. max_ctx, a table row outside 0 .. table_rows - 1) or
@@ -447,7 +448,7 @@ int msgl_prepare_extend(const int32_t* req_pool_indices, const int32_t* prefix_l
  * workspace: msgl_tree_attention_workspace_bytes(total_tokens, Hq, D, splits) bytes, 16-byte aligned, for
  * splits = msgl_tree_attention_splits(...) of the same bounds; a smaller one (NULL) is legal, long contexts are
  * then cut less.  Different cuts agree to fp32 rounding of the sums; one cut always gives the same bits.
- * Supported: D == 128; Hq/Hkv in {1, 2, 4, 8}; Hkv in {1, 2, 4, 8}; 0 <= scale. */
+ * Supported: D == 128; Hq/Hkv in {1, 2, 4, 8}; Hkv in {1, 2, 4, 8}; 0 <= scale <= 1e38; max_seqlen_k <= 2^30; out apart from q. */
 int msgl_tree_attention_splits(int bs, int max_seqlen_q, int max_seqlen_k, int64_t total_kv, int Hq, int Hkv);
 size_t msgl_tree_attention_workspace_bytes(int64_t total_tokens, int Hq, int D, int splits);
 int msgl_tree_attention(const void* q, int64_t q_stride, const void* k_cache, const void* v_cache, int64_t cache_stride,
@@ -463,7 +464,7 @@ int msgl_tree_attention(const void* q, int64_t q_stride, const void* k_cache, co
  *   accept_rows[b, i] = row (in the packed arrays) of the i-th node, accept_tokens[b, i] = target_tokens of that row, i.e. the
  *   i-th token generated; -1 behind the path ([bs, max_accept] both, dense);
  *   next_tokens[b] = the last of these (the next step's root; left as it is for a request without nodes);
- *   seq_lens[b] = prefix_lens[b] + accept_lens[b]  (seq_lens may be prefix_lens);
+ *   seq_lens[b] = prefix_lens[b] + accept_lens[b]  (seq_lens may be prefix_lens; no other output may be an input);
  *   and in every layer the K and V rows of the i-th node move to the slot of position prefix_lens[b] + i, which is
  *   out_cache_loc[cu_seqlens_q[b] + i].
  * kv_layers: device array [num_layers][2] of the K and V cache addresses ([slots, Hkv, D] bf16, slot stride cache_stride
@@ -481,7 +482,7 @@ int msgl_accept_tree(const int32_t* draft_tokens, const int32_t* target_tokens, 
  * A row with a NaN or +inf in it, or with nothing above -inf, has NaN log probabilities and entropy, as torch's log_softmax.
  * Next to the sampled token's choice (mini_sglang/layers/sampler.py:13-23) this is what a caller that reports log
  * probabilities needs; sums in fp32, one read of the logits.
- * 0 <= top <= min(vocab, MSGL_LOGPROBS_MAX_TOP), vocab <= 2^30.  workspace: msgl_token_logprobs_workspace_bytes bytes, 16-byte
+ * 0 <= top <= min(vocab, MSGL_LOGPROBS_MAX_TOP), vocab <= 2^30, rows * ceil(vocab / 4096) < 2^24.  workspace: msgl_token_logprobs_workspace_bytes bytes, 16-byte
  * aligned. */
 #define MSGL_LOGPROBS_MAX_TOP 32
 size_t msgl_token_logprobs_workspace_bytes(int rows, int vocab, int elem_bytes, int top);

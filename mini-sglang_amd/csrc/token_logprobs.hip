@@ -422,7 +422,7 @@ extern "C" int msgl_token_logprobs(const void* logits, int64_t row_stride, int e
                  (long long)row_stride);
     LogprobParams p;
     p.segments = logprob_segments(rows, vocab, elem_bytes);
-    MSGL_REQUIRE((int64_t)rows * p.segments <= 0x7fffffff, "msgl_token_logprobs: %d rows x %d segments", rows, p.segments);
+    MSGL_REQUIRE((int64_t)rows * p.segments <= 0xffffffffll / kLpThreads, "msgl_token_logprobs: %d rows x %d segments", rows, p.segments);
     const size_t need = msgl_token_logprobs_workspace_bytes(rows, vocab, elem_bytes, top);
     if (workspace == nullptr || workspace_bytes < need) {
         set_error("msgl_token_logprobs: workspace %zu < %zu bytes", workspace_bytes, need);

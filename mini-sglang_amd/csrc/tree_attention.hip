@@ -113,7 +113,7 @@ __device__ __forceinline__ TreeItem tree_item(const TreeParams& p, int b, int sp
     it.base = p.cu[b];
     it.n = min(p.cu[b + 1] - it.base, p.max_q);
     it.rows = it.n * p.group;
-    it.prefix = p.prefix[b];
+    it.prefix = max(p.prefix[b], 0);
     const int S = it.prefix + it.n;
     it.nsplit = min((S + p.chunk - 1) / p.chunk, p.splits);
     it.none = r0 >= it.rows || split >= it.nsplit;
@@ -739,7 +739,7 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeParams p) {
     if (b < p.bs) {
         base = p.cu[b];
         n = min(p.cu[b + 1] - base, p.max_q);
-        nsplit = min((p.prefix[b] + n + p.chunk - 1) / p.chunk, p.splits);
+        nsplit = min((max(p.prefix[b], 0) + n + p.chunk - 1) / p.chunk, p.splits);
     }
     const int node = r / p.Hq, hq = r - node * p.Hq;
     const bool live = node < n && nsplit > 1;  // (one run: written by the first kernel)
@@ -818,6 +818,7 @@ static int launch_wide(const TreeParams& p, int64_t blocks, hipStream_t stream) 
 }
 
 constexpr int kMaxTreeSplits = 256;
+constexpr int kMostKeys = 1 << 30;  // keys of a request: positions plus a run stay inside 32 bits
 
 // How the rows of a kv head are dealt: up to 64 to waves that share them and take different keys, more to waves that hold 32 or 64 rows each and
 // share the keys.
@@ -874,10 +875,13 @@ extern "C" int msgl_tree_attention(const void* q, int64_t q_stride, const void* 
     if (bs == 0 || total_tokens == 0 || max_seqlen_q == 0) return MSGL_OK;
     MSGL_REQUIRE(mask_words >= 1 && mask_words <= MSGL_TREE_MAX_WORDS && max_seqlen_q <= 64 * mask_words,
                  "msgl_tree_attention: %d mask words for up to %d nodes (at most %d words)", mask_words, max_seqlen_q, MSGL_TREE_MAX_WORDS);
-    MSGL_REQUIRE(max_seqlen_k >= 1, "msgl_tree_attention: max_seqlen_k %d", max_seqlen_k);
+    MSGL_REQUIRE(max_seqlen_k >= 1 && max_seqlen_k <= kMostKeys, "msgl_tree_attention: max_seqlen_k %d outside 1..%d", max_seqlen_k, kMostKeys);
     MSGL_REQUIRE(q && k_cache && v_cache && req_to_token && req_pool_indices && cu_seqlens_q && prefix_lens && tree_mask && out,
                  "msgl_tree_attention: null pointer argument");
-    MSGL_REQUIRE(scale >= 0.f && scale <= 3.0e38f, "msgl_tree_attention: scale must be finite and not negative");
+    MSGL_REQUIRE(scale >= 0.f && scale <= 1.0e38f, "msgl_tree_attention: scale must be in 0..1e38");
+    MSGL_REQUIRE(q != out, "msgl_tree_attention: out overwrites q");
+    MSGL_REQUIRE(q_stride >= 0 && out_stride >= (int64_t)Hq * D, "msgl_tree_attention: q_stride %lld, out_stride %lld (rows of %d elements)",
+                 (long long)q_stride, (long long)out_stride, Hq * D);
     MSGL_REQUIRE(aligned16(q) && aligned16(k_cache) && aligned16(v_cache) && aligned16(out) && q_stride % 8 == 0 && out_stride % 8 == 0 && cache_stride % 8 == 0,
                  "msgl_tree_attention: tensors must be 16-byte aligned with strides in multiples of 8");
     MSGL_REQUIRE(cache_stride >= (int64_t)Hkv * D && cache_stride <= 0x7fffffff, "msgl_tree_attention: cache_stride %lld", (long long)cache_stride);
@@ -903,7 +907,7 @@ extern "C" int msgl_tree_attention(const void* q, int64_t q_stride, const void* 
     MSGL_REQUIRE(splits == 1 || aligned16(workspace), "msgl_tree_attention: workspace must be 16-byte aligned");
     const int64_t items = (int64_t)bs * splits * Hkv;
     const int64_t blocks = sh.waves ? (items + 7) / 8 * 8 * p.row_tiles : items;
-    MSGL_REQUIRE(blocks <= 0x7fffffff, "msgl_tree_attention: %lld work groups", (long long)blocks);
+    MSGL_REQUIRE(blocks <= 0x7fffff, "msgl_tree_attention: %lld work groups", (long long)blocks);
     p.items = (int)items;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     int rc;

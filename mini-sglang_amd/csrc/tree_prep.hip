@@ -429,8 +429,12 @@ extern "C" int msgl_prepare_extend(const int32_t* req_pool_indices, const int32_
     MSGL_REQUIRE(r2t_stride >= max_ctx, "msgl_prepare_extend: r2t_stride %lld < max_ctx %d", (long long)r2t_stride, max_ctx);
     MSGL_REQUIRE(req_to_page == nullptr || r2p_stride >= (max_ctx + page_size - 1) / page_size, "msgl_prepare_extend: r2p_stride %lld < pages of a row",
                  (long long)r2p_stride);
-    MSGL_REQUIRE(seq_lens != prefix_lens && seq_lens != new_lens && seq_lens != alloc_lens && alloc_out != prefix_lens && alloc_out != new_lens,
-                 "msgl_prepare_extend: an output overwrites an input (only alloc_out may be alloc_lens, free_range_out free_range)");
+    const int32_t* const inputs[] = {alloc_lens, free_range, req_pool_indices, prefix_lens, new_lens, free_pages, parents};
+    const int32_t* const results[] = {alloc_out, free_range_out, positions, out_cache_loc, cu_seqlens_q, seq_lens, status};
+    for (int i = 0; i < 7; ++i)
+        for (int j = 0; j < 7; ++j)
+            MSGL_REQUIRE(inputs[i] == nullptr || inputs[i] != results[j] || (i == j && i < 2),
+                         "msgl_prepare_extend: an output overwrites an input (only alloc_out may be alloc_lens, free_range_out free_range)");
     const size_t need = msgl_prepare_extend_workspace_bytes(bs, capacity, max_ctx);
     if (need && (workspace_bytes < need || workspace == nullptr)) {
         set_error("msgl_prepare_extend: workspace %zu < %zu bytes", workspace ? workspace_bytes : (size_t)0, need);
@@ -467,6 +471,12 @@ extern "C" int msgl_accept_tree(const int32_t* draft_tokens, const int32_t* targ
     MSGL_REQUIRE(draft_tokens && target_tokens && parents && cu_seqlens_q && prefix_lens && out_cache_loc && accept_lens && accept_rows && accept_tokens &&
                      next_tokens && seq_lens && (num_layers == 0 || kv_layers),
                  "msgl_accept_tree: null pointer argument");
+    // a request may be read by several work groups while one writes its results: no result may lie on an input
+    for (const int32_t* in : {draft_tokens, target_tokens, parents, cu_seqlens_q, out_cache_loc})
+        for (const int32_t* result : {accept_lens, accept_rows, accept_tokens, next_tokens, seq_lens})
+            MSGL_REQUIRE(in != result, "msgl_accept_tree: an output overwrites an input (only seq_lens may be prefix_lens)");
+    MSGL_REQUIRE(accept_lens != prefix_lens && next_tokens != prefix_lens && accept_rows != prefix_lens && accept_tokens != prefix_lens,
+                 "msgl_accept_tree: an output overwrites an input (only seq_lens may be prefix_lens)");
     MSGL_REQUIRE(num_layers == 0 || (Hkv > 0 && D > 0 && (int64_t)Hkv * D % 8 == 0 && cache_stride >= (int64_t)Hkv * D && cache_stride % 8 == 0),
                  "msgl_accept_tree: Hkv=%d D=%d cache_stride=%lld (rows must be whole 16-byte pieces)", Hkv, D, (long long)cache_stride);
     AcceptParams p;

@@ -723,8 +723,7 @@ def prepare_extend(req_pool_indices: torch.Tensor, prefix_lens: torch.Tensor, ne
         page_at, page_stride = req_to_page.data_ptr(), req_to_page.stride(0)
     if bs == 0:
         return
-    small = bs <= 1024 and capacity <= 4096 and max_ctx <= 1 << 20  # (no workspace for steps of this size)
-    ws, ws_at, ws_bytes = _scratch(workspace, 0 if small else prepare_extend_workspace_bytes(bs, capacity, max_ctx), index)
+    ws, ws_at, ws_bytes = _scratch(workspace, _lib.msgl_prepare_extend_workspace_bytes(bs, capacity, max_ctx), index)
     _launch(index, _lib.msgl_prepare_extend, req_pool_indices.data_ptr(), prefix_lens.data_ptr(), new_lens.data_ptr(), alloc_lens.data_ptr(),
             free_pages.data_ptr(), free_pages.numel(), free_range.data_ptr(), req_to_token.data_ptr(), req_to_token.stride(0), rows, max_ctx,
             page_at, page_stride, parents_at, mask_at, words, positions.data_ptr(), out_cache_loc.data_ptr(), capacity, cu_seqlens_q.data_ptr(),
@@ -773,7 +772,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     need = 0
     if workspace is None:
         splits = _lib.msgl_tree_attention_splits(bs, max_seqlen_q, max_seqlen_k, total_kv, Hq, Hkv)
-        need = 4 * (D + 2) * T * Hq * splits if splits > 1 else 0
+        need = _lib.msgl_tree_attention_workspace_bytes(T, Hq, D, splits) if splits > 1 else 0
     ws, ws_at, ws_bytes = _scratch(workspace, need, index)
     _launch(index, _lib.msgl_tree_attention, q.data_ptr(), q.stride(0) if T > 1 else Hq * D, k_cache.data_ptr(), v_cache.data_ptr(), cs,
             req_to_token.data_ptr(), req_to_token.stride(0), req_pool_indices.data_ptr(), cu_seqlens_q.data_ptr(), prefix_lens.data_ptr(),

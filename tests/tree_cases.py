@@ -59,7 +59,7 @@ def attention_case(nodes, prefix, Hq, Hkv, page_size, seed, layout="interleaved"
     else:
         k, v = (torch.randn(slots, Hkv, D, generator=g).to(torch.bfloat16) for _ in range(2))
     q = (torch.randn(sum(nodes), Hq, D, generator=g) * 1.5).to(torch.bfloat16)
-    masks = [m for n in nodes for m in ancestor_masks(tree_parents(rng, n, chain))]
+    masks = [m for n in nodes for m in ancestor_masks(tree_parents(rng, n, chain)[:n])]
     words = words or max(1, -(-max(nodes) // 64))
     return dict(q=q, k=k, v=v, r2t=r2t, rows=torch.tensor(rows, dtype=torch.int32), cu=cumulative(nodes), prefix=torch.tensor(prefix, dtype=torch.int32),
                 mask=pack_masks(masks, words), masks=masks, nodes=list(nodes), prefix_list=list(prefix), scale=D ** -0.5)
