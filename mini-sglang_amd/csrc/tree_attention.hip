@@ -16,7 +16,8 @@
 //     slots per wave; the XOR swizzles that spread the fragment reads over the banks are applied to the source address.
 //   * The page table is read per token, also by LDS-DMA, four tiles ahead: any page size, no scalar path, nothing the compiler counts.
 //   * All these loads are inline asm and waited for by count; their order is K0 V0 t3 K1 V1 | t4 K2 V2 | t5 K3 V3 ... (t = table entries).
-// Long contexts are cut into runs of keys (one work group each) that leave (O, max, sum) in the workspace; a second kernel joins them.
+// Where requests are few or unequal, their tiles are dealt in equal shares (TreeWalk, tree_cut); runs of a request leave (O, max, sum) in the
+// workspace and a second kernel joins them.
 #include <type_traits>
 #include <utility>
 
@@ -32,6 +33,8 @@ constexpr int kTreeRing = 4 * kTreeHalf;            // per wave: two K tiles, tw
 constexpr int kTreeSlotRing = 4 * 256;              // per wave: table entries of four tiles (64 words each)
 constexpr int kTreeMergeRow = kHD + 4;              // floats per row of the exchange at the end (spread over the banks)
 constexpr int merge_bytes(int waves, int rb) { return waves * 32 * rb * (kTreeMergeRow + 2) * 4; }
+constexpr int kTreeBegin = 16;                      // tiles that the start of a run is worth (TreeWalk)
+constexpr int kLeastTiles = 4;                      // least tiles of a share: one per wave of the narrow kernel
 constexpr float kRescaleAt = 8.f;                   // log2 units a row's maximum may outgrow its reference before O is rescaled
 
 struct TreeParams {
@@ -51,8 +54,9 @@ struct TreeParams {
     int64_t out_stride;
     float* ws_o;   // [token][head][split][128]
     float* ws_ml;  // [token][head][split][2]
+    int32_t* ws_n; // [token][head]: runs
     int bs, Hq, Hkv, group;
-    int items, row_tiles, splits, chunk;
+    int items, row_tiles, splits, shares;
     int max_q;
     float scale_log2e;
 };
@@ -102,24 +106,127 @@ __device__ __forceinline__ uint32_t mask_bits(const uint64_t* row, int words, in
     return (uint32_t)v;
 }
 
-// What a work group is asked for: one request's run of keys [t0, t1) against rows r0 .. of a kv head, as (node, head) pairs.
+// What a work group does at a time: one request's run of keys [t0, t1) against rows r0 .. of a kv head, as (node, head) pairs.
 struct TreeItem {
     int b, base, n, rows, r0, prefix, t0, t1, split, nsplit;
-    bool none;
+    const int32_t* table;
 };
-__device__ __forceinline__ TreeItem tree_item(const TreeParams& p, int b, int split, int r0) {
-    TreeItem it;
-    it.b = b, it.split = split, it.r0 = r0;
-    it.base = p.cu[b];
-    it.n = min(p.cu[b + 1] - it.base, p.max_q);
-    it.rows = it.n * p.group;
-    it.prefix = max(p.prefix[b], 0);
-    const int S = it.prefix + it.n;
-    it.nsplit = min((S + p.chunk - 1) / p.chunk, p.splits);
-    it.none = r0 >= it.rows || split >= it.nsplit;
-    it.t0 = split * p.chunk;
-    it.t1 = split == p.splits - 1 ? S : min(S, it.t0 + p.chunk);
-    return it;
+
+// A request's lengths, and its tiles as far as it has rows from r0 on.
+struct TreeRequest {
+    int base, n, prefix, row, tiles;
+    __device__ __forceinline__ TreeRequest(const TreeParams& p, int b, int r0) {
+        base = p.cu[b], n = min(p.cu[b + 1] - base, p.max_q), prefix = max(p.prefix[b], 0), row = p.req_idx[b];
+        tiles = n * p.group > r0 ? (prefix + n + kTreeKeys - 1) / kTreeKeys : 0;
+    }
+};
+
+// Sum (maximum) of the lanes up to and including each, of values that are not negative.
+template <bool MAX>
+__device__ __forceinline__ int lanes_up_to(int x) {
+#define MSGL_TREE_SCAN(ctrl, rows)                                               \
+    {                                                                            \
+        const int y = __builtin_amdgcn_update_dpp(0, x, ctrl, rows, 0xf, false); \
+        x = MAX ? max(x, y) : x + y;                                             \
+    }
+    MSGL_TREE_SCAN(0x111, 0xf)  // within rows of 16 lanes: 1, 2, 4, 8 down
+    MSGL_TREE_SCAN(0x112, 0xf)
+    MSGL_TREE_SCAN(0x114, 0xf)
+    MSGL_TREE_SCAN(0x118, 0xf)
+    MSGL_TREE_SCAN(0x142, 0xa)  // the last lane of rows 0 and 2 into rows 1 and 3
+    MSGL_TREE_SCAN(0x143, 0xc)  // the last lane of row 1 into rows 2 and 3
+#undef MSGL_TREE_SCAN
+    return x;
+}
+
+// The way of a work group through the batch.  splits == 1: it has request `share` to itself.  Otherwise the requests' tiles lie end to end and
+// share k of them is [k len, (k + 1) len): every work group has the same number of tiles, whatever the requests' lengths are, a share holds the
+// end of one request, whole ones and the beginning of another, and a request is in at most `splits` shares.  To begin with a request costs about
+// as much as kTreeBegin tiles, and as many are counted in front of it; where shares of that length suffice with every request beginning a share of
+// its own, it does (its last share is then the shorter).  Every wave finds all this out by itself.
+struct TreeWalk {
+    int share, len, begin, b, base, tiles, at, end;  // base, tiles: first tile of request b in that order, and how many; at, end: of the share's tiles left
+    bool any;                                        // `it` holds a run
+    __device__ __forceinline__ int span(int real) const { return real == 0 ? 0 : begin ? real + begin : (int)((unsigned)(real + len - 1) / (unsigned)len) * len; }
+    __device__ __forceinline__ TreeWalk(const TreeParams& p, int k, int r0, int lane, TreeItem& it) {
+        share = 0, len = 1, begin = 0, b = k, base = 0, at = 0, end = 0, any = false;
+        if (p.splits == 1) {
+            const TreeRequest rq(p, k, r0);
+            len = max(rq.tiles, 1), end = rq.tiles;
+            take(p, rq, r0, it);
+            return;
+        }
+        begin = kTreeBegin;
+        const TreeRequest mine(p, min(lane, p.bs - 1), r0);
+        const int real = lane < p.bs ? mine.tiles : 0;
+        int first = span(real), upto = lanes_up_to<false>(first);
+        int total = __builtin_amdgcn_readlane(upto, 63), longest = first;
+        for (int b0 = 64; b0 < p.bs; b0 += 64) {
+            const int t = b0 + lane < p.bs ? span(TreeRequest(p, b0 + lane, r0).tiles) : 0;
+            total += __builtin_amdgcn_readlane(lanes_up_to<false>(t), 63), longest = max(longest, t);
+        }
+        share = k;
+        len = max((int)((unsigned)(total + p.shares - 1) / (unsigned)p.shares), kLeastTiles);
+        if (__any(longest > (int64_t)(p.splits - 1) * len))  // (the batch is longer than the bounds said)
+            len = (__builtin_amdgcn_readlane(lanes_up_to<true>(longest), 63) + p.splits - 2) / (p.splits - 1);
+        if (p.bs <= 64) {
+            const int own = (int)((unsigned)(real + len - 1) / (unsigned)len), own_upto = lanes_up_to<false>(own);
+            const int shares = __builtin_amdgcn_readlane(own_upto, 63);
+            if (shares <= p.shares) begin = 0, first = own * len, upto = own_upto * len, total = shares * len;
+        }
+        if ((int64_t)k * len >= total) return;
+        at = k * len, end = min(total - at, len) + at;
+        const uint64_t behind = __ballot(upto > at);  // the request that tile `at` belongs to
+        if (behind) {
+            b = __ffsll((unsigned long long)behind) - 1, base = __builtin_amdgcn_readlane(upto - first, b);
+            TreeRequest rq = mine;  // (the loads above brought it already)
+            rq.base = __builtin_amdgcn_readlane(mine.base, b), rq.n = __builtin_amdgcn_readlane(mine.n, b), rq.row = __builtin_amdgcn_readlane(mine.row, b);
+            rq.prefix = __builtin_amdgcn_readlane(mine.prefix, b), rq.tiles = __builtin_amdgcn_readlane(mine.tiles, b);
+            take(p, rq, r0, it);
+            return;
+        }
+        base = __builtin_amdgcn_readlane(upto, 63);
+        for (int b0 = 64; b0 < p.bs; b0 += 64) {
+            const int own = b0 + lane < p.bs ? span(TreeRequest(p, b0 + lane, r0).tiles) : 0;
+            const int sum = lanes_up_to<false>(own);
+            const uint64_t there = __ballot(base + sum > at);
+            if (there) {
+                const int l = __ffsll((unsigned long long)there) - 1;
+                b = b0 + l, base += __builtin_amdgcn_readlane(sum - own, l);
+                break;
+            }
+            base += __builtin_amdgcn_readlane(sum, 63);
+        }
+        take(p, TreeRequest(p, b, r0), r0, it);
+    }
+    // The run of request b (rq) that begins at tile `at`.
+    __device__ __forceinline__ void take(const TreeParams& p, const TreeRequest& rq, int r0, TreeItem& it) {
+        const int first = base + begin;
+        tiles = span(rq.tiles);
+        it.t0 = max(at - first, 0) * kTreeKeys;
+        const int from = (int)((unsigned)first / (unsigned)len);
+        it.split = share - from, it.nsplit = (int)((unsigned)(first + rq.tiles - 1) / (unsigned)len) - from + 1;
+        at = min(end, base + tiles);
+        it.t1 = min(rq.prefix + rq.n, (at - first) * kTreeKeys);
+        it.b = b, it.r0 = r0, it.base = rq.base, it.n = rq.n, it.rows = rq.n * p.group, it.prefix = rq.prefix;
+        it.table = p.r2t + (int64_t)rq.row * p.r2t_stride;
+        any = it.t0 < it.t1;
+    }
+    __device__ __forceinline__ void next(const TreeParams& p, int r0, TreeItem& it) {
+        any = false;
+        while (!any && at < end) {  // (a request without tiles is passed over)
+            base += tiles, ++b;
+            take(p, TreeRequest(p, b, r0), r0, it);
+        }
+    }
+};
+
+// The lane number, of which the compiler does not know that it is the same every time: what is derived from it is made anew for every request of a
+// share, instead of occupying (and spilling) registers all along.
+__device__ __forceinline__ int fresh_lane() {
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+    return lane;
 }
 
 // A wave's running state for RB blocks of 32 rows: O^T (dims 32 mb + 8 (i >> 2) + 4 half + (i & 3) in register i of block mb, row lane & 31),
@@ -315,11 +422,10 @@ __device__ __forceinline__ bool tile_values_masked(const char* vt, int lane, con
 // The values that are not finite, added to the rows that see them (a softmax weight is never 0, whatever 32 bits make of it).  o: this wave's rows in
 // LDS.  Runs only where a tile had such a value.
 __device__ __forceinline__ void add_odd_values(const TreeParams& p, const TreeItem& it, int row0, int rows, int h, int key0, int lane, float* o) {
-    const int32_t* table = p.r2t + (int64_t)p.req_idx[it.b] * p.r2t_stride;
     for (int r = lane; r < rows; r += 64) {
         const uint32_t see = row_sees(p, it, row0 + r, key0);
         for (int k = 0; k < kTreeKeys && key0 + k < it.t1; ++k) {
-            const uint16_t* v = reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(p.vc) + (uint64_t)(uint32_t)table[key0 + k] * p.slot_bytes) + h * kHD;
+            const uint16_t* v = reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(p.vc) + (uint64_t)(uint32_t)it.table[key0 + k] * p.slot_bytes) + h * kHD;
             for (int d = 0; d < kHD; ++d)
                 if ((v[d] & 0x7f80u) == 0x7f80u && (see >> k & 1)) o[r * kTreeMergeRow + d] += bf16_lo(v[d]);
         }
@@ -376,6 +482,7 @@ __device__ __forceinline__ void join_and_store(const TreeParams& p, const TreeIt
         const int node = row / p.group;
         const int hq = head(g) * p.group + row - node * p.group;
         const int64_t tok = it.base + node;
+        if (p.splits > 1 && it.split == 0 && d == 0) p.ws_n[tok * p.Hq + hq] = it.nsplit;
         if (it.nsplit == 1) {
             const float inv = L == 0.f ? 0.f : 1.0f / L;  // L == 0: the row sees nothing
             *reinterpret_cast<uint2*>(p.out + tok * p.out_stride + hq * kHD + d) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
@@ -390,13 +497,12 @@ __device__ __forceinline__ void join_and_store(const TreeParams& p, const TreeIt
 template <int RB>
 __global__ __launch_bounds__(kTreeWaves * 64, 1) void tree_attention_kernel(TreeParams p) {
     extern __shared__ __attribute__((aligned(1024))) char smem[];
-    // block -> (kv head, run of keys, request), heads fastest: a token row's pieces are read at about the same time
+    // block -> (kv head, share), heads fastest: a token row's pieces are read at about the same time
     const int h = blockIdx.x % (unsigned)p.Hkv;
-    const int id = blockIdx.x / (unsigned)p.Hkv;
-    const TreeItem it = tree_item(p, id / p.splits, id % p.splits, 0);
-    if (it.none) return;
-    const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    TreeItem it;
+    for (TreeWalk walk(p, blockIdx.x / (unsigned)p.Hkv, 0, threadIdx.x & 63, it); walk.any; __syncthreads(), walk.next(p, 0, it)) {
+    const int lane = fresh_lane();
     const int g4 = lane >> 4, q16 = lane & 15;
     const int all_tiles = (it.t1 - it.t0 + kTreeKeys - 1) / kTreeKeys;
     const int T = all_tiles > wave ? (all_tiles - wave + kTreeWaves - 1) / kTreeWaves : 0;  // own tiles: wave, wave + kTreeWaves, ...
@@ -412,7 +518,7 @@ __global__ __launch_bounds__(kTreeWaves * 64, 1) void tree_attention_kernel(Tree
     uint64_t odd = 0;  // tiles behind the plain ones that held a value that is not finite
     const int plain = (max(0, (min(it.prefix, it.t1) - it.t0) / kTreeKeys - wave) + kTreeWaves - 1) / kTreeWaves;  // own tiles that every row sees whole
     if (T > 0) {
-        const int32_t* table = p.r2t + (int64_t)p.req_idx[it.b] * p.r2t_stride;
+        const int32_t* table = it.table;
         // table entries of own tile j, lane (g4', i) <- key 4 i + g4' of the tile, so that a lane of the K/V loads finds its eight rows'
         // entries in 32 consecutive bytes.  Positions behind the run's last key repeat that key.
         const int word_key = 4 * (lane & 7) + ((lane >> 3) & 3);
@@ -490,6 +596,7 @@ __global__ __launch_bounds__(kTreeWaves * 64, 1) void tree_attention_kernel(Tree
     wait_loads<0>();
     join_and_store<RB, kTreeWaves, kTreeWaves>(p, it, st, smem, wave, lane, odd, it.t0 + (wave + plain * kTreeWaves) * kTreeKeys, kTreeWaves * kTreeKeys, [](int) { return 0; },
                             [&](int) { return h; });
+    }
 }
 
 // More than 64 rows per kv head: the NW waves hold 32 rows each and share the tiles, so that K and V are read once per 32 NW rows.  A tile is loaded by
@@ -539,11 +646,10 @@ __global__ __launch_bounds__(NW * 64, 2) void tree_attention_wide_kernel(TreePar
     const int item = (y / p.row_tiles) * 8 + (blockIdx.x & 7);
     if (item >= p.items) return;
     const int h = item % p.Hkv;
-    const int id = item / p.Hkv;
-    const TreeItem it = tree_item(p, id / p.splits, id % p.splits, rt * 32 * NW);
-    if (it.none) return;
-    const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    TreeItem it;
+    for (TreeWalk walk(p, item / p.Hkv, rt * 32 * NW, threadIdx.x & 63, it); walk.any; __syncthreads(), walk.next(p, rt * 32 * NW, it)) {
+    const int lane = fresh_lane();
     const int g4 = lane >> 4, q16 = lane & 15;
     const int row0 = it.r0 + wave * 32;
     const int T = (it.t1 - it.t0 + kTreeKeys - 1) / kTreeKeys;
@@ -551,7 +657,7 @@ __global__ __launch_bounds__(NW * 64, 2) void tree_attention_wide_kernel(TreePar
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
     char* words = smem + W::kRing + wave * 512;
     const uint32_t words_at = lds0 + W::kRing + wave * 512;
-    const int32_t* table = p.r2t + (int64_t)p.req_idx[it.b] * p.r2t_stride;
+    const int32_t* table = it.table;
     // entry kKeys t + kLoads g4' + i of a block: key kKeys wave + 4 i + g4' of the block's tile t
     const int in_tile = lane % W::kKeys;
     const int word_key = lane / W::kKeys * kTreeKeys + W::kKeys * wave + 4 * (in_tile % W::kLoads) + in_tile / W::kLoads;
@@ -723,6 +829,7 @@ __global__ __launch_bounds__(NW * 64, 2) void tree_attention_wide_kernel(TreePar
     }
     wait_loads<0>();
     join_and_store<1, 1, NW>(p, it, st, smem, wave, lane, odd, it.t0 + plain * kTreeKeys, kTreeKeys, [&](int g) { return it.r0 + g * 32; }, [&](int) { return h; });
+    }
 }
 
 // Joins the runs of a (token, head): GROUPS half-waves per row take every GROUPS-th run, four dims per lane, and meet in LDS.
@@ -739,9 +846,9 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeParams p) {
     if (b < p.bs) {
         base = p.cu[b];
         n = min(p.cu[b + 1] - base, p.max_q);
-        nsplit = min((max(p.prefix[b], 0) + n + p.chunk - 1) / p.chunk, p.splits);
     }
     const int node = r / p.Hq, hq = r - node * p.Hq;
+    if (node < n) nsplit = p.ws_n[(int64_t)(base + node) * p.Hq + hq];
     const bool live = node < n && nsplit > 1;  // (one run: written by the first kernel)
     const int64_t at = ((int64_t)(base + node) * p.Hq + hq) * p.splits;
     float M = kNegBigE, L = 0.f;
@@ -835,19 +942,34 @@ static TreeShape tree_shape(int max_q, int Hq, int Hkv) {
     return s;
 }
 
-// Runs of keys per request: about one work group per compute unit in all, each run at least four tiles long.  More runs even out unequal requests
-// but cost partial results: measured with 16 requests of 2000 to 4000 tokens x 16 nodes (32 / 8 heads) 61, 67, 84, 111 us at one, two, four and eight
-// groups per unit, 64 requests of 4096 to 8192 x 8 nodes 285, 308, 315, 339 us, 2 x 32 nodes x 130001 tokens (8 / 1 heads) 60, 87 us at one and two.
-static int tree_splits(int bs, int max_q, int max_k, int64_t total_kv, int Hq, int Hkv) {
-    if (bs <= 0 || max_q <= 0 || max_k <= 0 || Hkv <= 0 || Hq < Hkv) return 1;
+// How a launch is cut: work groups per (kv head, row tile), and most runs of a request (1: a work group per request).
+struct TreeCut {
+    int shares, splits;
+};
+// A work group per request, or equal shares of all tiles, one per compute unit: whichever is done sooner, counted in tiles.  A run costs its tiles
+// and kTreeBegin for its start; a second kernel has to join shared requests, which is worth kJoin tiles (4 to 8 us; a tile takes a narrow work
+// group 0.3 us, a wide one 1.1 us).  Both sides measured, in us, work group per request | shares:
+//   16 requests of 2000 to 4000 tokens x 16 nodes, 32 / 8 heads (128 work groups)      60 (equal runs of 1500 keys) | 47
+//   12 of 8000 to 16000 x 30 (96)  138 (same) | 112      3 of 15000 to 30000 x 70, 16 / 4 heads (24)  124 (same) | 90
+//   64 of 500 to 1000 x 8 (512)  44 | 55      64 of 4096 to 8192 x 8 (512)  280 | 278      32 of 250 to 500 x 60 (256)  34 | 41
+//   1 of 1000 x 4, 16 / 8 heads (8)  15 | 20      1 of 2000 x 4 (8)  20 | 20      1 of 500 x 60 (8)  28 | 24      7 of 500 to 1000 x 4 (56)  17 | 19
+static TreeCut tree_cut(int bs, int max_q, int max_k, int64_t total_kv, int Hq, int Hkv) {
+    const TreeCut whole = {bs, 1};
+    if (bs <= 0 || max_q <= 0 || max_k <= 0 || Hkv <= 0 || Hq < Hkv) return whole;
     const TreeShape sh = tree_shape(max_q, Hq, Hkv);
-    const int64_t keys = total_kv > 0 && total_kv < (int64_t)bs * max_k ? total_kv : (int64_t)bs * max_k;
-    const int64_t per_key = (int64_t)Hkv * sh.row_tiles;
-    const int64_t want = device_cus();
-    int64_t chunk = (keys * per_key + want - 1) / want;
-    if (chunk < kTreeKeys * kTreeWaves) chunk = kTreeKeys * kTreeWaves;
-    int64_t splits = (max_k + chunk - 1) / chunk;
-    return (int)(splits < kMaxTreeSplits ? splits : kMaxTreeSplits);
+    const int64_t units = device_cus(), across = (int64_t)Hkv * sh.row_tiles;
+    const int64_t most = ((int64_t)max_k + kTreeKeys - 1) / kTreeKeys;
+    const int64_t tiles = total_kv > 0 && total_kv < (int64_t)bs * max_k ? total_kv / kTreeKeys + bs : bs * most;
+    const int64_t mean = (tiles + bs - 1) / bs;
+    const int64_t all = tiles + (int64_t)bs * kTreeBegin;
+    const int64_t least = sh.waves ? 6 : kLeastTiles, kJoin = sh.waves ? 6 : 28;
+    int64_t shares = across < units ? units / across : 1;
+    if (shares > (all + least - 1) / least) shares = (all + least - 1) / least;
+    const int64_t len = (all + shares - 1) / shares;
+    const int64_t alone = bs * across <= units ? kTreeBegin + most : (kTreeBegin + mean) * bs * across / units + most - mean;
+    if (alone <= kTreeBegin + len + kJoin) return whole;
+    const int64_t splits = (most + len - 1) / len + 1;
+    return {(int)shares, (int)(splits < kMaxTreeSplits ? splits : kMaxTreeSplits)};
 }
 
 }  // namespace msgl
@@ -855,11 +977,11 @@ static int tree_splits(int bs, int max_q, int max_k, int64_t total_kv, int Hq, i
 using namespace msgl;
 
 extern "C" int msgl_tree_attention_splits(int bs, int max_seqlen_q, int max_seqlen_k, int64_t total_kv, int Hq, int Hkv) {
-    return tree_splits(bs, max_seqlen_q, max_seqlen_k, total_kv, Hq, Hkv);
+    return tree_cut(bs, max_seqlen_q, max_seqlen_k, total_kv, Hq, Hkv).splits;
 }
 extern "C" size_t msgl_tree_attention_workspace_bytes(int64_t total_tokens, int Hq, int D, int splits) {
     if (total_tokens <= 0 || Hq <= 0 || D <= 0 || splits <= 1) return 0;
-    return (size_t)total_tokens * Hq * splits * (D + 2) * sizeof(float);
+    return (size_t)total_tokens * Hq * ((size_t)splits * (D + 2) + 1) * sizeof(float);
 }
 
 extern "C" int msgl_tree_attention(const void* q, int64_t q_stride, const void* k_cache, const void* v_cache, int64_t cache_stride,
@@ -895,17 +1017,20 @@ extern "C" int msgl_tree_attention(const void* q, int64_t q_stride, const void* 
     const TreeShape sh = tree_shape(max_seqlen_q, Hq, Hkv);
     p.row_tiles = sh.row_tiles;
     p.scale_log2e = scale * 1.44269504088896340736f;
-    int splits = tree_splits(bs, max_seqlen_q, max_seqlen_k, total_kv, Hq, Hkv);
-    // as many runs as the workspace has room for
-    const size_t one = (size_t)total_tokens * Hq * (D + 2) * sizeof(float);
-    const size_t room = workspace ? workspace_bytes / one : 0;
-    if ((size_t)splits > room) splits = room > 1 ? (int)room : 1;
-    p.splits = splits;
-    p.chunk = (((max_seqlen_k + splits - 1) / splits) + kTreeKeys - 1) / kTreeKeys * kTreeKeys;
+    TreeCut cut = tree_cut(bs, max_seqlen_q, max_seqlen_k, total_kv, Hq, Hkv);
+    if (cut.splits > 1) {  // as many runs as the workspace has room for
+        const size_t per_row = workspace ? workspace_bytes / sizeof(float) / ((size_t)total_tokens * Hq) : 0;
+        const size_t room = per_row ? (per_row - 1) / (D + 2) : 0;
+        if ((size_t)cut.splits > room) cut.splits = (int)room;
+        if (cut.splits < 2) cut = {bs, 1};
+    }
+    const int splits = cut.splits;
+    p.splits = splits, p.shares = cut.shares;
     p.ws_o = static_cast<float*>(workspace);
     p.ws_ml = p.ws_o + (splits > 1 ? (size_t)total_tokens * Hq * splits * kHD : 0);
+    p.ws_n = reinterpret_cast<int32_t*>(p.ws_ml + (splits > 1 ? (size_t)total_tokens * Hq * splits * 2 : 0));
     MSGL_REQUIRE(splits == 1 || aligned16(workspace), "msgl_tree_attention: workspace must be 16-byte aligned");
-    const int64_t items = (int64_t)bs * splits * Hkv;
+    const int64_t items = (int64_t)cut.shares * Hkv;
     const int64_t blocks = sh.waves ? (items + 7) / 8 * 8 * p.row_tiles : items;
     MSGL_REQUIRE(blocks <= 0x7fffff, "msgl_tree_attention: %lld work groups", (long long)blocks);
     p.items = (int)items;

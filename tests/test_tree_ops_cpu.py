@@ -100,7 +100,7 @@ def test_nothing_to_do_is_no_error_and_needs_no_workspace():
     assert _call("msgl_token_logprobs", LOGPROBS, LOGPROBS_OK, dict(rows=0))[0] == 0
     lib, _ = _lib()
     assert lib.msgl_prepare_extend_workspace_bytes(1024, 4096, 1 << 20) == 0 and lib.msgl_prepare_extend_workspace_bytes(1025, 1, 64) == 1025 * 16
-    assert lib.msgl_tree_attention_workspace_bytes(10, 8, 128, 1) == 0 and lib.msgl_tree_attention_workspace_bytes(10, 8, 128, 3) == 10 * 8 * 3 * 130 * 4
+    assert lib.msgl_tree_attention_workspace_bytes(10, 8, 128, 1) == 0 and lib.msgl_tree_attention_workspace_bytes(10, 8, 128, 3) == 10 * 8 * (3 * 130 + 1) * 4
     assert lib.msgl_token_logprobs_workspace_bytes(0, 100, 2, 0) == 0
 
 
