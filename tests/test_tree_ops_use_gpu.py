@@ -211,3 +211,28 @@ def test_wrappers_refuse():
         ops.prepare_extend(*args, 16, parents=_i32([0, 0]), tree_mask=torch.zeros(2, 17, dtype=torch.int64, device=DEV))
     with pytest.raises(Exception, match="overwrites"):
         ops.prepare_extend(*args[:10], args[1], args[11], 16)
+
+
+@pytest.mark.parametrize("bs,longest,most,Hq,Hkv", [(70, 2500, 6, 4, 1), (130, 900, 12, 8, 1), (9, 6000, 20, 8, 4), (5, 4000, 70, 16, 2), (3, 9000, 1, 8, 8)])
+def test_shares_of_unequal_requests(bs, longest, most, Hq, Hkv):
+    """Requests of very different length, some without nodes: work groups that end one request and begin others, row tiles that not every request
+    has, more requests than lanes; with the whole workspace, with room for a few runs per request only, and with wrong hints."""
+    ops = _ops()
+    rng = random.Random(bs)
+    nodes = [0 if rng.random() < 0.15 else rng.randint(1, most) for _ in range(bs)]
+    nodes[rng.randrange(bs)] = most
+    prefix = [int(longest * rng.random() ** 3) for _ in range(bs)]
+    prefix[bs // 2] = longest
+    c = tc.attention_case(nodes, prefix, Hq, Hkv, 16, bs)
+    a = _args(c)
+    total = sum(n + p for n, p in zip(nodes, prefix))
+    splits = ops.tree_attention_splits(bs, max(nodes), a[9], Hq, Hkv, total)
+    assert splits > 1
+    first = ops.tree_attention(*a, total_kv=total)
+    _check(first, c)
+    assert torch.equal(first, ops.tree_attention(*a, total_kv=total))
+    for room in (1, 2, 3, splits + 5):
+        ws = torch.empty(ops.tree_attention_workspace_bytes(sum(nodes), Hq, D, room) + 16, dtype=torch.uint8, device=DEV)
+        _check(ops.tree_attention(*a, total_kv=total, workspace=ws), c)
+    a[9] = longest // 3
+    _check(ops.tree_attention(*a, total_kv=total // 4), c)
