@@ -149,7 +149,30 @@ __device__ __forceinline__ float piece_value(const uint4& v, int e) {
     return e & 1 ? bf16_hi(w[e >> 1]) : bf16_lo(w[e >> 1]);
 }
 
-template <int BYTES, int LOADS>
+// A row's results from its sums against `ref`.
+struct RowResult {
+    double ref, lnz;
+    __device__ __forceinline__ RowResult(const LogprobParams& p, int64_t row, int bytes, double ref_, float z, float t) : ref(ref_) {
+        if (z == 0.f) z = __builtin_nanf("");  // no element above -inf
+        lnz = (double)logf(z);
+        if (threadIdx.x != 0) return;
+        const int token = p.tokens[row];
+        float x = __builtin_nanf("");
+        if ((unsigned)token < (unsigned)p.vocab) {
+            const char* at = p.logits + row * p.row_bytes + (int64_t)token * bytes;
+            x = bytes == 4 ? *reinterpret_cast<const float*>(at) : bf16_lo(*reinterpret_cast<const uint16_t*>(at));
+        }
+        p.logprobs[row] = (float)(((double)x - ref) - lnz);
+        p.entropy[row] = logf(z) - t / z;
+    }
+    __device__ __forceinline__ void put(const LogprobParams& p, int64_t row, int rank, uint64_t key) const {
+        p.top_ids[row * p.top + rank] = (int32_t)~(uint32_t)key;
+        p.top_logprobs[row * p.top + rank] = (float)(((double)key_value((uint32_t)(key >> 32)) - ref) - lnz);
+    }
+};
+
+// WHOLE: the segment is the whole row, and its results are final.
+template <int BYTES, int LOADS, bool WHOLE>
 __global__ __launch_bounds__(kLpThreads) void logprob_segment_kernel(LogprobParams p) {
     constexpr int E = 16 / BYTES;                     // elements per piece
     constexpr int kPieces = kLpThreads * LOADS;       // pieces per segment
@@ -232,11 +255,20 @@ __global__ __launch_bounds__(kLpThreads) void logprob_segment_kernel(LogprobPara
     z = t = 0.f;
 #pragma unroll
     for (int w = 0; w < kLpWaves; ++w) z += lds_f[w][0], t += lds_f[w][1];
-    if (tid == 0) p.stats[row * p.segments + seg] = SegmentStats{tame ? (double)ref2 * kLn2d : (double)ref, z, t * kLn2};
+    const double reference = tame ? (double)ref2 * kLn2d : (double)ref;
+    std::conditional_t<WHOLE, RowResult, SegmentStats> result = [&] {
+        if constexpr (WHOLE) return RowResult(p, row, BYTES, reference, z, t * kLn2);
+        else return SegmentStats{reference, z, t * kLn2};
+    }();
+    if constexpr (!WHOLE) {
+        if (tid == 0) p.stats[row * p.segments + seg] = result;
+    }
     if (p.top == 0) return;
 
-    uint64_t* out = p.keys + (row * p.segments + seg) * p.top;
-    auto put = [&](int rank, uint64_t key) { out[rank] = key; };
+    auto put = [&](int rank, uint64_t key) {
+        if constexpr (WHOLE) result.put(p, row, rank, key);
+        else p.keys[(row * p.segments + seg) * p.top + rank] = key;
+    };
     bool few = z == z;  // (NaN or infinities in the segment: no sum, and no plain order)
     if (few) {
         // candidates: values at or above the bar; with `ties` only values above it, and of those at it the ones within the first pieces
@@ -311,7 +343,7 @@ __global__ __launch_bounds__(kLpThreads) void logprob_segment_kernel(LogprobPara
         }
         last = block_max_key(offer, found.key[0]);
         stale = offer == last;
-        if (tid == 0) out[k] = last;  // 0: the segment has fewer elements
+        if (tid == 0) put(k, last);  // 0: the segment has fewer elements
     }
 }
 
@@ -336,24 +368,10 @@ __global__ __launch_bounds__(kLpThreads) void logprob_row_kernel(LogprobParams p
         t += f * (e.t + fmaxf(d, -200.f) * e.z);
     }
     z = wave_sum(z), t = wave_sum(t);
-    if (z == 0.f) z = __builtin_nanf("");  // no element above -inf
-    const double lnz = (double)logf(z);
-    if (tid == 0) {
-        const int token = p.tokens[row];
-        float x = __builtin_nanf("");
-        if ((unsigned)token < (unsigned)p.vocab) {
-            const char* at = p.logits + row * p.row_bytes + (int64_t)token * bytes;
-            x = bytes == 4 ? *reinterpret_cast<const float*>(at) : bf16_lo(*reinterpret_cast<const uint16_t*>(at));
-        }
-        p.logprobs[row] = (float)(((double)x - ref) - lnz);
-        p.entropy[row] = logf(z) - t / z;
-    }
+    const RowResult result(p, row, bytes, ref, z, t);
     if (p.top == 0) return;
     const uint64_t* keys = p.keys + row * p.segments * p.top;
-    auto put = [&](int rank, uint64_t key) {
-        p.top_ids[row * p.top + rank] = (int32_t)~(uint32_t)key;
-        p.top_logprobs[row * p.top + rank] = (float)(((double)key_value((uint32_t)(key >> 32)) - ref) - lnz);
-    };
+    auto put = [&](int rank, uint64_t key) { result.put(p, row, rank, key); };
     // the k-th largest of some k or more of the keys bounds the k-th largest of all from below: of the segments' best ones, as many per
     // segment as it takes
     if (tid < 64) {
@@ -388,15 +406,18 @@ __global__ __launch_bounds__(kLpThreads) void logprob_row_kernel(LogprobParams p
     }
 }
 
-// Elements per thread: 32, or 16 where that would be fewer than four groups per compute unit.  Measured on a vocabulary of 151936 with five
+// Elements per thread: as many as it takes for the whole row if 32 will do (one launch instead of two: a bf16 row of 8000 tokens with five alternatives 7.8 -> 4.3 us, and 4.5 us of host time less), else 32, or 16
+// where that would be fewer than four groups per compute unit.  Measured on a vocabulary of 151936 with five
 // alternatives, us with 16 / 32 / 64 elements per thread: one bf16 row 8.3 / 9.4 / 10.1, 32 rows 10.6 / 11.2 / 12.2, 64 rows 14.2 / 13.5 / 15.1, 1000 rows
 // 94 / 87 / 91; fp32 with 8 / 16 / 32: one row 8.8 / 8.7 / 8.9, 32 rows 13.9 / 11.8 / 12.1, 64 rows 18.3 / 16.1 / 15.6, 1000 rows 153 / 114 / 105.
-static int logprob_elements(int rows, int vocab) {
+static bool logprob_fits(int vocab, int bytes, int elements) { return (int64_t)vocab + 16 / bytes - 1 <= elements * kLpThreads; }
+static int logprob_elements(int rows, int vocab, int bytes) {
+    if (logprob_fits(vocab, bytes, 32)) return logprob_fits(vocab, bytes, 16) ? 16 : 32;
     const int64_t segments = ((int64_t)vocab + 32 * kLpThreads - 1) / (32 * kLpThreads);
     return rows * segments < 4 * (int64_t)device_cus() ? 16 : 32;
 }
 static int logprob_segments(int rows, int vocab, int bytes) {
-    const int64_t per = (int64_t)kLpThreads * logprob_elements(rows, vocab);
+    const int64_t per = (int64_t)kLpThreads * logprob_elements(rows, vocab, bytes);
     return (int)(((int64_t)vocab + 16 / bytes - 1 + per - 1) / per);  // (a row's first piece may begin up to 16 / bytes - 1 elements early)
 }
 
@@ -406,7 +427,8 @@ using namespace msgl;
 
 extern "C" size_t msgl_token_logprobs_workspace_bytes(int rows, int vocab, int elem_bytes, int top) {
     if (rows <= 0 || vocab <= 0 || (elem_bytes != 2 && elem_bytes != 4) || top < 0) return 0;
-    return (size_t)rows * logprob_segments(rows, vocab, elem_bytes) * (sizeof(SegmentStats) + (size_t)top * sizeof(uint64_t));
+    const int segments = logprob_segments(rows, vocab, elem_bytes);
+    return segments == 1 ? 0 : (size_t)rows * segments * (sizeof(SegmentStats) + (size_t)top * sizeof(uint64_t));
 }
 
 extern "C" int msgl_token_logprobs(const void* logits, int64_t row_stride, int elem_bytes, const int32_t* token_ids, float* logprobs,
@@ -424,7 +446,7 @@ extern "C" int msgl_token_logprobs(const void* logits, int64_t row_stride, int e
     p.segments = logprob_segments(rows, vocab, elem_bytes);
     MSGL_REQUIRE((int64_t)rows * p.segments <= 0xffffffffll / kLpThreads, "msgl_token_logprobs: %d rows x %d segments", rows, p.segments);
     const size_t need = msgl_token_logprobs_workspace_bytes(rows, vocab, elem_bytes, top);
-    if (workspace == nullptr || workspace_bytes < need) {
+    if (need && (workspace == nullptr || workspace_bytes < need)) {
         set_error("msgl_token_logprobs: workspace %zu < %zu bytes", workspace_bytes, need);
         return MSGL_E_WORKSPACE;
     }
@@ -436,11 +458,20 @@ extern "C" int msgl_token_logprobs(const void* logits, int64_t row_stride, int e
     p.vocab = vocab, p.top = top;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const dim3 grid((unsigned)(rows * p.segments));
-    const bool most = logprob_elements(rows, vocab) == 32;
-    if (elem_bytes == 2 && most) hipLaunchKernelGGL((logprob_segment_kernel<2, 4>), grid, dim3(kLpThreads), 0, st, p);
-    else if (elem_bytes == 2) hipLaunchKernelGGL((logprob_segment_kernel<2, 2>), grid, dim3(kLpThreads), 0, st, p);
-    else if (most) hipLaunchKernelGGL((logprob_segment_kernel<4, 8>), grid, dim3(kLpThreads), 0, st, p);
-    else hipLaunchKernelGGL((logprob_segment_kernel<4, 4>), grid, dim3(kLpThreads), 0, st, p);
+    const bool most = logprob_elements(rows, vocab, elem_bytes) == 32, whole = p.segments == 1;
+    auto launch = [&](auto bytes, auto loads) {
+        constexpr int B = decltype(bytes)::value, L = decltype(loads)::value;
+        if (whole) hipLaunchKernelGGL((logprob_segment_kernel<B, L, true>), grid, dim3(kLpThreads), 0, st, p);
+        else hipLaunchKernelGGL((logprob_segment_kernel<B, L, false>), grid, dim3(kLpThreads), 0, st, p);
+    };
+    constexpr std::integral_constant<int, 2> two{};
+    constexpr std::integral_constant<int, 4> four{};
+    constexpr std::integral_constant<int, 8> eight{};
+    if (elem_bytes == 2 && most) launch(two, four);
+    else if (elem_bytes == 2) launch(two, two);
+    else if (most) launch(four, eight);
+    else launch(four, four);
+    if (whole) return check_launch("logprob_segment_kernel");
     hipLaunchKernelGGL(logprob_row_kernel, dim3((unsigned)rows), dim3(kLpThreads), 0, st, p, elem_bytes);
     return check_launch("token_logprobs kernels");
 }

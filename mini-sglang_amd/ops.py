@@ -761,7 +761,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     if T and not 0 < max_seqlen_q <= 64 * words:
         raise ValueError(f"max_seqlen_q {max_seqlen_q} outside 1..{64 * words} (64 nodes per mask word)")
     if out is None:
-        out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=index)
+        out = q.new_empty((T, Hq, D))
         out_stride = Hq * D
     else:
         if out.get_device() != index or out.dtype is not torch.bfloat16 or out.shape != q.shape or out.stride()[1:] != (D, 1):
@@ -855,13 +855,15 @@ def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, top_k: int = 0
     index = _gpu_index(logits, "logits")
     if logits.dtype is not torch.bfloat16 and logits.dtype is not torch.float32:
         raise ValueError(f"logits must be bf16 or fp32 (got {logits.dtype})")
-    rows, vocab, rs = _rows_view(logits, "logits")
+    if logits.dim() != 2 or (logits.shape[1] != 1 and logits.stride(1) != 1):
+        raise ValueError(f"logits must be 2-D with a dense last dim (got shape {tuple(logits.shape)}, strides {logits.stride()})")
+    rows, vocab = logits.shape
+    rs = logits.stride(0) if rows > 1 else vocab
     _i32_on(index, rows, "token_ids", token_ids)
     if not 0 <= top_k <= min(vocab, LOGPROBS_MAX_TOP):
         raise ValueError(f"top_k {top_k} outside 0..min(vocab, {LOGPROBS_MAX_TOP})")
-    logprobs, entropy = torch.empty((2, rows), dtype=torch.float32, device=index).unbind(0)
-    ids = torch.empty((rows, top_k), dtype=torch.int32, device=index)
-    top = torch.empty((rows, top_k), dtype=torch.float32, device=index)
+    logprobs, entropy = logits.new_empty(rows, dtype=torch.float32), logits.new_empty(rows, dtype=torch.float32)
+    ids, top = token_ids.new_empty((rows, top_k)), logits.new_empty((rows, top_k), dtype=torch.float32)
     if rows:
         size = 2 if logits.dtype is torch.bfloat16 else 4
         need = _lib.msgl_token_logprobs_workspace_bytes(rows, vocab, size, top_k) if workspace is None else 0

@@ -78,7 +78,7 @@ def test_accept_tree_refuses(change, words):
 
 
 LOGPROBS = "logits stride elem ids logprobs entropy top_ids top_lp rows vocab top ws ws_bytes stream".split()
-LOGPROBS_OK = dict(logits=A[0], stride=1000, elem=2, ids=A[1], logprobs=A[2], entropy=A[3], top_ids=A[4], top_lp=A[5], rows=3, vocab=1000, top=4, ws=A[6],
+LOGPROBS_OK = dict(logits=A[0], stride=20000, elem=2, ids=A[1], logprobs=A[2], entropy=A[3], top_ids=A[4], top_lp=A[5], rows=3, vocab=20000, top=4, ws=A[6],
                    ws_bytes=1 << 20, stream=None)
 
 
@@ -101,7 +101,8 @@ def test_nothing_to_do_is_no_error_and_needs_no_workspace():
     lib, _ = _lib()
     assert lib.msgl_prepare_extend_workspace_bytes(1024, 4096, 1 << 20) == 0 and lib.msgl_prepare_extend_workspace_bytes(1025, 1, 64) == 1025 * 16
     assert lib.msgl_tree_attention_workspace_bytes(10, 8, 128, 1) == 0 and lib.msgl_tree_attention_workspace_bytes(10, 8, 128, 3) == 10 * 8 * (3 * 130 + 1) * 4
-    assert lib.msgl_token_logprobs_workspace_bytes(0, 100, 2, 0) == 0
+    assert lib.msgl_token_logprobs_workspace_bytes(0, 100, 2, 0) == 0 and lib.msgl_token_logprobs_workspace_bytes(5, 8185, 2, 9) == 0  # one segment
+    assert lib.msgl_token_logprobs_workspace_bytes(5, 8186, 2, 9) > 0 and lib.msgl_token_logprobs_workspace_bytes(5, 8189, 4, 9) == 0
 
 
 def test_splits_follow_the_bounds():

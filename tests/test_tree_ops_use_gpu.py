@@ -184,7 +184,7 @@ def test_wrappers_refuse():
         with pytest.raises(ValueError, match=words):
             ops.token_logprobs(*args)
     with pytest.raises(Exception, match="workspace"):
-        ops.token_logprobs(x, tok, 2, workspace=torch.empty(16, dtype=torch.uint8, device=DEV))
+        ops.token_logprobs(torch.zeros(3, 10000, device=DEV), tok, 2, workspace=torch.empty(16, dtype=torch.uint8, device=DEV))
     kv = torch.zeros(10, 2, 2, D, dtype=torch.bfloat16, device=DEV)
     for k, v in (([kv[:, 0]], []), ([kv[:, 0], kv[:9, 0]], [kv[:, 1], kv[:9, 1]]), ([kv[:, 0].float()], [kv[:, 1].float()])):
         with pytest.raises(ValueError):
