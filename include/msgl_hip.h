@@ -424,8 +424,9 @@ int msgl_prepare_decode_paged(const int32_t* req_pool_indices, int32_t* seq_lens
  * 4 (more tokens than `capacity`, more nodes than the mask has bits); then cu_seqlens_q is all 0,
  * every row is a row behind the last token, and lengths, table and free range stay as they were.
  * req_to_page (NULL = none) gets the page ids of pages taken.  parents and tree_mask: both or
- * neither.  workspace: msgl_prepare_extend_workspace_bytes bytes, 16-byte aligned (0, and NULL, for small steps). */
-size_t msgl_prepare_extend_workspace_bytes(int bs, int32_t capacity, int32_t max_ctx);
+ * neither.  workspace: msgl_prepare_extend_workspace_bytes bytes, 16-byte aligned (0, and NULL, for small steps, and for most that are not
+ * in place; in_place: alloc_out is alloc_lens or free_range_out is free_range). */
+size_t msgl_prepare_extend_workspace_bytes(int bs, int32_t capacity, int32_t max_ctx, int in_place);
 int msgl_prepare_extend(const int32_t* req_pool_indices, const int32_t* prefix_lens, const int32_t* new_lens, const int32_t* alloc_lens,
                         const int32_t* free_pages, int32_t free_capacity, const int32_t* free_range, int32_t* req_to_token,
                         int64_t r2t_stride, int32_t table_rows, int32_t max_ctx, int32_t* req_to_page, int64_t r2p_stride,

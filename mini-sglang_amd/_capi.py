@@ -80,7 +80,7 @@ SIGNATURES = {
         [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p, c_void_p,
          c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p],
     ),
-    "msgl_prepare_extend_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "msgl_prepare_extend_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
     "msgl_prepare_extend": (
         c_int,
         [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p, c_int64,

@@ -214,9 +214,13 @@ __global__ __launch_bounds__(256) void extend_prepare_tree_kernel(ExtendPrepPara
     place_tree(p, p.scratch[b], base, min(p.cu[b + 1] - base, p.words * 64));
 }
 
-// Both phases in one work group, for steps of a few thousand tokens: what bounds such a step is latency, and one launch with one barrier has
-// the least of it (4 requests of 8 nodes: 4.9 + 2.4 us as two launches).  Counts fit 32 bits (msgl_prepare_extend sees to it).
-constexpr int kSmallRequests = 1024, kSmallTokens = 4096;
+// Both phases in one launch: what bounds a step is latency, and one launch with one barrier has the least of it (4 requests of 8 nodes 4.9 + 2.4 ->
+// 4.1 us, 200 prompts of 450 to 900 tokens 5.1 + 4 -> 6.2 us).  Every work group counts all requests and places its share of the tokens; the first writes the lengths.  In place, where a work group's
+// inputs are the first's outputs, there is only the first, and only for steps of a few thousand tokens.  Counts fit 32 bits (one_launch).
+constexpr int kSmallRequests = 1024, kSmallTokens = 4096, kMostSmall = 1 << 20;
+static bool one_launch(int bs, int32_t capacity, int32_t max_ctx, bool in_place) {
+    return bs <= kSmallRequests && capacity <= (in_place ? kSmallTokens : kMostSmall) && max_ctx <= kMostSmall;
+}
 __global__ __launch_bounds__(kScanThreads) void extend_prepare_small_kernel(ExtendPrepParams p) {
     __shared__ int4 req[kSmallRequests];           // prefix, alloc, page offset inside the wave's requests, table row
     __shared__ int start[kSmallRequests];          // first token inside the wave's requests
@@ -257,27 +261,28 @@ __global__ __launch_bounds__(kScanThreads) void extend_prepare_small_kernel(Exte
     int refuse = earlier;
     if (!refuse)
         refuse = any & 4 ? 3 : any & 2 ? 2 : ((any & 1) || total > p.capacity) ? 4 : (head < 0 || taken > (int64_t)min(valid_end, p.free_capacity) - head) ? 1 : 0;
-    if (tid < p.bs) {
+    const bool writer = blockIdx.x == 0;
+    if (writer && tid < p.bs) {
         p.cu[tid] = refuse ? 0 : tokens - counted + before(wave, 0);
         p.seq_lens[tid] = refuse ? L : L + n;
         if (!refuse || p.alloc_out != p.alloc) p.alloc_out[tid] = refuse ? A : max(A, L + n);
     }
-    if (tid == 0) {
+    if (writer && tid == 0) {
         p.cu[p.bs] = refuse ? 0 : total;
         if (refuse) *p.status = refuse;
         if (!refuse || p.free_range_out != p.free_range) p.free_range_out[0] = refuse ? head : head + taken, p.free_range_out[1] = valid_end;
     }
-    clear_behind(p, refuse ? 0 : total, tid, kScanThreads);
+    clear_behind(p, refuse ? 0 : total, blockIdx.x * kScanThreads + tid, gridDim.x * kScanThreads);
     if (refuse) return;
     if (p.parents) {
-        for (int b = wave; b < p.bs; b += kScanThreads / 64) {
+        for (int b = blockIdx.x * (kScanThreads / 64) + wave; b < p.bs; b += gridDim.x * (kScanThreads / 64)) {
             const int4 rq = req[b];
             const int w = b >> 6, base = start[b] + before(w, 0);
             const int end = b + 1 < p.bs ? start[b + 1] + before((b + 1) >> 6, 0) : total;
             place_tree(p, make_int4(rq.x, rq.y, rq.z + head + before(w, 1), rq.w), base, end - base);
         }
     } else {
-        for (int t = tid; t < total; t += kScanThreads) {
+        for (int t = blockIdx.x * kScanThreads + tid; t < total; t += gridDim.x * kScanThreads) {
             int w = 0, base = 0;  // the last wave whose requests start at or before t, then the last request among them
 #pragma unroll
             for (int k = 0, at = 0; k < kScanThreads / 64 - 1; ++k) {
@@ -404,8 +409,8 @@ __global__ __launch_bounds__(256) void accept_tree_kernel(AcceptParams p) {
 using namespace msgl;
 
 // (the largest sums of the one-group kernel: 1024 requests of at most `capacity` tokens and max_ctx pages)
-extern "C" size_t msgl_prepare_extend_workspace_bytes(int bs, int32_t capacity, int32_t max_ctx) {
-    if (bs <= 0 || (bs <= kSmallRequests && capacity <= kSmallTokens && max_ctx <= 1 << 20)) return 0;
+extern "C" size_t msgl_prepare_extend_workspace_bytes(int bs, int32_t capacity, int32_t max_ctx, int in_place) {
+    if (bs <= 0 || one_launch(bs, capacity, max_ctx, in_place != 0)) return 0;
     return (size_t)bs * sizeof(int4);
 }
 
@@ -435,7 +440,8 @@ extern "C" int msgl_prepare_extend(const int32_t* req_pool_indices, const int32_
         for (int j = 0; j < 7; ++j)
             MSGL_REQUIRE(inputs[i] == nullptr || inputs[i] != results[j] || (i == j && i < 2),
                          "msgl_prepare_extend: an output overwrites an input (only alloc_out may be alloc_lens, free_range_out free_range)");
-    const size_t need = msgl_prepare_extend_workspace_bytes(bs, capacity, max_ctx);
+    const bool in_place = alloc_out == alloc_lens || free_range_out == free_range;
+    const size_t need = msgl_prepare_extend_workspace_bytes(bs, capacity, max_ctx, in_place);
     if (need && (workspace_bytes < need || workspace == nullptr)) {
         set_error("msgl_prepare_extend: workspace %zu < %zu bytes", workspace ? workspace_bytes : (size_t)0, need);
         return MSGL_E_WORKSPACE;
@@ -452,7 +458,9 @@ extern "C" int msgl_prepare_extend(const int32_t* req_pool_indices, const int32_
     p.capacity = capacity, p.words = parents ? mask_words : 0, p.bs = bs, p.ps = page_size;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     if (need == 0) {
-        hipLaunchKernelGGL(extend_prepare_small_kernel, dim3(1), dim3(kScanThreads), 0, st, p);
+        const int share = parents ? (bs + kScanThreads / 64 - 1) / (kScanThreads / 64) : (capacity + kScanThreads - 1) / kScanThreads;
+        const unsigned groups = in_place || share < 1 ? 1u : (unsigned)share;
+        hipLaunchKernelGGL(extend_prepare_small_kernel, dim3(groups), dim3(kScanThreads), 0, st, p);
         return check_launch("extend_prepare_small_kernel");
     }
     hipLaunchKernelGGL(extend_prepare_scan_kernel, dim3(1), dim3(kScanThreads), 0, st, p);

@@ -99,7 +99,8 @@ def test_nothing_to_do_is_no_error_and_needs_no_workspace():
     assert _call("msgl_accept_tree", ACCEPT, ACCEPT_OK, dict(bs=0))[0] == 0
     assert _call("msgl_token_logprobs", LOGPROBS, LOGPROBS_OK, dict(rows=0))[0] == 0
     lib, _ = _lib()
-    assert lib.msgl_prepare_extend_workspace_bytes(1024, 4096, 1 << 20) == 0 and lib.msgl_prepare_extend_workspace_bytes(1025, 1, 64) == 1025 * 16
+    assert lib.msgl_prepare_extend_workspace_bytes(1024, 4096, 1 << 20, 1) == 0 and lib.msgl_prepare_extend_workspace_bytes(1025, 1, 64, 0) == 1025 * 16
+    assert lib.msgl_prepare_extend_workspace_bytes(10, 4097, 64, 1) == 160 and lib.msgl_prepare_extend_workspace_bytes(10, 1 << 20, 64, 0) == 0
     assert lib.msgl_tree_attention_workspace_bytes(10, 8, 128, 1) == 0 and lib.msgl_tree_attention_workspace_bytes(10, 8, 128, 3) == 10 * 8 * (3 * 130 + 1) * 4
     assert lib.msgl_token_logprobs_workspace_bytes(0, 100, 2, 0) == 0 and lib.msgl_token_logprobs_workspace_bytes(5, 8185, 2, 9) == 0  # one segment
     assert lib.msgl_token_logprobs_workspace_bytes(5, 8186, 2, 9) > 0 and lib.msgl_token_logprobs_workspace_bytes(5, 8189, 4, 9) == 0

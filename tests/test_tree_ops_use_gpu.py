@@ -236,3 +236,23 @@ def test_shares_of_unequal_requests(bs, longest, most, Hq, Hkv):
         _check(ops.tree_attention(*a, total_kv=total, workspace=ws), c)
     a[9] = longest // 3
     _check(ops.tree_attention(*a, total_kv=total // 4), c)
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("bs,most,tree", [(1024, 4, True), (1025, 4, True), (300, 90, False), (70, 130, True), (3, 5000, False), (200, 25, True), (1024, 9, False)])
+def test_prepare_extend_in_place_and_apart(bs, most, tree, in_place):
+    """Steps on both sides of every bound of the one-launch form, in place and not, accepted and refused."""
+    from test_tree_ops_gpu import _prepare
+
+    rng = random.Random(bs + most)
+    prefix = [rng.randint(0, 50) for _ in range(bs)]
+    new = [rng.randint(0, most) for _ in range(bs)]
+    new[-1] = most
+    alloc = [p + rng.choice([0, 0, 2, 20]) for p in prefix]
+    ok = dict(prefix=prefix, new=new, alloc=alloc, page_size=16, seed=bs, tree=tree, in_place=in_place)
+    assert _prepare(**ok) == 0
+    assert _prepare(**ok, capacity=sum(new) + 1500) == 0
+    assert _prepare(**ok, cut=3) == 1
+    assert _prepare(**ok, capacity=sum(new) - 1) == 4
+    assert _prepare(**ok, status=5) == 5
+    assert _prepare(**dict(ok, alloc=[-1] + alloc[1:])) == 3
