@@ -9,8 +9,8 @@
 // Order of the alternatives: by value, ties to the lower index, NaN above everything (as msgl_argmax).  Value and index are one
 // 64-bit key: the float's bits mapped to an unsigned number that rises with the value, then the index's complement.
 // The k best of a segment: the k-th largest of a wave's 64 lane maxima is no larger than the segment's k-th largest value, so the few values
-// that reach it (in every wave's view: the largest of the four) are all that has to be ranked.  The k-th largest lane maximum comes from
-// bisecting its bits with ballots.  Segments where that leaves too many (long ties that are not a fill from the segment's start on, NaN,
+// that reach it (in every wave's view: the largest of the four) are all that has to be ranked; so are those that reach the least of the waves'
+// k/4-th largest, and whichever bar is higher counts (the second from kTwoBars alternatives on).  A wave's k-th largest lane maximum comes from bisecting its bits with ballots.  Segments where that leaves too many (long ties that are not a fill from the segment's start on, NaN,
 // infinities) are taken apart winner by winner instead.
 #include <type_traits>
 
@@ -22,6 +22,9 @@ namespace msgl {
 constexpr int kLpThreads = 256;
 constexpr int kLpWaves = kLpThreads / 64;
 constexpr int kLpCandidates = 256;  // per wave
+// alternatives from which on the second bar pays for its ballots: 1000 bf16 rows of 151936 with 5, 8, 12, 20, 32 alternatives take
+// 85, 88, 93, 113, 166 us with one and 88, 89, 91, 95, 103 with both
+constexpr int kTwoBars = 12;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
 constexpr double kLn2d = 0.693147180559945309417;
 
@@ -87,6 +90,18 @@ __device__ __forceinline__ uint32_t wave_kth(uint32_t key, int k, int bits) {
     for (int b = 31; b > 31 - bits; --b) {
         const uint32_t with = t | 1u << b;
         if (__popcll(__ballot(key >= with)) >= k) t = with;
+    }
+    return t;
+}
+
+// The same for two ranks at a time.
+__device__ __forceinline__ uint2 wave_kth2(uint32_t key, int k0, int k1, int bits) {
+    uint2 t = make_uint2(0, 0);
+    for (int b = 31; b > 31 - bits; --b) {
+        const uint2 with = make_uint2(t.x | 1u << b, t.y | 1u << b);
+        const uint64_t at0 = __ballot(key >= with.x), at1 = __ballot(key >= with.y);
+        if (__popcll(at0) >= k0) t.x = with.x;
+        if (__popcll(at1) >= k1) t.y = with.y;
     }
     return t;
 }
@@ -177,7 +192,7 @@ __global__ __launch_bounds__(kLpThreads) void logprob_segment_kernel(LogprobPara
     constexpr int E = 16 / BYTES;                     // elements per piece
     constexpr int kPieces = kLpThreads * LOADS;       // pieces per segment
     __shared__ float lds_f[kLpWaves][2];
-    __shared__ uint32_t lds_t[kLpWaves];
+    __shared__ uint32_t lds_t[kLpWaves], lds_s[kLpWaves];
     __shared__ Candidates found;
     __shared__ int lds_ties[kLpWaves];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -221,14 +236,17 @@ __global__ __launch_bounds__(kLpThreads) void logprob_segment_kernel(LogprobPara
         mine = fmaxf(mine, best[j]);
     }
     const float top_wave = wave_max(mine);
-    // 16 bits of the threshold are enough to leave few candidates
-    const uint32_t bar_wave = p.top ? wave_kth(order_key(mine), p.top, 16) : 0;
-    if (lane == 0) lds_f[wave][0] = top_wave, lds_t[wave] = bar_wave;
+    // 16 bits of the thresholds are enough to leave few candidates
+    uint2 bar_wave = make_uint2(0, 0);
+    if (p.top >= kTwoBars) bar_wave = wave_kth2(order_key(mine), p.top, (p.top + kLpWaves - 1) / kLpWaves, 16);
+    else if (p.top) bar_wave.x = wave_kth(order_key(mine), p.top, 16);
+    if (lane == 0) lds_f[wave][0] = top_wave, lds_t[wave] = bar_wave.x, lds_s[wave] = bar_wave.y;
     __syncthreads();
     float m = lds_f[0][0];
-    uint32_t bar = max(lds_t[0], kLowestKey);
+    uint32_t bar = max(lds_t[0], kLowestKey), least = lds_s[0];
 #pragma unroll
-    for (int w = 1; w < kLpWaves; ++w) m = fmaxf(m, lds_f[w][0]), bar = max(bar, lds_t[w]);
+    for (int w = 1; w < kLpWaves; ++w) m = fmaxf(m, lds_f[w][0]), bar = max(bar, lds_t[w]), least = min(least, lds_s[w]);
+    bar = max(bar, least);
     const float ref = m == -INFINITY ? 0.f : m;  // nothing but -inf here: every e is 0 (or NaN)
     float z = 0.f, t = 0.f;
     auto add = [&](auto log2_of) {
