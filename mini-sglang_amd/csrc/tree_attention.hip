@@ -7,7 +7,7 @@
 // head, packed node after node, 32 to a block.  S^T = K.Q^T and O^T += V^T.P^T on v_mfma_f32_32x32x16_bf16: the row sits on the lane in
 // both products (lane & 31), so maximum, sum and rescaling are in-lane plus one swap of lane halves, and the exponentiated scores,
 // packed to bf16, are the second product's operand as they stand.  (P is rounded to bf16 as that product's operand type asks: half a
-// step, 2^-9 relative, per probability, unbiased, and the sum is taken of the unrounded ones.)
+// step, 2^-8 relative at most, per probability, unbiased, and the sum is taken of the unrounded ones.)
 //
 // With up to 64 rows per kv head the pass over K and V bounds the kernel (a 32-key tile costs a wave 512 matrix cycles per 32 rows
 // where HBM takes 1250 cycles of the compute unit).  The work group's four waves take every fourth 32-key tile each, with RB blocks of
@@ -494,14 +494,10 @@ __device__ __forceinline__ void join_and_store(const TreeParams& p, const TreeIt
     }
 }
 
+// One run, up to 64 rows: tiles are private to a wave.  Measured: 64 requests of 8192 tokens x 8 nodes, 32 / 8 heads, 345 us = 6.3 TB/s, 0.89 of what a
+// read-only stream reaches on this chip; with 16 nodes (two blocks of rows) 358 us.
 template <int RB>
-__global__ __launch_bounds__(kTreeWaves * 64, 1) void tree_attention_kernel(TreeParams p) {
-    extern __shared__ __attribute__((aligned(1024))) char smem[];
-    // block -> (kv head, share), heads fastest: a token row's pieces are read at about the same time
-    const int h = blockIdx.x % (unsigned)p.Hkv;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    TreeItem it;
-    for (TreeWalk walk(p, blockIdx.x / (unsigned)p.Hkv, 0, threadIdx.x & 63, it); walk.any; __syncthreads(), walk.next(p, 0, it)) {
+__device__ __forceinline__ void narrow_run(const TreeParams& p, const TreeItem& it, int h, int wave, char* smem) {
     const int lane = fresh_lane();
     const int g4 = lane >> 4, q16 = lane & 15;
     const int all_tiles = (it.t1 - it.t0 + kTreeKeys - 1) / kTreeKeys;
@@ -596,14 +592,25 @@ __global__ __launch_bounds__(kTreeWaves * 64, 1) void tree_attention_kernel(Tree
     wait_loads<0>();
     join_and_store<RB, kTreeWaves, kTreeWaves>(p, it, st, smem, wave, lane, odd, it.t0 + (wave + plain * kTreeWaves) * kTreeKeys, kTreeWaves * kTreeKeys, [](int) { return 0; },
                             [&](int) { return h; });
-    }
+}
+template <int RB>
+__global__ __launch_bounds__(kTreeWaves * 64, 1) void tree_attention_kernel(TreeParams p) {
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    // block -> (kv head, share), heads fastest: a token row's pieces are read at about the same time
+    const int h = blockIdx.x % (unsigned)p.Hkv;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    TreeItem it;
+    for (TreeWalk walk(p, blockIdx.x / (unsigned)p.Hkv, 0, threadIdx.x & 63, it); walk.any; __syncthreads(), walk.next(p, 0, it))
+        narrow_run<RB>(p, it, h, wave, smem);
 }
 
 // More than 64 rows per kv head: the NW waves hold 32 rows each and share the tiles, so that K and V are read once per 32 NW rows.  A tile is loaded by
 // all waves, 32 / NW keys each, SLOTS - 2 tiles ahead into a ring; a wave waits for its own loads of tile j, then the barrier says that everybody's
 // have landed and that everybody is done with tile j - 2, whose slot is filled anew.  Two waves per SIMD either way (NW = 8 and one work group
 // per compute unit, or NW = 4 and two): a wave issues an instruction about every eighth cycle, whatever it is, so one wave cannot keep
-// softmax and matrix products side by side (measured with 64 rows a wave, one wave per SIMD: 786 TFLOP/s with all keys in L2).
+// softmax and matrix products side by side.  Measured: 32 requests of 16000 tokens x 64 nodes, 32 / 8 heads, 607 us = 890 TFLOP/s, K and V at
+// 3.5 TB/s beside it (a dense product of 8192^3 reaches 1228 on this chip, whose clock gives way under such load); 40 requests of 4000 to
+// 8000 x 30 nodes (four waves) 208 us = 4.8 TB/s, bound by the issue of its one wave per SIMD.
 template <int NW>
 struct TreeWide {
     static constexpr int kSlots = NW == 8 ? 8 : 4;
@@ -637,18 +644,8 @@ __device__ __forceinline__ void dma_rows4(uint64_t k, uint64_t v, uint32_t dst) 
 }
 
 template <int NW, bool NT>
-__global__ __launch_bounds__(NW * 64, 2) void tree_attention_wide_kernel(TreeParams p) {
+__device__ __forceinline__ void wide_run(const TreeParams& p, const TreeItem& it, int h, int wave, char* smem) {
     using W = TreeWide<NW>;
-    extern __shared__ __attribute__((aligned(1024))) char smem[];
-    // block -> item, row tile: the row tiles of an item run on the same XCD (block ids modulo 8), whose L2 then holds the keys for all of them
-    const int y = blockIdx.x >> 3;
-    const int rt = y % p.row_tiles;
-    const int item = (y / p.row_tiles) * 8 + (blockIdx.x & 7);
-    if (item >= p.items) return;
-    const int h = item % p.Hkv;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    TreeItem it;
-    for (TreeWalk walk(p, item / p.Hkv, rt * 32 * NW, threadIdx.x & 63, it); walk.any; __syncthreads(), walk.next(p, rt * 32 * NW, it)) {
     const int lane = fresh_lane();
     const int g4 = lane >> 4, q16 = lane & 15;
     const int row0 = it.r0 + wave * 32;
@@ -829,7 +826,20 @@ __global__ __launch_bounds__(NW * 64, 2) void tree_attention_wide_kernel(TreePar
     }
     wait_loads<0>();
     join_and_store<1, 1, NW>(p, it, st, smem, wave, lane, odd, it.t0 + plain * kTreeKeys, kTreeKeys, [&](int g) { return it.r0 + g * 32; }, [&](int) { return h; });
-    }
+}
+template <int NW, bool NT>
+__global__ __launch_bounds__(NW * 64, 2) void tree_attention_wide_kernel(TreeParams p) {
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    // block -> item, row tile: the row tiles of an item run on the same XCD (block ids modulo 8), whose L2 then holds the keys for all of them
+    const int y = blockIdx.x >> 3;
+    const int rt = y % p.row_tiles;
+    const int item = (y / p.row_tiles) * 8 + (blockIdx.x & 7);
+    if (item >= p.items) return;
+    const int h = item % p.Hkv;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    TreeItem it;
+    for (TreeWalk walk(p, item / p.Hkv, rt * 32 * NW, threadIdx.x & 63, it); walk.any; __syncthreads(), walk.next(p, rt * 32 * NW, it))
+        wide_run<NW, NT>(p, it, h, wave, smem);
 }
 
 // Joins the runs of a (token, head): GROUPS half-waves per row take every GROUPS-th run, four dims per lane, and meet in LDS.
