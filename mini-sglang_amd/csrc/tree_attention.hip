@@ -848,19 +848,13 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeParams p) {
     __shared__ float lds[8][kHD + 2];
     const int lane = threadIdx.x & 31, hw = threadIdx.x >> 5;
     const int g = hw % GROUPS;
-    const int per = p.max_q * p.Hq;  // (node, head) pairs of a request
-    const int64_t id = (int64_t)blockIdx.x * (8 / GROUPS) + hw / GROUPS;
-    const int b = (int)(id / per);
-    const int r = (int)(id - (int64_t)b * per);
-    int base = 0, n = 0, nsplit = 0;
-    if (b < p.bs) {
-        base = p.cu[b];
-        n = min(p.cu[b + 1] - base, p.max_q);
-    }
-    const int node = r / p.Hq, hq = r - node * p.Hq;
-    if (node < n) nsplit = p.ws_n[(int64_t)(base + node) * p.Hq + hq];
-    const bool live = node < n && nsplit > 1;  // (one run: written by the first kernel)
-    const int64_t at = ((int64_t)(base + node) * p.Hq + hq) * p.splits;
+    const int b = blockIdx.y;
+    const int base = p.cu[b], n = min(p.cu[b + 1] - base, p.max_q);
+    const int r = blockIdx.x * (8 / GROUPS) + hw / GROUPS;  // (node, head) pair of the request
+    const int64_t pair = (int64_t)base * p.Hq + r;
+    const int nsplit = r < n * p.Hq ? p.ws_n[pair] : 0;
+    const bool live = nsplit > 1;  // (one run: written by the first kernel)
+    const int64_t at = pair * p.splits;
     float M = kNegBigE, L = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     if (live) {
@@ -908,7 +902,8 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeParams p) {
     }
     if (!live) return;
     const float inv = L == 0.f ? 0.f : 1.0f / L;
-    *reinterpret_cast<uint2*>(p.out + (int64_t)(base + node) * p.out_stride + hq * kHD + 4 * lane) =
+    const int node = r / p.Hq;
+    *reinterpret_cast<uint2*>(p.out + (int64_t)(base + node) * p.out_stride + (r - node * p.Hq) * kHD + 4 * lane) =
         make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
 }
 
@@ -977,7 +972,7 @@ static TreeCut tree_cut(int bs, int max_q, int max_k, int64_t total_kv, int Hq, 
     if (shares > (all + least - 1) / least) shares = (all + least - 1) / least;
     const int64_t len = (all + shares - 1) / shares;
     const int64_t alone = bs * across <= units ? kTreeBegin + most : (kTreeBegin + mean) * bs * across / units + most - mean;
-    if (alone <= kTreeBegin + len + kJoin) return whole;
+    if (alone <= kTreeBegin + len + kJoin || bs > 65535) return whole;
     const int64_t splits = (most + len - 1) / len + 1;
     return {(int)shares, (int)(splits < kMaxTreeSplits ? splits : kMaxTreeSplits)};
 }
@@ -1055,9 +1050,9 @@ extern "C" int msgl_tree_attention(const void* q, int64_t q_stride, const void* 
     }
     if (rc != MSGL_OK || splits == 1) return rc;
     // half-waves per row: as many as there are runs for, up to eight
-    const int64_t rows = (int64_t)bs * max_seqlen_q * Hq;
-    if (splits <= 8) hipLaunchKernelGGL(tree_merge_kernel<1>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, p);
-    else if (splits <= 32) hipLaunchKernelGGL(tree_merge_kernel<4>, dim3((unsigned)((rows + 1) / 2)), dim3(256), 0, st, p);
-    else hipLaunchKernelGGL(tree_merge_kernel<8>, dim3((unsigned)rows), dim3(256), 0, st, p);
+    const unsigned rows = (unsigned)max_seqlen_q * Hq;
+    if (splits <= 8) hipLaunchKernelGGL(tree_merge_kernel<1>, dim3((rows + 7) / 8, bs), dim3(256), 0, st, p);
+    else if (splits <= 32) hipLaunchKernelGGL(tree_merge_kernel<4>, dim3((rows + 1) / 2, bs), dim3(256), 0, st, p);
+    else hipLaunchKernelGGL(tree_merge_kernel<8>, dim3(rows, bs), dim3(256), 0, st, p);
     return check_launch("tree_merge_kernel");
 }
