@@ -44,7 +44,7 @@ class HipAttnMetadata:
     extend_plan: Optional[torch.Tensor] = None  # launch order of the (request, query tile) items, longest first
     # verify (drafted trees): bounds that may be captured, and buffers of their own so that a captured step keeps its addresses
     total_kv: int = 0
-    verify_out: Optional[torch.Tensor] = None        # rows behind the last node stay 0
+    verify_out: Optional[torch.Tensor] = None        # rows behind the last node: 0, or an earlier step's finite values
     verify_workspace: Optional[torch.Tensor] = None
     # metadata of a captured batch size: its launches use the workspace that was sized before the first capture
     static: bool = False

@@ -960,7 +960,7 @@ struct TreeCut {
 //   1 of 1000 x 4, 16 / 8 heads (8)  15 | 20      1 of 2000 x 4 (8)  20 | 20      1 of 500 x 60 (8)  28 | 24      7 of 500 to 1000 x 4 (56)  17 | 19
 static TreeCut tree_cut(int bs, int max_q, int max_k, int64_t total_kv, int Hq, int Hkv) {
     const TreeCut whole = {bs, 1};
-    if (bs <= 0 || max_q <= 0 || max_k <= 0 || Hkv <= 0 || Hq < Hkv) return whole;
+    if (bs <= 0 || bs > 65535 || max_q <= 0 || max_k <= 0 || Hkv <= 0 || Hq < Hkv) return whole;
     const TreeShape sh = tree_shape(max_q, Hq, Hkv);
     const int64_t units = device_cus(), across = (int64_t)Hkv * sh.row_tiles;
     const int64_t most = ((int64_t)max_k + kTreeKeys - 1) / kTreeKeys;
@@ -972,7 +972,7 @@ static TreeCut tree_cut(int bs, int max_q, int max_k, int64_t total_kv, int Hq, 
     if (shares > (all + least - 1) / least) shares = (all + least - 1) / least;
     const int64_t len = (all + shares - 1) / shares;
     const int64_t alone = bs * across <= units ? kTreeBegin + most : (kTreeBegin + mean) * bs * across / units + most - mean;
-    if (alone <= kTreeBegin + len + kJoin || bs > 65535) return whole;
+    if (alone <= kTreeBegin + len + kJoin) return whole;
     const int64_t splits = (most + len - 1) / len + 1;
     return {(int)shares, (int)(splits < kMaxTreeSplits ? splits : kMaxTreeSplits)};
 }

@@ -424,7 +424,8 @@ extern "C" int msgl_prepare_extend(const int32_t* req_pool_indices, const int32_
                  "msgl_prepare_extend: bs=%d page_size=%d free_capacity=%d max_ctx=%d table_rows=%d capacity=%d", bs, page_size, free_capacity, max_ctx,
                  table_rows, capacity);
     if (bs == 0) return MSGL_OK;
-    MSGL_REQUIRE(max_ctx <= 0x7fffffff - page_size, "msgl_prepare_extend: max_ctx %d + page_size %d leaves 32 bits", max_ctx, page_size);
+    MSGL_REQUIRE(max_ctx <= 0x7fffffff - page_size && capacity <= 1 << 30, "msgl_prepare_extend: max_ctx %d + page_size %d or capacity %d leaves 32 bits",
+                 max_ctx, page_size, capacity);
     MSGL_REQUIRE(req_pool_indices && prefix_lens && new_lens && alloc_lens && free_pages && free_range && req_to_token && cu_seqlens_q && seq_lens &&
                      alloc_out && free_range_out && status && (capacity == 0 || (positions && out_cache_loc)),
                  "msgl_prepare_extend: null pointer argument");

@@ -33,7 +33,7 @@ class TreeDecoder:
         if any(r.sampling_params.temperature != 0 for r in batch.reqs):
             raise ValueError("drafted trees are accepted greedily: temperature must be 0")
         self.mr, self.batch, self.max_nodes, self.max_new_tokens, self.logprobs = mr, batch, max_nodes, max_new_tokens, logprobs
-        self.use_graph = use_graph
+        self.use_graph, self.vocab = use_graph, mr.model_config.vocab_size
         self.bs, dev = batch.batch_size, mr.device
         bs, rows = self.bs, self.bs * max_nodes
         i32 = dict(dtype=torch.int32, device=dev)
@@ -121,6 +121,8 @@ class TreeDecoder:
                 raise ValueError(f"a draft has {len(tokens)} tokens and {len(par)} parents; at most {self.max_nodes - 1} nodes were announced")
             if any(not 0 <= p <= i for i, p in enumerate(par)):
                 raise ValueError("a draft's parent must be an earlier node")
+            if any(not 0 <= t < self.vocab for t in tokens):
+                raise ValueError(f"a drafted token is outside the vocabulary of {self.vocab}")
             ids += [r.last_token_id, *tokens]
             parents += [-1, *par]
             lens.append(1 + len(tokens))

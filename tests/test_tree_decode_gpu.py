@@ -98,6 +98,9 @@ def test_tree_step_refusal_changes_nothing():
         assert dec.step(drafts) == other.step(drafts)
     with pytest.raises(ValueError, match="parent"):
         dec.step([([1], [1]), ([], [])])
+    for token in (-1, 2048):
+        with pytest.raises(ValueError, match="vocabulary"):
+            dec.step([([token], [0]), ([], [])])
     with pytest.raises(ValueError, match="announced"):
         dec.step([([1] * 6, [0] * 6), ([], [])])
     with pytest.raises(ValueError, match="drafts for"):

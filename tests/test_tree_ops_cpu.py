@@ -32,6 +32,7 @@ PREPARE_OK = dict(req=A[0], prefix=A[1], new=A[2], alloc=A[3], free=A[4], free_c
 @pytest.mark.parametrize("change,words", [
     (dict(bs=-1), "bs=-1"), (dict(page_size=0), "page_size=0"), (dict(capacity=-1), "capacity=-1"), (dict(max_ctx=0), "max_ctx=0"),
     (dict(table_rows=0), "table_rows=0"), (dict(free_capacity=-2), "free_capacity=-2"), (dict(max_ctx=2 ** 31 - 5, r2t_stride=2 ** 40), "32 bits"),
+    (dict(capacity=2 ** 30 + 1), "32 bits"),
     *[({k: None}, "null pointer") for k in "req prefix new alloc free range r2t positions loc cu seq alloc_out range_out status".split()],
     (dict(parents=None), "go together"), (dict(mask=None), "go together"), (dict(words=0), "mask_words"), (dict(words=17), "mask_words"),
     (dict(r2t_stride=63), "r2t_stride"), (dict(r2p=A[14], r2p_stride=3), "r2p_stride"),
@@ -111,6 +112,7 @@ def test_splits_follow_the_bounds():
 
     assert ops.tree_attention_splits(64, 8, 8192, 16, 8) == 1                # enough requests for every unit
     assert ops.tree_attention_splits(1, 4, 100, 16, 8) == 1                  # nothing worth cutting
+    assert ops.tree_attention_splits(0, 4, 100, 16, 8) == ops.tree_attention_splits(2 ** 31 - 1, 4, 2 ** 30, 16, 8, 2 ** 62) == 1
     assert 1 < ops.tree_attention_splits(1, 4, 2 ** 30, 16, 8) <= 256
     assert ops.tree_attention_splits(2, 32, 130001, 4, 1) > 64
     assert ops.tree_attention_splits(16, 16, 16000, 16, 8, 16 * 4000) >= ops.tree_attention_splits(16, 16, 16000, 16, 8) >= 1  # short ones beside a long one
