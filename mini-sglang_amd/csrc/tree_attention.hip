@@ -306,22 +306,42 @@ __device__ __forceinline__ void tile_scores(const bf16x8_t (&kf)[8], const bf16x
     }
 }
 
-// What a row sees of the tile that begins at key0: bit k for key k.
-__device__ __forceinline__ uint32_t row_sees(const TreeParams& p, const TreeItem& it, int row, int key0) {
+__device__ __forceinline__ const uint64_t* row_mask(const TreeParams& p, const TreeItem& it, int row) {
+    return p.mask + (int64_t)(it.base + min(row, it.rows - 1) / p.group) * p.words;
+}
+// What a row sees of the tile that begins at key0: bit k for key k.  word: its mask, if that is one word.
+__device__ __forceinline__ uint32_t row_sees(const TreeParams& p, const TreeItem& it, int row, uint64_t word, int key0) {
     const int rel = key0 - it.prefix;
-    const uint64_t* bits = p.mask + (int64_t)(it.base + min(row, it.rows - 1) / p.group) * p.words;
-    uint32_t see = rel >= 0 ? mask_bits(bits, p.words, rel) : rel <= -32 ? ~0u : (mask_bits(bits, p.words, 0) << -rel) | ((1u << -rel) - 1);
+    uint32_t see = ~0u;
+    if (rel > -32) {
+        const int off = max(rel, 0);
+        const uint32_t bits = p.words == 1 ? (off < 64 ? (uint32_t)(word >> off) : 0) : mask_bits(row_mask(p, it, row), p.words, off);
+        see = rel >= 0 ? bits : (bits << -rel) | ((1u << -rel) - 1);
+    }
     if (key0 + kTreeKeys > it.t1) see &= (1u << (it.t1 - key0)) - 1;
     return see;
+}
+
+// The lanes' rows' masks where they are one word each, in registers after this.  The wide kernel reads them at the start: in its loop they would be
+// waited for together with all the loads that the compiler does not count, for up to three tiles.
+template <int RB>
+__device__ __forceinline__ void load_masks(const TreeParams& p, const TreeItem& it, int row0, int lane, uint64_t (&word)[RB]) {
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+        word[rb] = 0;
+        if (p.words == 1) word[rb] = *row_mask(p, it, row0 + rb * 32 + (lane & 31));
+    }
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) asm volatile("" : "+v"(word[rb]));
 }
 
 // Hides what the rows do not see of the tile that begins at key0.
 // s[rb][i]: key 8 (i >> 2) + 4 half + (i & 3) of the tile, row lane & 31 of the block.
 template <int RB>
-__device__ __forceinline__ void tile_mask(const TreeParams& p, const TreeItem& it, int row0, int key0, int lane, f32x16_t (&s)[RB]) {
+__device__ __forceinline__ void tile_mask(const TreeParams& p, const TreeItem& it, int row0, const uint64_t (&word)[RB], int key0, int lane, f32x16_t (&s)[RB]) {
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-        const uint32_t bits = row_sees(p, it, row0 + rb * 32 + (lane & 31), key0) >> (4 * (lane >> 5));
+        const uint32_t bits = row_sees(p, it, row0 + rb * 32 + (lane & 31), word[rb], key0) >> (4 * (lane >> 5));
 #pragma unroll
         for (int i = 0; i < 16; ++i)
             if (!(bits >> (8 * (i >> 2) + (i & 3)) & 1)) s[rb][i] = -INFINITY;
@@ -423,7 +443,7 @@ __device__ __forceinline__ bool tile_values_masked(const char* vt, int lane, con
 // LDS.  Runs only where a tile had such a value.
 __device__ __forceinline__ void add_odd_values(const TreeParams& p, const TreeItem& it, int row0, int rows, int h, int key0, int lane, float* o) {
     for (int r = lane; r < rows; r += 64) {
-        const uint32_t see = row_sees(p, it, row0 + r, key0);
+        const uint32_t see = row_sees(p, it, row0 + r, p.words == 1 ? *row_mask(p, it, row0 + r) : 0, key0);
         for (int k = 0; k < kTreeKeys && key0 + k < it.t1; ++k) {
             const uint16_t* v = reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(p.vc) + (uint64_t)(uint32_t)it.table[key0 + k] * p.slot_bytes) + h * kHD;
             for (int d = 0; d < kHD; ++d)
@@ -491,6 +511,39 @@ __device__ __forceinline__ void join_and_store(const TreeParams& p, const TreeIt
             *reinterpret_cast<float4*>(p.ws_o + at * kHD + d) = acc;
             if (d == 0) *reinterpret_cast<float2*>(p.ws_ml + at * 2) = make_float2(M, L);
         }
+    }
+}
+
+// The same where no state has to be joined and no value was odd: from the registers, eight or sixteen bytes a lane and instruction, four dims each.
+// (Over LDS in whole rows this was 16 times around a loop of 60 instructions.  With the masks at hand: 1 request of 500 tokens x 60 nodes, 32 / 8 heads,
+// 25.5 -> 23 us, 8 of 3000 x 90, 64 / 8 heads, 88 -> 82.5 us.)
+__device__ __forceinline__ void store_rows(const TreeParams& p, const TreeItem& it, const TreeState<1>& st, int row0, int h, int lane) {
+    const float l = st.l[0] + __shfl_xor(st.l[0], 32);
+    const int row = row0 + (lane & 31), half = lane >> 5;
+    if (row >= it.rows) return;
+    const int node = row / p.group;
+    const int hq = h * p.group + row - node * p.group;
+    const int64_t tok = it.base + node, pair = tok * p.Hq + hq;
+    if (p.splits > 1 && it.split == 0 && half == 0) p.ws_n[pair] = it.nsplit;
+    if (it.nsplit == 1) {
+        const float inv = l == 0.f ? 0.f : 1.0f / l;  // l == 0: the row sees nothing
+        uint16_t* out = p.out + tok * p.out_stride + hq * kHD + 4 * half;
+#pragma unroll
+        for (int mb = 0; mb < 4; ++mb)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<uint2*>(out + 32 * mb + 8 * i) = make_uint2(pack_bf16(st.o[0][mb][4 * i] * inv, st.o[0][mb][4 * i + 1] * inv),
+                                                                              pack_bf16(st.o[0][mb][4 * i + 2] * inv, st.o[0][mb][4 * i + 3] * inv));
+    } else {
+        const int64_t at = pair * p.splits + it.split;
+        float* out = p.ws_o + at * kHD + 4 * half;
+#pragma unroll
+        for (int mb = 0; mb < 4; ++mb)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<float4*>(out + 32 * mb + 8 * i) =
+                    make_float4(st.o[0][mb][4 * i], st.o[0][mb][4 * i + 1], st.o[0][mb][4 * i + 2], st.o[0][mb][4 * i + 3]);
+        if (half == 0) *reinterpret_cast<float2*>(p.ws_ml + at * 2) = make_float2(st.m[0], l);
     }
 }
 
@@ -582,7 +635,9 @@ __device__ __forceinline__ void narrow_run(const TreeParams& p, const TreeItem& 
             f32x16_t s[RB];
             bf16x8_t pf[RB][2];
             keys_of(j, s);
-            tile_mask<RB>(p, it, 0, it.t0 + (wave + j * kTreeWaves) * kTreeKeys, lane, s);
+            uint64_t word[RB];  // (a wave has one such tile as a rule: asked for at the start, its mask would only make that longer)
+            load_masks<RB>(p, it, 0, lane, word);
+            tile_mask<RB>(p, it, 0, word, it.t0 + (wave + j * kTreeWaves) * kTreeKeys, lane, s);
             tile_reference<RB>(p.scale_log2e, s, st);
             tile_probabilities<RB>(p.scale_log2e, s, st, pf);
             if (tile_values_masked<RB>(wait_values(j), lane, pf, st)) odd |= 1ull << (j - plain);
@@ -666,6 +721,8 @@ __device__ __forceinline__ void wide_run(const TreeParams& p, const TreeItem& it
     issue_words(1);
     bf16x8_t qf[1][8];
     load_queries<1>(p, it, row0, h, lane, qf);
+    uint64_t word[1];
+    load_masks<1>(p, it, row0, lane, word);
     wait_loads<0>();
     uint64_t kfrom[W::kLoads];
 #pragma unroll
@@ -818,13 +875,17 @@ __device__ __forceinline__ void wide_run(const TreeParams& p, const TreeItem& it
         refill(j);
         read_keys(tile_at(j), lane, kf);
         tile_scores<1>(kf, qf, s);
-        if (j >= plain) tile_mask<1>(p, it, row0, it.t0 + j * kTreeKeys, lane, s);
+        if (j >= plain) tile_mask<1>(p, it, row0, word, it.t0 + j * kTreeKeys, lane, s);
         tile_reference<1>(p.scale_log2e, s, st);
         tile_probabilities<1>(p.scale_log2e, s, st, pf);
         if (j < plain) tile_values<1>(tile_at(j) + kTreeHalf, lane, pf, st);
         else if (tile_values_masked<1>(tile_at(j) + kTreeHalf, lane, pf, st)) odd |= 1ull << (j - plain);
     }
     wait_loads<0>();
+    if (!__syncthreads_or(odd != 0)) {
+        store_rows(p, it, st, row0, h, lane);
+        return;
+    }
     join_and_store<1, 1, NW>(p, it, st, smem, wave, lane, odd, it.t0 + plain * kTreeKeys, kTreeKeys, [&](int g) { return it.r0 + g * 32; }, [&](int) { return h; });
 }
 template <int NW, bool NT>
