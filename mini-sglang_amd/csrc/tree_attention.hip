@@ -12,10 +12,13 @@
 // With up to 64 rows per kv head the pass over K and V bounds the kernel (a 32-key tile costs a wave 512 matrix cycles per 32 rows
 // where HBM takes 1250 cycles of the compute unit).  The work group's four waves take every fourth 32-key tile each, with RB blocks of
 // 32 rows: tiles are private to a wave, so the loop has no barrier.
-//   * K and V rows go from HBM to LDS without passing registers, 16 bytes a lane, four rows of 256 bytes an instruction, into two tile
-//     slots per wave; the XOR swizzles that spread the fragment reads over the banks are applied to the source address.
-//   * The page table is read per token, also by LDS-DMA, four tiles ahead: any page size, no scalar path, nothing the compiler counts.
-//   * All these loads are inline asm and waited for by count; their order is K0 V0 t3 K1 V1 | t4 K2 V2 | t5 K3 V3 ... (t = table entries).
+//   * K and V rows go from HBM to LDS without passing registers, 16 bytes a lane, four rows of 256 bytes an instruction; the XOR swizzles that
+//     spread the fragment reads over the banks are applied to the source address.  With one block of rows a wave has room for one tile, and
+//     a second work group fits on the compute unit: its loop runs beside the other's start and end (200 requests of 1000 tokens x 8 nodes
+//     130 -> 116 us; long runs the same).  With two blocks, one work group fits, and a wave has room for two tiles.
+//   * The page table is read per token, also by LDS-DMA, three or four tiles ahead: any page size, no scalar path, nothing the compiler counts.
+//   * All these loads are inline asm and waited for by count; their order is K0 V0 | t3 K1 V1 | t4 K2 V2 ..., two slots K0 V0 t3 K1 V1 | t4 K2 V2 ...
+//     (t = table entries).
 // Where requests are few or unequal, their tiles are dealt in equal shares (TreeWalk, tree_cut); runs of a request leave (O, max, sum) in the
 // workspace and a second kernel joins them.
 #include <type_traits>
@@ -29,7 +32,8 @@ namespace msgl {
 constexpr int kTreeWaves = 4;
 constexpr int kTreeKeys = 32;                       // keys per tile
 constexpr int kTreeHalf = kTreeKeys * kHD * 2;      // bytes of a K or V tile
-constexpr int kTreeRing = 4 * kTreeHalf;            // per wave: two K tiles, two V tiles
+constexpr int tile_slots(int rb) { return rb == 1 ? 1 : 2; }                 // narrow kernel: tiles of K, and of V, a wave has room for
+constexpr int tree_ring(int rb) { return 2 * tile_slots(rb) * kTreeHalf; }  // and their bytes
 constexpr int kTreeSlotRing = 4 * 256;              // per wave: table entries of four tiles (64 words each)
 constexpr int kTreeMergeRow = kHD + 4;              // floats per row of the exchange at the end (spread over the banks)
 constexpr int merge_bytes(int waves, int rb) { return waves * 32 * rb * (kTreeMergeRow + 2) * 4; }
@@ -547,7 +551,7 @@ __device__ __forceinline__ void store_rows(const TreeParams& p, const TreeItem& 
     }
 }
 
-// One run, up to 64 rows: tiles are private to a wave.  Measured: 64 requests of 8192 tokens x 8 nodes, 32 / 8 heads, 345 us = 6.3 TB/s, 0.89 of what a
+// One run, up to 64 rows: tiles are private to a wave.  Measured: 64 requests of 8192 tokens x 8 nodes, 32 / 8 heads, 341 us = 6.3 TB/s, 0.89 of what a
 // read-only stream reaches on this chip; with 16 nodes (two blocks of rows) 358 us.
 template <int RB>
 __device__ __forceinline__ void narrow_run(const TreeParams& p, const TreeItem& it, int h, int wave, char* smem) {
@@ -557,10 +561,11 @@ __device__ __forceinline__ void narrow_run(const TreeParams& p, const TreeItem& 
     const int T = all_tiles > wave ? (all_tiles - wave + kTreeWaves - 1) / kTreeWaves : 0;  // own tiles: wave, wave + kTreeWaves, ...
 
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
-    char* ring = smem + wave * kTreeRing;
-    char* words = smem + kTreeWaves * kTreeRing + wave * kTreeSlotRing;
-    const uint32_t ring_at = lds0 + wave * kTreeRing;
-    const uint32_t words_at = lds0 + kTreeWaves * kTreeRing + wave * kTreeSlotRing;
+    constexpr int SL = tile_slots(RB), kRing = tree_ring(RB);
+    char* ring = smem + wave * kRing;
+    char* words = smem + kTreeWaves * kRing + wave * kTreeSlotRing;
+    const uint32_t ring_at = lds0 + wave * kRing;
+    const uint32_t words_at = lds0 + kTreeWaves * kRing + wave * kTreeSlotRing;
 
     TreeState<RB> st;
     st.clear();
@@ -593,33 +598,33 @@ __device__ __forceinline__ void narrow_run(const TreeParams& p, const TreeItem& 
             uint64_t a[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) a[i] = (uint64_t)s[i] * p.slot_bytes + (values ? vfrom : kfrom[i & 3]);
-            dma_tile<true>(a, ring_at + ((values ? 2 : 0) + (j & 1)) * kTreeHalf);
+            dma_tile<true>(a, ring_at + ((values ? SL : 0) + j % SL) * kTreeHalf);
         };
         issue_rows(0, false);
         issue_rows(0, true);
-        if (T > 1) {
+        if (SL == 2 && T > 1) {
             issue_words(3);
             issue_rows(1, false);
             issue_rows(1, true);
         }
-        // outstanding behind K(j): V(j), and if there is a next tile t(j+3), K(j+1), V(j+1)
+        // two slots: outstanding behind K(j) are V(j), and if there is a next tile t(j+3), K(j+1), V(j+1); one slot: V(j)
         auto keys_of = [&](int j, f32x16_t (&s)[RB]) __attribute__((always_inline)) {
-            if (j + 1 < T) wait_loads<25>();
+            if (SL == 2 && j + 1 < T) wait_loads<25>();
             else wait_loads<8>();
             bf16x8_t kf[8];
-            read_keys(ring + (j & 1) * kTreeHalf, lane, kf);
-            if (j + 2 < T) {
-                issue_words(j + 4);
-                issue_rows(j + 2, false);
+            read_keys(ring + j % SL * kTreeHalf, lane, kf);
+            if (j + SL < T) {
+                issue_words(j + SL + 2);
+                issue_rows(j + SL, false);
             }
             tile_scores<RB>(kf, qf, s);
         };
-        // outstanding behind V(j): t(j+3), K(j+1), V(j+1), t(j+4), K(j+2)
+        // two slots: outstanding behind V(j) are t(j+3), K(j+1), V(j+1), t(j+4), K(j+2); one slot: t(j+3), K(j+1)
         auto wait_values = [&](int j) __attribute__((always_inline)) {
-            if (j + 2 < T) wait_loads<26>();
-            else if (j + 1 < T) wait_loads<17>();
+            if (SL == 2 && j + 2 < T) wait_loads<26>();
+            else if (j + 1 < T) wait_loads<SL == 2 ? 17 : 9>();
             else wait_loads<0>();
-            return ring + (2 + (j & 1)) * kTreeHalf;
+            return ring + (SL + j % SL) * kTreeHalf;
         };
         int j = 0;
         for (; j < plain; ++j) {
@@ -629,7 +634,7 @@ __device__ __forceinline__ void narrow_run(const TreeParams& p, const TreeItem& 
             tile_reference<RB>(p.scale_log2e, s, st);
             tile_probabilities<RB>(p.scale_log2e, s, st, pf);
             tile_values<RB>(wait_values(j), lane, pf, st);
-            if (j + 2 < T) issue_rows(j + 2, true);
+            if (j + SL < T) issue_rows(j + SL, true);
         }
         for (; j < T; ++j) {
             f32x16_t s[RB];
@@ -641,7 +646,7 @@ __device__ __forceinline__ void narrow_run(const TreeParams& p, const TreeItem& 
             tile_reference<RB>(p.scale_log2e, s, st);
             tile_probabilities<RB>(p.scale_log2e, s, st, pf);
             if (tile_values_masked<RB>(wait_values(j), lane, pf, st)) odd |= 1ull << (j - plain);
-            if (j + 2 < T) issue_rows(j + 2, true);
+            if (j + SL < T) issue_rows(j + SL, true);
         }
     }
     wait_loads<0>();
@@ -649,7 +654,7 @@ __device__ __forceinline__ void narrow_run(const TreeParams& p, const TreeItem& 
                             [&](int) { return h; });
 }
 template <int RB>
-__global__ __launch_bounds__(kTreeWaves * 64, 1) void tree_attention_kernel(TreeParams p) {
+__global__ __launch_bounds__(kTreeWaves * 64, tile_slots(RB) == 1 ? 2 : 1) void tree_attention_kernel(TreeParams p) {
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     // block -> (kv head, share), heads fastest: a token row's pieces are read at about the same time
     const int h = blockIdx.x % (unsigned)p.Hkv;
@@ -980,7 +985,7 @@ static int launch_tree(K kernel, PerDeviceOnce& once, int lds, int waves, const 
 }
 template <int RB>
 static int launch_narrow(const TreeParams& p, int64_t blocks, hipStream_t stream) {
-    constexpr int kTiles = kTreeWaves * (kTreeRing + kTreeSlotRing), kJoin = merge_bytes(kTreeWaves, RB);
+    constexpr int kTiles = kTreeWaves * (tree_ring(RB) + kTreeSlotRing), kJoin = merge_bytes(kTreeWaves, RB);
     static PerDeviceOnce once;
     return launch_tree(&tree_attention_kernel<RB>, once, kTiles > kJoin ? kTiles : kJoin, kTreeWaves, p, blocks, stream);
 }
@@ -1014,7 +1019,8 @@ struct TreeCut {
 };
 // A work group per request, or equal shares of all tiles, one per compute unit: whichever is done sooner, counted in tiles.  A run costs its tiles
 // and kTreeBegin for its start; a second kernel has to join shared requests, which is worth kJoin tiles (4 to 8 us; a tile takes a narrow work
-// group 0.3 us, a wide one 1.1 us).  Both sides measured, in us, work group per request | shares:
+// group 0.3 us, a wide one 1.1 us).  Shares for the two work groups per unit that fit in some forms were slower than one (64 requests of
+// 4096 to 8192 x 8 286 | 275, 12 of 8000 to 16000 x 30 126 | 112).  Both sides measured, in us, work group per request | shares:
 //   16 requests of 2000 to 4000 tokens x 16 nodes, 32 / 8 heads (128 work groups)      60 (equal runs of 1500 keys) | 47
 //   12 of 8000 to 16000 x 30 (96)  138 (same) | 112      3 of 15000 to 30000 x 70, 16 / 4 heads (24)  124 (same) | 90
 //   64 of 500 to 1000 x 8 (512)  44 | 55      64 of 4096 to 8192 x 8 (512)  280 | 278      32 of 250 to 500 x 60 (256)  34 | 41
