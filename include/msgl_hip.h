@@ -58,6 +58,9 @@ const char* msgl_last_error(void);
  *   MSGL_VARIANT_EXTEND_WIDE      0 = eight waves (one head each), 1 = four waves (both heads each)
  *   MSGL_VARIANT_EXTEND_RING      2 / 3 slots in the K/V tile ring of the eight-wave extend kernel
  *   MSGL_VARIANT_EXTEND_KEY_SPLIT 1..8 key runs per extend work item (needs the workspace)
+ *   MSGL_VARIANT_TREE_FORM        above 32 rows per kv head: 0 = row tiles of 32, 1 = the form that reads the keys once
+ *                                 per 64, 128 or 256 rows
+ *   MSGL_VARIANT_TREE_SHARES      0 = a tree attention work group per request, 1 = equal shares of all tiles
  * ------------------------------------------------------------------------- */
 #define MSGL_VARIANT_AUTO (-1)
 #define MSGL_VARIANT_DECODE_MFMA 0
@@ -67,7 +70,9 @@ const char* msgl_last_error(void);
 #define MSGL_VARIANT_EXTEND_RING 4
 #define MSGL_VARIANT_EXTEND_KEY_SPLIT 5
 #define MSGL_VARIANT_DECODE_MFMA_DEPTH 6
-#define MSGL_VARIANT_COUNT 7
+#define MSGL_VARIANT_TREE_FORM 7
+#define MSGL_VARIANT_TREE_SHARES 8
+#define MSGL_VARIANT_COUNT 9
 int msgl_set_variant(int which, int value);
 int msgl_get_variant(int which);
 

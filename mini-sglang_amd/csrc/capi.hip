@@ -35,7 +35,8 @@ int device_cus() {
 }
 
 static int g_variant[MSGL_VARIANT_COUNT] = {MSGL_VARIANT_AUTO, MSGL_VARIANT_AUTO, MSGL_VARIANT_AUTO, MSGL_VARIANT_AUTO,
-                                            MSGL_VARIANT_AUTO, MSGL_VARIANT_AUTO, MSGL_VARIANT_AUTO};
+                                            MSGL_VARIANT_AUTO, MSGL_VARIANT_AUTO, MSGL_VARIANT_AUTO, MSGL_VARIANT_AUTO,
+                                            MSGL_VARIANT_AUTO};
 int variant(int which) { return __atomic_load_n(&g_variant[which], __ATOMIC_RELAXED); }
 
 }  // namespace msgl

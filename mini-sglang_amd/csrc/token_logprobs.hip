@@ -10,8 +10,9 @@
 // 64-bit key: the float's bits mapped to an unsigned number that rises with the value, then the index's complement.
 // The k best of a segment: the k-th largest of a wave's 64 lane maxima is no larger than the segment's k-th largest value, so the few values
 // that reach it (in every wave's view: the largest of the four) are all that has to be ranked; so are those that reach the least of the waves'
-// k/4-th largest, and whichever bar is higher counts (the second from kTwoBars alternatives on).  A wave's k-th largest lane maximum comes from bisecting its bits with ballots.  Segments where that leaves too many (long ties that are not a fill from the segment's start on, NaN,
-// infinities) are taken apart winner by winner instead.
+// k/4-th largest, and whichever bar is higher counts (the second from kTwoBars alternatives on).  A wave's k-th largest lane maximum comes from
+// bisecting its bits with ballots.  Segments where that leaves too many (long ties that are not a fill from the segment's start on, NaN, infinities)
+// are taken apart winner by winner instead.
 #include <type_traits>
 
 #include "extend_common.h"
@@ -424,10 +425,11 @@ __global__ __launch_bounds__(kLpThreads) void logprob_row_kernel(LogprobParams p
     }
 }
 
-// Elements per thread: as many as it takes for the whole row if 32 will do (one launch instead of two: a bf16 row of 8000 tokens with five alternatives 7.8 -> 4.3 us, and 4.5 us of host time less), else 32, or 16
-// where that would be fewer than four groups per compute unit.  Measured on a vocabulary of 151936 with five
-// alternatives, us with 16 / 32 / 64 elements per thread: one bf16 row 8.3 / 9.4 / 10.1, 32 rows 10.6 / 11.2 / 12.2, 64 rows 14.2 / 13.5 / 15.1, 1000 rows
-// 94 / 87 / 91; fp32 with 8 / 16 / 32: one row 8.8 / 8.7 / 8.9, 32 rows 13.9 / 11.8 / 12.1, 64 rows 18.3 / 16.1 / 15.6, 1000 rows 153 / 114 / 105.
+// Elements per thread: as many as it takes for the whole row if 32 will do (one launch instead of two: a bf16 row of 8000 tokens with five alternatives
+// 7.8 -> 4.3 us, and 4.5 us of host time less), else 32, or 16 where that would be fewer than four groups per compute unit.  Measured on a vocabulary
+// of 151936 with five alternatives, us with 16 / 32 / 64 elements per thread: one bf16 row 8.3 / 9.4 / 10.1, 32 rows 10.6 / 11.2 / 12.2, 64 rows 14.2 /
+// 13.5 / 15.1, 1000 rows 94 / 87 / 91; fp32 with 8 / 16 / 32: one row 8.8 / 8.7 / 8.9, 32 rows 13.9 / 11.8 / 12.1, 64 rows 18.3 / 16.1 / 15.6, 1000
+// rows 153 / 114 / 105.
 static bool logprob_fits(int vocab, int bytes, int elements) { return (int64_t)vocab + 16 / bytes - 1 <= elements * kLpThreads; }
 static int logprob_elements(int rows, int vocab, int bytes) {
     if (logprob_fits(vocab, bytes, 32)) return logprob_fits(vocab, bytes, 16) ? 16 : 32;

@@ -9,9 +9,9 @@
 // packed to bf16, are the second product's operand as they stand.  (P is rounded to bf16 as that product's operand type asks: half a
 // step, 2^-8 relative at most, per probability, unbiased, and the sum is taken of the unrounded ones.)
 //
-// With up to 64 rows per kv head the pass over K and V bounds the kernel (a 32-key tile costs a wave 512 matrix cycles per 32 rows
-// where HBM takes 1250 cycles of the compute unit).  The work group's four waves take every fourth 32-key tile each, with RB blocks of
-// 32 rows: tiles are private to a wave, so the loop has no barrier.
+// The narrow kernel, for up to 64 rows per kv head and for tiles of 32 rows of small launches: the pass over K and V bounds it (a 32-key tile
+// costs a wave 512 matrix cycles per 32 rows where HBM takes 1250 cycles of the compute unit).  The work group's four waves take every fourth 32-key
+// tile each, with RB blocks of 32 rows: tiles are private to a wave, so the loop has no barrier.
 //   * K and V rows go from HBM to LDS without passing registers, 16 bytes a lane, four rows of 256 bytes an instruction; the XOR swizzles that
 //     spread the fragment reads over the banks are applied to the source address.  With one block of rows a wave has room for one tile, and
 //     a second work group fits on the compute unit: its loop runs beside the other's start and end (200 requests of 1000 tokens x 8 nodes
@@ -19,7 +19,7 @@
 //   * The page table is read per token, also by LDS-DMA, three or four tiles ahead: any page size, no scalar path, nothing the compiler counts.
 //   * All these loads are inline asm and waited for by count; their order is K0 V0 | t3 K1 V1 | t4 K2 V2 ..., two slots K0 V0 t3 K1 V1 | t4 K2 V2 ...
 //     (t = table entries).
-// Where requests are few or unequal, their tiles are dealt in equal shares (TreeWalk, tree_cut); runs of a request leave (O, max, sum) in the
+// Where requests are few or unequal, their tiles are dealt in equal shares (TreeWalk, tree_plan); runs of a request leave (O, max, sum) in the
 // workspace and a second kernel joins them.
 #include <type_traits>
 #include <utility>
@@ -222,6 +222,17 @@ struct TreeWalk {
             base += tiles, ++b;
             take(p, TreeRequest(p, b, r0), r0, it);
         }
+    }
+};
+
+// block -> (item, row tile), item = (share, kv head): heads fastest, so that a token row's pieces are read at about the same time, and the row tiles
+// of an item on the same XCD (block ids modulo 8), whose L2 then holds the keys for all of them.
+struct TreeBlock {
+    int item, row_tile;
+    __device__ __forceinline__ explicit TreeBlock(const TreeParams& p) {
+        const int y = blockIdx.x >> 3;
+        row_tile = y % p.row_tiles;
+        item = (y / p.row_tiles) * 8 + (blockIdx.x & 7);
     }
 };
 
@@ -553,7 +564,7 @@ __device__ __forceinline__ void store_rows(const TreeParams& p, const TreeItem& 
 
 // One run, up to 64 rows: tiles are private to a wave.  Measured: 64 requests of 8192 tokens x 8 nodes, 32 / 8 heads, 341 us = 6.3 TB/s, 0.89 of what a
 // read-only stream reaches on this chip; with 16 nodes (two blocks of rows) 358 us.
-template <int RB>
+template <int RB, bool NT>
 __device__ __forceinline__ void narrow_run(const TreeParams& p, const TreeItem& it, int h, int wave, char* smem) {
     const int lane = fresh_lane();
     const int g4 = lane >> 4, q16 = lane & 15;
@@ -584,7 +595,7 @@ __device__ __forceinline__ void narrow_run(const TreeParams& p, const TreeItem& 
         issue_words(1);
         issue_words(2);
         bf16x8_t qf[RB][8];
-        load_queries<RB>(p, it, 0, h, lane, qf);
+        load_queries<RB>(p, it, it.r0, h, lane, qf);
         wait_loads<0>();  // from here on the loads in flight are this kernel's to count
 
         // a lane loads piece q16 of rows 4 i + g4, so it fetches the piece that belongs there (read_keys, read_values)
@@ -598,7 +609,7 @@ __device__ __forceinline__ void narrow_run(const TreeParams& p, const TreeItem& 
             uint64_t a[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) a[i] = (uint64_t)s[i] * p.slot_bytes + (values ? vfrom : kfrom[i & 3]);
-            dma_tile<true>(a, ring_at + ((values ? SL : 0) + j % SL) * kTreeHalf);
+            dma_tile<NT>(a, ring_at + ((values ? SL : 0) + j % SL) * kTreeHalf);
         };
         issue_rows(0, false);
         issue_rows(0, true);
@@ -641,8 +652,8 @@ __device__ __forceinline__ void narrow_run(const TreeParams& p, const TreeItem& 
             bf16x8_t pf[RB][2];
             keys_of(j, s);
             uint64_t word[RB];  // (a wave has one such tile as a rule: asked for at the start, its mask would only make that longer)
-            load_masks<RB>(p, it, 0, lane, word);
-            tile_mask<RB>(p, it, 0, word, it.t0 + (wave + j * kTreeWaves) * kTreeKeys, lane, s);
+            load_masks<RB>(p, it, it.r0, lane, word);
+            tile_mask<RB>(p, it, it.r0, word, it.t0 + (wave + j * kTreeWaves) * kTreeKeys, lane, s);
             tile_reference<RB>(p.scale_log2e, s, st);
             tile_probabilities<RB>(p.scale_log2e, s, st, pf);
             if (tile_values_masked<RB>(wait_values(j), lane, pf, st)) odd |= 1ull << (j - plain);
@@ -650,27 +661,28 @@ __device__ __forceinline__ void narrow_run(const TreeParams& p, const TreeItem& 
         }
     }
     wait_loads<0>();
-    join_and_store<RB, kTreeWaves, kTreeWaves>(p, it, st, smem, wave, lane, odd, it.t0 + (wave + plain * kTreeWaves) * kTreeKeys, kTreeWaves * kTreeKeys, [](int) { return 0; },
+    join_and_store<RB, kTreeWaves, kTreeWaves>(p, it, st, smem, wave, lane, odd, it.t0 + (wave + plain * kTreeWaves) * kTreeKeys, kTreeWaves * kTreeKeys, [&](int) { return it.r0; },
                             [&](int) { return h; });
 }
-template <int RB>
+template <int RB, bool NT>
 __global__ __launch_bounds__(kTreeWaves * 64, tile_slots(RB) == 1 ? 2 : 1) void tree_attention_kernel(TreeParams p) {
     extern __shared__ __attribute__((aligned(1024))) char smem[];
-    // block -> (kv head, share), heads fastest: a token row's pieces are read at about the same time
-    const int h = blockIdx.x % (unsigned)p.Hkv;
+    const TreeBlock at(p);
+    if (at.item >= p.items) return;
+    const int r0 = at.row_tile * 32 * RB, h = at.item % p.Hkv;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     TreeItem it;
-    for (TreeWalk walk(p, blockIdx.x / (unsigned)p.Hkv, 0, threadIdx.x & 63, it); walk.any; __syncthreads(), walk.next(p, 0, it))
-        narrow_run<RB>(p, it, h, wave, smem);
+    for (TreeWalk walk(p, at.item / p.Hkv, r0, threadIdx.x & 63, it); walk.any; __syncthreads(), walk.next(p, r0, it))
+        narrow_run<RB, NT>(p, it, h, wave, smem);
 }
 
-// More than 64 rows per kv head: the NW waves hold 32 rows each and share the tiles, so that K and V are read once per 32 NW rows.  A tile is loaded by
-// all waves, 32 / NW keys each, SLOTS - 2 tiles ahead into a ring; a wave waits for its own loads of tile j, then the barrier says that everybody's
-// have landed and that everybody is done with tile j - 2, whose slot is filled anew.  Two waves per SIMD either way (NW = 8 and one work group
-// per compute unit, or NW = 4 and two): a wave issues an instruction about every eighth cycle, whatever it is, so one wave cannot keep
-// softmax and matrix products side by side.  Measured: 32 requests of 16000 tokens x 64 nodes, 32 / 8 heads, 607 us = 890 TFLOP/s, K and V at
-// 3.5 TB/s beside it (a dense product of 8192^3 reaches 1228 on this chip, whose clock gives way under such load); 40 requests of 4000 to
-// 8000 x 30 nodes (four waves) 208 us = 4.8 TB/s, bound by the issue of its one wave per SIMD.
+// The wide kernel, for more than 64 rows per kv head in large launches: the NW waves hold 32 rows each and share the tiles, so that K and V are read
+// once per 32 NW rows.  A tile is loaded by all waves, 32 / NW keys each, SLOTS - 2 tiles ahead into a ring; a wave waits for its own loads of tile j,
+// then the barrier says that everybody's have landed and that everybody is done with tile j - 2, whose slot is filled anew.  Two waves per SIMD either
+// way (NW = 8 and one work group per compute unit, or NW = 4 and two): a wave issues an instruction about every eighth cycle, whatever it is, so one
+// wave cannot keep softmax and matrix products side by side.  Measured: 32 requests of 16000 tokens x 64 nodes, 32 / 8 heads, 607 us = 890 TFLOP/s, K
+// and V at 3.5 TB/s beside it (a dense product of 8192^3 reaches 1228 on this chip, whose clock gives way under such load); 40 requests of 4000 to 8000
+// x 30 nodes (four waves) 208 us = 4.8 TB/s, bound by the issue of its one wave per SIMD.
 template <int NW>
 struct TreeWide {
     static constexpr int kSlots = NW == 8 ? 8 : 4;
@@ -896,15 +908,12 @@ __device__ __forceinline__ void wide_run(const TreeParams& p, const TreeItem& it
 template <int NW, bool NT>
 __global__ __launch_bounds__(NW * 64, 2) void tree_attention_wide_kernel(TreeParams p) {
     extern __shared__ __attribute__((aligned(1024))) char smem[];
-    // block -> item, row tile: the row tiles of an item run on the same XCD (block ids modulo 8), whose L2 then holds the keys for all of them
-    const int y = blockIdx.x >> 3;
-    const int rt = y % p.row_tiles;
-    const int item = (y / p.row_tiles) * 8 + (blockIdx.x & 7);
-    if (item >= p.items) return;
-    const int h = item % p.Hkv;
+    const TreeBlock at(p);
+    if (at.item >= p.items) return;
+    const int r0 = at.row_tile * 32 * NW, h = at.item % p.Hkv;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     TreeItem it;
-    for (TreeWalk walk(p, item / p.Hkv, rt * 32 * NW, threadIdx.x & 63, it); walk.any; __syncthreads(), walk.next(p, rt * 32 * NW, it))
+    for (TreeWalk walk(p, at.item / p.Hkv, r0, threadIdx.x & 63, it); walk.any; __syncthreads(), walk.next(p, r0, it))
         wide_run<NW, NT>(p, it, h, wave, smem);
 }
 
@@ -983,11 +992,11 @@ static int launch_tree(K kernel, PerDeviceOnce& once, int lds, int waves, const 
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(waves * 64), lds, stream, p);
     return check_launch("tree_attention_kernel");
 }
-template <int RB>
+template <int RB, bool NT>
 static int launch_narrow(const TreeParams& p, int64_t blocks, hipStream_t stream) {
     constexpr int kTiles = kTreeWaves * (tree_ring(RB) + kTreeSlotRing), kJoin = merge_bytes(kTreeWaves, RB);
     static PerDeviceOnce once;
-    return launch_tree(&tree_attention_kernel<RB>, once, kTiles > kJoin ? kTiles : kJoin, kTreeWaves, p, blocks, stream);
+    return launch_tree(&tree_attention_kernel<RB, NT>, once, kTiles > kJoin ? kTiles : kJoin, kTreeWaves, p, blocks, stream);
 }
 template <int NW, bool NT>
 static int launch_wide(const TreeParams& p, int64_t blocks, hipStream_t stream) {
@@ -998,50 +1007,66 @@ static int launch_wide(const TreeParams& p, int64_t blocks, hipStream_t stream) 
 constexpr int kMaxTreeSplits = 256;
 constexpr int kMostKeys = 1 << 30;  // keys of a request: positions plus a run stay inside 32 bits
 
-// How the rows of a kv head are dealt: up to 64 to waves that share them and take different keys, more to waves that hold 32 or 64 rows each and
-// share the keys.
-struct TreeShape {
-    int waves;  // 0: the narrow kernel
-    int rb, row_tiles;
+// How a launch is laid out: the kernel (waves of the wide one, 0: the narrow one with rb blocks of 32 rows), its row tiles, work groups per
+// (kv head, row tile), most runs of a request (1: a work group per request).
+struct TreePlan {
+    int waves, rb, row_tiles, shares, splits;
+    int64_t cost;  // ns
 };
-static TreeShape tree_shape(int max_q, int Hq, int Hkv) {
-    const int64_t rows = (int64_t)max_q * (Hq / Hkv);
-    TreeShape s;
-    s.waves = rows <= 64 ? 0 : rows <= 128 ? 4 : 8;
-    s.rb = rows > 32 && rows <= 64 ? 2 : 1;
-    s.row_tiles = s.waves ? (int)((rows + 32 * s.waves - 1) / (32 * s.waves)) : 1;
-    return s;
-}
-
-// How a launch is cut: work groups per (kv head, row tile), and most runs of a request (1: a work group per request).
-struct TreeCut {
-    int shares, splits;
-};
-// A work group per request, or equal shares of all tiles, one per compute unit: whichever is done sooner, counted in tiles.  A run costs its tiles
-// and kTreeBegin for its start; a second kernel has to join shared requests, which is worth kJoin tiles (4 to 8 us; a tile takes a narrow work
-// group 0.3 us, a wide one 1.1 us).  Shares for the two work groups per unit that fit in some forms were slower than one (64 requests of
-// 4096 to 8192 x 8 286 | 275, 12 of 8000 to 16000 x 30 126 | 112).  Both sides measured, in us, work group per request | shares:
+// The cost of a layout: a work group per request, or equal shares of all tiles, one per compute unit, whichever is done sooner, counted in tiles. A
+// run costs its tiles and kTreeBegin for its start; a second kernel has to join shared requests, which is worth `join` tiles (4 to 8 us). Then
+// the tiles' time, or the memory's (2.6 ns per tile of one kv head; narrow row tiles of an item drift apart and read most of it again).
+// Measured, in us, work group per request | shares (two shares per unit where two work groups fit were slower: 12 requests of 8000 to 16000 x 30
+// nodes, 32 / 8 heads, 126 instead of 112):
 //   16 requests of 2000 to 4000 tokens x 16 nodes, 32 / 8 heads (128 work groups)      60 (equal runs of 1500 keys) | 47
 //   12 of 8000 to 16000 x 30 (96)  138 (same) | 112      3 of 15000 to 30000 x 70, 16 / 4 heads (24)  124 (same) | 90
-//   64 of 500 to 1000 x 8 (512)  44 | 55      64 of 4096 to 8192 x 8 (512)  280 | 278      32 of 250 to 500 x 60 (256)  34 | 41
-//   1 of 1000 x 4, 16 / 8 heads (8)  15 | 20      1 of 2000 x 4 (8)  20 | 20      1 of 500 x 60 (8)  28 | 24      7 of 500 to 1000 x 4 (56)  17 | 19
-static TreeCut tree_cut(int bs, int max_q, int max_k, int64_t total_kv, int Hq, int Hkv) {
-    const TreeCut whole = {bs, 1};
-    if (bs <= 0 || bs > 65535 || max_q <= 0 || max_k <= 0 || Hkv <= 0 || Hq < Hkv) return whole;
-    const TreeShape sh = tree_shape(max_q, Hq, Hkv);
-    const int64_t units = device_cus(), across = (int64_t)Hkv * sh.row_tiles;
-    const int64_t most = ((int64_t)max_k + kTreeKeys - 1) / kTreeKeys;
-    const int64_t tiles = total_kv > 0 && total_kv < (int64_t)bs * max_k ? total_kv / kTreeKeys + bs : bs * most;
-    const int64_t mean = (tiles + bs - 1) / bs;
-    const int64_t all = tiles + (int64_t)bs * kTreeBegin;
-    const int64_t least = sh.waves ? 6 : kLeastTiles, kJoin = sh.waves ? 6 : 28;
+//   64 of 500 to 1000 x 8 (512)  44 | 55      48 of 4096 to 8192 x 8 (384)  243 | 207      32 of 250 to 500 x 60 (256)  34 | 41
+//   1 of 1000 x 4, 16 / 8 heads (8)  15 | 20      1 of 2000 x 4 (8)  20 | 20      7 of 500 to 1000 x 4 (56)  17 | 19
+static TreePlan tree_plan_of(int waves, int rb, int tile_ns, int64_t rows, int bs, int max_k, int64_t tiles, int Hkv) {
+    const int64_t units = device_cus(), tile_rows = 32 * (waves ? waves : rb), row_tiles = (rows + tile_rows - 1) / tile_rows;
+    const int64_t across = Hkv * row_tiles, items = bs * across;
+    const int64_t most = ((int64_t)max_k + kTreeKeys - 1) / kTreeKeys, mean = (tiles + bs - 1) / bs, all = tiles + (int64_t)bs * kTreeBegin;
+    const int64_t least = waves ? 6 : kLeastTiles, join = waves ? 6 : 28;
     int64_t shares = across < units ? units / across : 1;
     if (shares > (all + least - 1) / least) shares = (all + least - 1) / least;
     const int64_t len = (all + shares - 1) / shares;
-    const int64_t alone = bs * across <= units ? kTreeBegin + most : (kTreeBegin + mean) * bs * across / units + most - mean;
-    if (alone <= kTreeBegin + len + kJoin) return whole;
-    const int64_t splits = (most + len - 1) / len + 1;
-    return {(int)shares, (int)(splits < kMaxTreeSplits ? splits : kMaxTreeSplits)};
+    const bool two_fit = waves == 4 || (waves == 0 && rb == 1);
+    const int64_t alone = items <= units ? kTreeBegin + most : (kTreeBegin + mean) * (two_fit ? items : (items + units - 1) / units * units) / units + most - mean;
+    const int64_t shared = kTreeBegin + len + join;
+    TreePlan t = {waves, rb, (int)row_tiles, bs, 1, alone * tile_ns};
+    const int forced = variant(MSGL_VARIANT_TREE_SHARES);
+    if (forced < 0 ? shared < alone : forced == 1) {
+        const int64_t splits = (most + len - 1) / len + 1;
+        t.shares = (int)shares, t.splits = (int)(splits < kMaxTreeSplits ? splits : kMaxTreeSplits), t.cost = shared * tile_ns;
+    }
+    const int64_t memory = tiles * Hkv * 26 / 10 * (!waves && row_tiles > 1 ? 7 : 4) / 4 + kTreeBegin * tile_ns;
+    if (t.cost < memory) t.cost = memory;
+    return t;
+}
+// More than 32 rows per kv head: row tiles of 32 in the narrow kernel's smaller form, which starts soonest and fits twice on a compute unit, or the
+// form that reads K and V once (64 rows) or once per 128 or 256 rows.  The tile times are those of the forms with enough to do. Measured with
+// 32 / 8 heads, three sets of inputs in turn, us, row tiles of 32 | the other form:
+//   requests x nodes    300 tokens    1000        4000        16000 (ragged: half to all of them)
+//   1 x 16              13 | 15       14 | 21     18 | 21     21 | 28
+//   16 x 16             13 | 16       16 | 24     59 | 48
+//   1 x 60              13 | 22       15 | 25     20 | 32     43 | 43
+//   4 x 60              13 | 23       16 | 30     35 | 41     130 | 68
+//   16 x 60             25 | 25       37 | 41     112 | 73
+//   100 x 30            73 | 42       130 | 81
+static TreePlan tree_plan(int bs, int max_q, int max_k, int64_t total_kv, int Hq, int Hkv) {
+    const TreePlan none = {0, 1, 1, bs, 1, 0};
+    if (bs <= 0 || max_q <= 0 || max_k <= 0 || Hkv <= 0 || Hq < Hkv) return none;
+    const int64_t rows = (int64_t)max_q * (Hq / Hkv);
+    const int64_t tiles = total_kv > 0 && total_kv < (int64_t)bs * max_k ? total_kv / kTreeKeys + bs : bs * (((int64_t)max_k + kTreeKeys - 1) / kTreeKeys);
+    auto of = [&](int waves, int rb, int tile_ns) { return tree_plan_of(waves, rb, tile_ns, rows, bs, max_k, tiles, Hkv); };
+    TreePlan best = of(0, 1, 250);
+    if (rows > 32) {
+        const TreePlan other = rows <= 64 ? of(0, 2, 490) : rows <= 128 ? of(4, 1, 650) : of(8, 1, 1100);
+        const int forced = variant(MSGL_VARIANT_TREE_FORM);
+        if (forced < 0 ? other.cost <= best.cost : forced == 1) best = other;
+    }
+    if (bs > 65535) best.shares = bs, best.splits = 1;
+    return best;
 }
 
 }  // namespace msgl
@@ -1049,7 +1074,7 @@ static TreeCut tree_cut(int bs, int max_q, int max_k, int64_t total_kv, int Hq, 
 using namespace msgl;
 
 extern "C" int msgl_tree_attention_splits(int bs, int max_seqlen_q, int max_seqlen_k, int64_t total_kv, int Hq, int Hkv) {
-    return tree_cut(bs, max_seqlen_q, max_seqlen_k, total_kv, Hq, Hkv).splits;
+    return tree_plan(bs, max_seqlen_q, max_seqlen_k, total_kv, Hq, Hkv).splits;
 }
 extern "C" size_t msgl_tree_attention_workspace_bytes(int64_t total_tokens, int Hq, int D, int splits) {
     if (total_tokens <= 0 || Hq <= 0 || D <= 0 || splits <= 1) return 0;
@@ -1086,35 +1111,32 @@ extern "C" int msgl_tree_attention(const void* q, int64_t q_stride, const void* 
     p.mask = tree_mask, p.words = mask_words;
     p.out = static_cast<uint16_t*>(out), p.out_stride = out_stride;
     p.bs = bs, p.Hq = Hq, p.Hkv = Hkv, p.group = Hq / Hkv, p.max_q = max_seqlen_q;
-    const TreeShape sh = tree_shape(max_seqlen_q, Hq, Hkv);
-    p.row_tiles = sh.row_tiles;
+    TreePlan plan = tree_plan(bs, max_seqlen_q, max_seqlen_k, total_kv, Hq, Hkv);
+    p.row_tiles = plan.row_tiles;
     p.scale_log2e = scale * 1.44269504088896340736f;
-    TreeCut cut = tree_cut(bs, max_seqlen_q, max_seqlen_k, total_kv, Hq, Hkv);
-    if (cut.splits > 1) {  // as many runs as the workspace has room for
+    if (plan.splits > 1) {  // as many runs as the workspace has room for
         const size_t per_row = workspace ? workspace_bytes / sizeof(float) / ((size_t)total_tokens * Hq) : 0;
         const size_t room = per_row ? (per_row - 1) / (D + 2) : 0;
-        if ((size_t)cut.splits > room) cut.splits = (int)room;
-        if (cut.splits < 2) cut = {bs, 1};
+        if ((size_t)plan.splits > room) plan.splits = (int)room;
+        if (plan.splits < 2) plan.splits = 1, plan.shares = bs;
     }
-    const int splits = cut.splits;
-    p.splits = splits, p.shares = cut.shares;
+    const int splits = plan.splits;
+    p.splits = splits, p.shares = plan.shares;
     p.ws_o = static_cast<float*>(workspace);
     p.ws_ml = p.ws_o + (splits > 1 ? (size_t)total_tokens * Hq * splits * kHD : 0);
     p.ws_n = reinterpret_cast<int32_t*>(p.ws_ml + (splits > 1 ? (size_t)total_tokens * Hq * splits * 2 : 0));
     MSGL_REQUIRE(splits == 1 || aligned16(workspace), "msgl_tree_attention: workspace must be 16-byte aligned");
-    const int64_t items = (int64_t)cut.shares * Hkv;
-    const int64_t blocks = sh.waves ? (items + 7) / 8 * 8 * p.row_tiles : items;
+    const int64_t items = (int64_t)plan.shares * Hkv;
+    const int64_t blocks = (items + 7) / 8 * 8 * p.row_tiles;
     MSGL_REQUIRE(blocks <= 0x7fffff, "msgl_tree_attention: %lld work groups", (long long)blocks);
     p.items = (int)items;
     const hipStream_t st = static_cast<hipStream_t>(stream);
+    const bool once = p.row_tiles == 1;  // K and V are read by one work group: past the caches
     int rc;
-    if (sh.waves) {
-        const bool once = p.row_tiles == 1;  // K and V are read by one work group: past the caches
-        if (sh.waves == 4) rc = once ? launch_wide<4, true>(p, blocks, st) : launch_wide<4, false>(p, blocks, st);
-        else rc = once ? launch_wide<8, true>(p, blocks, st) : launch_wide<8, false>(p, blocks, st);
-    } else {
-        rc = sh.rb == 1 ? launch_narrow<1>(p, blocks, st) : launch_narrow<2>(p, blocks, st);
-    }
+    if (plan.waves == 8) rc = once ? launch_wide<8, true>(p, blocks, st) : launch_wide<8, false>(p, blocks, st);
+    else if (plan.waves == 4) rc = launch_wide<4, true>(p, blocks, st);
+    else if (plan.rb == 2) rc = launch_narrow<2, true>(p, blocks, st);
+    else rc = once ? launch_narrow<1, true>(p, blocks, st) : launch_narrow<1, false>(p, blocks, st);
     if (rc != MSGL_OK || splits == 1) return rc;
     // half-waves per row: as many as there are runs for, up to eight
     const unsigned rows = (unsigned)max_seqlen_q * Hq;

@@ -215,8 +215,9 @@ __global__ __launch_bounds__(256) void extend_prepare_tree_kernel(ExtendPrepPara
 }
 
 // Both phases in one launch: what bounds a step is latency, and one launch with one barrier has the least of it (4 requests of 8 nodes 4.9 + 2.4 ->
-// 4.1 us, 200 prompts of 450 to 900 tokens 5.1 + 4 -> 6.2 us).  Every work group counts all requests and places its share of the tokens; the first writes the lengths.  In place, where a work group's
-// inputs are the first's outputs, there is only the first, and only for steps of a few thousand tokens.  Counts fit 32 bits (one_launch).
+// 4.1 us, 200 prompts of 450 to 900 tokens 5.1 + 4 -> 6.2 us).  Every work group counts all requests and places its share of the tokens; the first
+// writes the lengths.  In place, where a work group's inputs are the first's outputs, there is only the first, and only for steps of a few thousand
+// tokens.  Counts fit 32 bits (one_launch).
 constexpr int kSmallRequests = 1024, kSmallTokens = 4096, kMostSmall = 1 << 20;
 static bool one_launch(int bs, int32_t capacity, int32_t max_ctx, bool in_place) {
     return bs <= kSmallRequests && capacity <= (in_place ? kSmallTokens : kMostSmall) && max_ctx <= kMostSmall;
