@@ -1011,7 +1011,7 @@ constexpr int kMostKeys = 1 << 30;  // keys of a request: positions plus a run s
 // (kv head, row tile), most runs of a request (1: a work group per request).
 struct TreePlan {
     int waves, rb, row_tiles, shares, splits;
-    int64_t cost;  // ns
+    double cost;  // ns
 };
 // The cost of a layout: a work group per request, or equal shares of all tiles, one per compute unit, whichever is done sooner, counted in tiles. A
 // run costs its tiles and kTreeBegin for its start; a second kernel has to join shared requests, which is worth `join` tiles (4 to 8 us). Then
@@ -1031,15 +1031,15 @@ static TreePlan tree_plan_of(int waves, int rb, int tile_ns, int64_t rows, int b
     if (shares > (all + least - 1) / least) shares = (all + least - 1) / least;
     const int64_t len = (all + shares - 1) / shares;
     const bool two_fit = waves == 4 || (waves == 0 && rb == 1);
-    const int64_t alone = items <= units ? kTreeBegin + most : (kTreeBegin + mean) * (two_fit ? items : (items + units - 1) / units * units) / units + most - mean;
-    const int64_t shared = kTreeBegin + len + join;
+    const double rounds = two_fit ? (double)items / units : (double)((items + units - 1) / units);
+    const double alone = items <= units ? kTreeBegin + most : (kTreeBegin + mean) * rounds + most - mean, shared = kTreeBegin + len + join;
     TreePlan t = {waves, rb, (int)row_tiles, bs, 1, alone * tile_ns};
     const int forced = variant(MSGL_VARIANT_TREE_SHARES);
     if (forced < 0 ? shared < alone : forced == 1) {
         const int64_t splits = (most + len - 1) / len + 1;
         t.shares = (int)shares, t.splits = (int)(splits < kMaxTreeSplits ? splits : kMaxTreeSplits), t.cost = shared * tile_ns;
     }
-    const int64_t memory = tiles * Hkv * 26 / 10 * (!waves && row_tiles > 1 ? 7 : 4) / 4 + kTreeBegin * tile_ns;
+    const double memory = 2.6 * tiles * Hkv * (!waves && row_tiles > 1 ? 1.75 : 1.0) + kTreeBegin * tile_ns;
     if (t.cost < memory) t.cost = memory;
     return t;
 }
