@@ -623,13 +623,17 @@ LOGPROBS_MAX_TOP = 32      # MSGL_LOGPROBS_MAX_TOP
 
 # These wrappers sit in a decode step's critical path at a handful of microseconds of kernel each: they test first and word the complaint only when
 # there is one.
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+_INT32, _INT64 = torch.int32, torch.int64
+
+
 def _launch(index: int, entry, *args) -> None:
     """entry(*args, stream) on the device's current stream, with that device current while the kernels are launched."""
-    if torch.cuda.current_device() == index:
+    if _current_device() == index:
         status = entry(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
@@ -645,25 +649,28 @@ def _gpu_index(t: torch.Tensor, name: str) -> int:
 
 
 def _i32_on(index: int, n: int, names: str, *tensors: torch.Tensor) -> None:
-    """Every tensor is a dense 1-D int32 tensor of n entries on device `index`; `names`, space separated, for the complaint."""
+    """Every tensor is a dense int32 tensor of n entries on device `index`; `names`, space separated, for the complaint."""
+    i32 = _INT32
     for t in tensors:
-        if t.dtype is not torch.int32 or t.numel() != n or t.get_device() != index or t.dim() != 1 or not t.is_contiguous():
+        if t.dtype is not i32 or t.numel() != n or t.get_device() != index or not t.is_contiguous():
             name = names.split()[[x is t for x in tensors].index(True)]
-            raise ValueError(f"{name} must be a contiguous 1-D int32 tensor of {n} entries on the same GPU as the others "
+            raise ValueError(f"{name} must be a contiguous int32 tensor of {n} entries on the same GPU as the others "
                              f"(got {t.dtype} {tuple(t.shape)}, strides {t.stride()}, on {t.device})")
 
 
 def _table_on(index: int, t: torch.Tensor, name: str) -> None:
-    if t.get_device() != index or t.dtype is not torch.int32 or t.dim() != 2 or t.stride(1) != 1 or t.stride(0) < t.shape[1]:
+    strides = t.stride()
+    if t.get_device() != index or t.dtype is not _INT32 or len(strides) != 2 or strides[1] != 1 or strides[0] < t.shape[1]:
         raise ValueError(f"{name} must be an int32 [reqs, ctx] tensor with dense rows on the same GPU as the others")
 
 
 def _mask_on(index: int, t: torch.Tensor, rows: int) -> int:
     """Words per row of a tree mask."""
-    if t.get_device() != index or t.dtype is not torch.int64 or t.dim() != 2 or t.shape[0] != rows or not t.is_contiguous() \
-            or not 1 <= t.shape[1] <= TREE_MAX_WORDS:
+    shape = t.shape
+    if t.get_device() != index or t.dtype is not _INT64 or len(shape) != 2 or shape[0] != rows or not t.is_contiguous() \
+            or not 1 <= shape[1] <= TREE_MAX_WORDS:
         raise ValueError(f"tree_mask must be a contiguous int64 [{rows}, 1..{TREE_MAX_WORDS}] tensor on the same GPU as the others")
-    return t.shape[1]
+    return shape[1]
 
 
 def _scratch(workspace: Optional[torch.Tensor], need: int, index: int) -> Tuple[Optional[torch.Tensor], Optional[int], int]:
@@ -763,7 +770,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     if T and not 0 < max_seqlen_q <= 64 * words:
         raise ValueError(f"max_seqlen_q {max_seqlen_q} outside 1..{64 * words} (64 nodes per mask word)")
     if out is None:
-        out = q.new_empty((T, Hq, D))
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((T, Hq, D))
         out_stride = Hq * D
     else:
         if out.get_device() != index or out.dtype is not torch.bfloat16 or out.shape != q.shape or out.stride()[1:] != (D, 1):
@@ -784,11 +791,11 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
 
 def _cache_on(index: int, k: torch.Tensor, v: torch.Tensor, D: int) -> Tuple[int, int, int]:
     """(slots, Hkv, slot stride) of a [slots, Hkv, D] K/V pair on device `index`, heads dense per slot."""
-    stride = k.stride()
-    if k.dtype is not torch.bfloat16 or v.dtype is not torch.bfloat16 or k.get_device() != index or v.get_device() != index or k.dim() != 3 \
-            or k.shape != v.shape or k.shape[2] != D or stride != v.stride() or stride[1:] != (D, 1) or stride[0] < k.shape[1] * D:
+    stride, shape, bf16 = k.stride(), k.shape, torch.bfloat16
+    if k.dtype is not bf16 or v.dtype is not bf16 or k.get_device() != index or v.get_device() != index or len(shape) != 3 or shape != v.shape \
+            or shape[2] != D or stride != v.stride() or stride[1] != D or stride[2] != 1 or stride[0] < shape[1] * D:
         raise ValueError(f"k_cache / v_cache must be bfloat16 [slots, Hkv, {D}] of one slot stride on the same GPU as the others, [Hkv, D] dense per slot")
-    return k.shape[0], k.shape[1], stride[0]
+    return shape[0], shape[1], stride[0]
 
 
 @dataclass
@@ -864,14 +871,17 @@ def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, top_k: int = 0
     _i32_on(index, rows, "token_ids", token_ids)
     if not 0 <= top_k <= min(vocab, LOGPROBS_MAX_TOP):
         raise ValueError(f"top_k {top_k} outside 0..min(vocab, {LOGPROBS_MAX_TOP})")
-    logprobs, entropy = logits.new_empty(rows, dtype=torch.float32), logits.new_empty(rows, dtype=torch.float32)
-    ids, top = token_ids.new_empty((rows, top_k)), logits.new_empty((rows, top_k), dtype=torch.float32)
+    per = rows * top_k
+    results = logits.new_empty(2 * (rows + per), dtype=torch.float32)  # one allocation
+    logprobs, entropy, top, ids = results.split_with_sizes((rows, rows, per, per))
+    ids, top = ids.view(_INT32).view(rows, top_k), top.view(rows, top_k)
     if rows:
         size = 2 if logits.dtype is torch.bfloat16 else 4
         need = _lib.msgl_token_logprobs_workspace_bytes(rows, vocab, size, top_k) if workspace is None else 0
         ws, ws_at, ws_bytes = _scratch(workspace, need, index)
-        _launch(index, _lib.msgl_token_logprobs, logits.data_ptr(), rs, size, token_ids.data_ptr(), logprobs.data_ptr(), entropy.data_ptr(),
-                ids.data_ptr() if top_k else None, top.data_ptr() if top_k else None, rows, vocab, top_k, ws_at, ws_bytes)
+        at = results.data_ptr()
+        _launch(index, _lib.msgl_token_logprobs, logits.data_ptr(), rs, size, token_ids.data_ptr(), at, at + 4 * rows,
+                at + 8 * rows + 4 * per, at + 8 * rows, rows, vocab, top_k, ws_at, ws_bytes)
     return logprobs, entropy, ids, top
 
 
