@@ -23,7 +23,8 @@ _REFUSED = {1: "free list exhausted", 2: "context longer than the page table row
 class TreeDecoder:
     """``max_nodes``: most nodes of a request's tree, the root (its last token) included.  ``max_new_tokens``: how far the contexts may grow
     before the captured bounds have to be renewed (done when needed).  ``logprobs``: None, or the number of alternatives to report with every
-    accepted token's log probability (``last_logprobs``)."""
+    accepted token's log probability (``last_logprobs``).  The step is captured inside torch's inference mode, like this package's other captured
+    loops: as long as such a graph was the first one alive in the process, torch refuses captures outside inference mode."""
 
     def __init__(self, model_runner, batch: BatchInfo, max_nodes: int, *, max_new_tokens: int = 1024, logprobs: Optional[int] = None,
                  use_graph: bool = True):

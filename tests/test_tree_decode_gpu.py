@@ -1,11 +1,20 @@
 """The speculative step as it is used: slots and masks, the model over all nodes with tree attention, greedy tokens, log probabilities, acceptance and
 the move of cache rows, captured in one graph, on a small stack; its tokens are those of plain greedy decoding whatever was drafted."""
+import gc
 import random
 
 import pytest
 import torch
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def no_decoder_outlives_its_test():
+    """torch's captured graphs share the generator's two seed tensors, made by the first of them that is alive: made inside inference mode, where this
+    package captures its steps, they would refuse a capture outside it.  (A test that expects exceptions leaves its decoder to the collector.)"""
+    yield
+    gc.collect()
 
 
 def _build(ps, lens, budget=96, use_graph=False):

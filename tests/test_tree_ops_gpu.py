@@ -192,7 +192,7 @@ def test_tree_attention_captured_and_on_another_stream():
     _check(out, first)
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph):
+    with torch.inference_mode(), torch.cuda.graph(graph):
         step()
     for c in (second, first, second):
         load(c)
@@ -484,7 +484,7 @@ def test_token_logprobs_captured():
     ops.token_logprobs(x, tok, 5, workspace=ws)
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph):
+    with torch.inference_mode(), torch.cuda.graph(graph):
         out = ops.token_logprobs(x, tok, 5, workspace=ws)
     for seed in range(3):
         x.copy_(torch.randn(4, 30001, generator=torch.Generator().manual_seed(seed)) * 3)

@@ -46,7 +46,7 @@ def test_two_graphs_with_workspaces_of_their_own_making():
     pool = torch.cuda.graph_pool_handle()
     for i, a in enumerate(args):
         g = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(g, pool=pool):
+        with torch.inference_mode(), torch.cuda.graph(g, pool=pool):
             outs.append((ops.tree_attention(*a), *ops.token_logprobs(scaled[i], tok, 6)))
         graphs.append(g)
     for order in ([0, 1], [1, 0], [0, 0, 1]):
@@ -137,7 +137,7 @@ def test_a_step_over_and_over_in_place_and_captured():
     step(captured, layers[1])     # no request has a node: nothing changes
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph):
+    with torch.inference_mode(), torch.cuda.graph(graph):
         step(captured, layers[1])
     total = 0
     for i in range(25):
