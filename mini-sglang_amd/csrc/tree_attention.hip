@@ -60,6 +60,7 @@ struct TreeParams {
     float* ws_ml;  // [token][head][split][2]
     int32_t* ws_n; // [token][head]: runs
     int bs, Hq, Hkv, group;
+    int hq_shift, hkv_shift, group_shift;  // (all powers of two)
     int items, row_tiles, splits, shares;
     int max_q;
     float scale_log2e;
@@ -278,8 +279,8 @@ __device__ __forceinline__ void load_queries(const TreeParams& p, const TreeItem
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
         const int r = min(row0 + rb * 32 + (lane & 31), it.rows - 1);
-        const int node = r / p.group;
-        const uint16_t* qp = p.q + (int64_t)(it.base + node) * p.q_stride + (h * p.group + r - node * p.group) * kHD + (lane >> 5) * 8;
+        const int node = r >> p.group_shift;
+        const uint16_t* qp = p.q + (int64_t)(it.base + node) * p.q_stride + (h * p.group + (r & (p.group - 1))) * kHD + (lane >> 5) * 8;
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) qf[rb][ks] = as_bf16x8(*reinterpret_cast<const uint4*>(qp + ks * 16));
     }
@@ -322,7 +323,7 @@ __device__ __forceinline__ void tile_scores(const bf16x8_t (&kf)[8], const bf16x
 }
 
 __device__ __forceinline__ const uint64_t* row_mask(const TreeParams& p, const TreeItem& it, int row) {
-    return p.mask + (int64_t)(it.base + min(row, it.rows - 1) / p.group) * p.words;
+    return p.mask + (int64_t)(it.base + (min(row, it.rows - 1) >> p.group_shift)) * p.words;
 }
 // What a row sees of the tile that begins at key0: bit k for key k.  word: its mask, if that is one word.
 __device__ __forceinline__ uint32_t row_sees(const TreeParams& p, const TreeItem& it, int row, uint64_t word, int key0) {
@@ -514,8 +515,8 @@ __device__ __forceinline__ void join_and_store(const TreeParams& p, const TreeIt
             const float4 x = *reinterpret_cast<const float4*>(lds_o + ((g * WPH + w) * R + r) * kTreeMergeRow + d);
             acc.x += f * x.x, acc.y += f * x.y, acc.z += f * x.z, acc.w += f * x.w;
         }
-        const int node = row / p.group;
-        const int hq = head(g) * p.group + row - node * p.group;
+        const int node = row >> p.group_shift;
+        const int hq = head(g) * p.group + (row & (p.group - 1));
         const int64_t tok = it.base + node;
         if (p.splits > 1 && it.split == 0 && d == 0) p.ws_n[tok * p.Hq + hq] = it.nsplit;
         if (it.nsplit == 1) {
@@ -536,8 +537,8 @@ __device__ __forceinline__ void store_rows(const TreeParams& p, const TreeItem& 
     const float l = st.l[0] + __shfl_xor(st.l[0], 32);
     const int row = row0 + (lane & 31), half = lane >> 5;
     if (row >= it.rows) return;
-    const int node = row / p.group;
-    const int hq = h * p.group + row - node * p.group;
+    const int node = row >> p.group_shift;
+    const int hq = h * p.group + (row & (p.group - 1));
     const int64_t tok = it.base + node, pair = tok * p.Hq + hq;
     if (p.splits > 1 && it.split == 0 && half == 0) p.ws_n[pair] = it.nsplit;
     if (it.nsplit == 1) {
@@ -669,10 +670,10 @@ __global__ __launch_bounds__(kTreeWaves * 64, tile_slots(RB) == 1 ? 2 : 1) void 
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     const TreeBlock at(p);
     if (at.item >= p.items) return;
-    const int r0 = at.row_tile * 32 * RB, h = at.item % p.Hkv;
+    const int r0 = at.row_tile * 32 * RB, h = at.item & (p.Hkv - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     TreeItem it;
-    for (TreeWalk walk(p, at.item / p.Hkv, r0, threadIdx.x & 63, it); walk.any; __syncthreads(), walk.next(p, r0, it))
+    for (TreeWalk walk(p, at.item >> p.hkv_shift, r0, threadIdx.x & 63, it); walk.any; __syncthreads(), walk.next(p, r0, it))
         narrow_run<RB, NT>(p, it, h, wave, smem);
 }
 
@@ -910,10 +911,10 @@ __global__ __launch_bounds__(NW * 64, 2) void tree_attention_wide_kernel(TreePar
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     const TreeBlock at(p);
     if (at.item >= p.items) return;
-    const int r0 = at.row_tile * 32 * NW, h = at.item % p.Hkv;
+    const int r0 = at.row_tile * 32 * NW, h = at.item & (p.Hkv - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     TreeItem it;
-    for (TreeWalk walk(p, at.item / p.Hkv, r0, threadIdx.x & 63, it); walk.any; __syncthreads(), walk.next(p, r0, it))
+    for (TreeWalk walk(p, at.item >> p.hkv_shift, r0, threadIdx.x & 63, it); walk.any; __syncthreads(), walk.next(p, r0, it))
         wide_run<NW, NT>(p, it, h, wave, smem);
 }
 
@@ -977,8 +978,8 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeParams p) {
     }
     if (!live) return;
     const float inv = L == 0.f ? 0.f : 1.0f / L;
-    const int node = r / p.Hq;
-    *reinterpret_cast<uint2*>(p.out + (int64_t)(base + node) * p.out_stride + (r - node * p.Hq) * kHD + 4 * lane) =
+    const int node = r >> p.hq_shift;
+    *reinterpret_cast<uint2*>(p.out + (int64_t)(base + node) * p.out_stride + (r & (p.Hq - 1)) * kHD + 4 * lane) =
         make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
 }
 
@@ -1111,6 +1112,7 @@ extern "C" int msgl_tree_attention(const void* q, int64_t q_stride, const void* 
     p.mask = tree_mask, p.words = mask_words;
     p.out = static_cast<uint16_t*>(out), p.out_stride = out_stride;
     p.bs = bs, p.Hq = Hq, p.Hkv = Hkv, p.group = Hq / Hkv, p.max_q = max_seqlen_q;
+    p.hq_shift = __builtin_ctz(Hq), p.hkv_shift = __builtin_ctz(Hkv), p.group_shift = __builtin_ctz(Hq / Hkv);
     TreePlan plan = tree_plan(bs, max_seqlen_q, max_seqlen_k, total_kv, Hq, Hkv);
     p.row_tiles = plan.row_tiles;
     p.scale_log2e = scale * 1.44269504088896340736f;
