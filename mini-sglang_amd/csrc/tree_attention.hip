@@ -21,6 +21,7 @@
 //     (t = table entries).
 // Where requests are few or unequal, their tiles are dealt in equal shares (TreeWalk, tree_plan); runs of a request leave (O, max, sum) in the
 // workspace and a second kernel joins them.
+#include <cmath>
 #include <type_traits>
 #include <utility>
 
@@ -1025,15 +1026,18 @@ struct TreePlan {
 //   1 of 1000 x 4, 16 / 8 heads (8)  15 | 20      1 of 2000 x 4 (8)  20 | 20      7 of 500 to 1000 x 4 (56)  17 | 19
 static TreePlan tree_plan_of(int waves, int rb, int tile_ns, int64_t rows, int bs, int max_k, int64_t tiles, int Hkv) {
     const int64_t units = device_cus(), tile_rows = 32 * (waves ? waves : rb), row_tiles = (rows + tile_rows - 1) / tile_rows;
-    const int64_t across = Hkv * row_tiles, items = bs * across;
+    // an XCD gets every eighth item, with all its row tiles
+    const int64_t xcd_units = units >= 8 ? units / 8 : 1;
+    const double load = (double)((((int64_t)bs * Hkv + 7) / 8) * row_tiles) / xcd_units;
     const int64_t most = ((int64_t)max_k + kTreeKeys - 1) / kTreeKeys, mean = (tiles + bs - 1) / bs, all = tiles + (int64_t)bs * kTreeBegin;
     const int64_t least = waves ? 6 : kLeastTiles, join = waves ? 6 : 28;
-    int64_t shares = across < units ? units / across : 1;
+    int64_t shares = 8 * (xcd_units / row_tiles) / Hkv;
+    if (shares < 1) shares = 1;
     if (shares > (all + least - 1) / least) shares = (all + least - 1) / least;
     const int64_t len = (all + shares - 1) / shares;
     const bool two_fit = waves == 4 || (waves == 0 && rb == 1);
-    const double rounds = two_fit ? (double)items / units : (double)((items + units - 1) / units);
-    const double alone = items <= units ? kTreeBegin + most : (kTreeBegin + mean) * rounds + most - mean, shared = kTreeBegin + len + join;
+    const double alone = load <= 1 ? kTreeBegin + most : (kTreeBegin + mean) * (two_fit ? load : ceil(load)) + most - mean;
+    const double shared = (kTreeBegin + len) * (row_tiles > xcd_units ? (double)row_tiles / xcd_units : 1.0) + join;
     TreePlan t = {waves, rb, (int)row_tiles, bs, 1, alone * tile_ns};
     const int forced = variant(MSGL_VARIANT_TREE_SHARES);
     if (forced < 0 ? shared < alone : forced == 1) {
