@@ -427,7 +427,7 @@ extern "C" int msgl_prepare_extend(const int32_t* req_pool_indices, const int32_
     if (bs == 0) return MSGL_OK;
     MSGL_REQUIRE(max_ctx <= 0x7fffffff - page_size && capacity <= 1 << 30, "msgl_prepare_extend: max_ctx %d + page_size %d or capacity %d leaves 32 bits",
                  max_ctx, page_size, capacity);
-    MSGL_REQUIRE(req_pool_indices && prefix_lens && new_lens && alloc_lens && free_pages && free_range && req_to_token && cu_seqlens_q && seq_lens &&
+    MSGL_REQUIRE(req_pool_indices && prefix_lens && new_lens && alloc_lens && (free_pages || free_capacity == 0) && free_range && req_to_token && cu_seqlens_q && seq_lens &&
                      alloc_out && free_range_out && status && (capacity == 0 || (positions && out_cache_loc)),
                  "msgl_prepare_extend: null pointer argument");
     MSGL_REQUIRE((parents == nullptr) == (tree_mask == nullptr), "msgl_prepare_extend: parents and tree_mask go together");

@@ -294,3 +294,19 @@ def test_every_form_over_long_prefixes(variants, form, nodes, prefix, Hq, Hkv):
     a = _args(c)
     _check(_ops().tree_attention(*a), c)
     _check(_ops().tree_attention(*a, workspace=torch.empty(16, dtype=torch.uint8, device=DEV)), c)
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+def test_prepare_extend_with_an_empty_free_list(in_place):
+    """No page left at all: a step that needs none goes through, one that needs one is refused."""
+    ops = _ops()
+    for new, status in (([3, 0], 0), ([4, 0], 1)):
+        alloc, rng = _i32([8, 5]), _i32([0, 0])
+        r2t = torch.zeros(2, 32, dtype=torch.int32, device=DEV)
+        r2t[0, :8], r2t[1, :5] = torch.arange(8, 16), torch.arange(24, 29)
+        pos, loc, cu, seq, st = _i32([9] * 4), _i32([9] * 4), _i32([9] * 3), _i32([9] * 2), _i32([0])
+        extra = {} if in_place else dict(alloc_out=_i32([0, 0]), free_range_out=_i32([7, 7]))
+        ops.prepare_extend(_i32([0, 1]), _i32([5, 5]), _i32(new), alloc, _i32([]), rng, r2t, pos, loc, cu, seq, st, 8, **extra)
+        assert int(st) == status and cu.tolist() == ([0, 3, 3] if status == 0 else [0, 0, 0])
+        assert loc.tolist() == ([13, 14, 15, 0] if status == 0 else [0] * 4)
+        assert (rng if in_place else extra["free_range_out"]).tolist() == [0, 0]
