@@ -27,7 +27,7 @@ constexpr int kLpCandidates = 256;  // per wave
 // 85, 88, 93, 113, 166 us with one and 88, 89, 91, 95, 103 with both
 constexpr int kTwoBars = 12;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
-constexpr double kLn2d = 0.693147180559945309417;
+constexpr double kPerLog2 = 1.0 / (double)kLog2e;  // not ln 2: undoes exactly what the multiplication by the rounded kLog2e does to the reference
 
 struct SegmentStats {
     double ref;  // natural units: e = exp(x - ref)
@@ -261,7 +261,8 @@ __global__ __launch_bounds__(kLpThreads) void logprob_segment_kernel(LogprobPara
                 t += x * fmaxf(d, -200.f);  // 2^-200 is 0 in 32 bits: -inf and the like add 0, not 0 * inf
             }
     };
-    // (x - ref) log2 e as one multiply-add against a whole number near ref log2 e, itself the reference then; huge values (a mask's lowest value
+    // (x - ref) log2 e as one multiply-add against a whole number near ref log2 e, itself the reference then (as kPerLog2 gives it: the constant's
+    // rounding is then one of x - ref, not of x); huge values (a mask's lowest value
     // in every place) do not survive the multiplication and are subtracted first
     const bool tame = fabsf(ref) < 1e5f;
     const float ref2 = rintf(ref * kLog2e);
@@ -274,7 +275,7 @@ __global__ __launch_bounds__(kLpThreads) void logprob_segment_kernel(LogprobPara
     z = t = 0.f;
 #pragma unroll
     for (int w = 0; w < kLpWaves; ++w) z += lds_f[w][0], t += lds_f[w][1];
-    const double reference = tame ? (double)ref2 * kLn2d : (double)ref;
+    const double reference = tame ? (double)ref2 * kPerLog2 : (double)ref;
     std::conditional_t<WHOLE, RowResult, SegmentStats> result = [&] {
         if constexpr (WHOLE) return RowResult(p, row, BYTES, reference, z, t * kLn2);
         else return SegmentStats{reference, z, t * kLn2};

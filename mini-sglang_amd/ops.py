@@ -848,8 +848,10 @@ def accept_tree(draft_tokens: torch.Tensor, target_tokens: torch.Tensor, parents
             raise ValueError("the caches must live on the same GPU as the others")
         table, count, stride = layers.table.data_ptr(), len(layers.k), layers.slot_stride
         _, Hkv, D = layers.k[0].shape
-    _launch(index, _lib.msgl_accept_tree, draft_tokens.data_ptr(), target_tokens.data_ptr(), parents.data_ptr(), cu_seqlens_q.data_ptr(),
-            prefix_lens.data_ptr(), out_cache_loc.data_ptr(), table, count, stride, Hkv, D, accept_lens.data_ptr(), accept_rows.data_ptr(),
+    cu_at = cu_seqlens_q.data_ptr()
+    nodes = [t.data_ptr() for t in (draft_tokens, target_tokens, parents, out_cache_loc)] if T else [cu_at] * 4  # (no node: none of them is read)
+    _launch(index, _lib.msgl_accept_tree, *nodes[:3], cu_at, prefix_lens.data_ptr(), nodes[3], table, count, stride, Hkv, D,
+            accept_lens.data_ptr(), accept_rows.data_ptr(),
             accept_tokens.data_ptr(), next_tokens.data_ptr(), seq_lens.data_ptr(), bs, accept_rows.shape[1])
 
 

@@ -310,3 +310,26 @@ def test_prepare_extend_with_an_empty_free_list(in_place):
         assert int(st) == status and cu.tolist() == ([0, 3, 3] if status == 0 else [0, 0, 0])
         assert loc.tolist() == ([13, 14, 15, 0] if status == 0 else [0] * 4)
         assert (rng if in_place else extra["free_range_out"]).tolist() == [0, 0]
+
+
+def test_accept_tree_without_any_node():
+    ops = _ops()
+    none, lens, nxt, seq = _i32([]), _i32([9, 9]), _i32([9, 9]), _i32([0, 0])
+    rows, tokens = _i32([[9], [9]]), _i32([[9], [9]])
+    ops.accept_tree(none, none, none, _i32([0, 0, 0]), _i32([5, 7]), none, None, lens, rows, tokens, nxt, seq)
+    assert lens.tolist() == [0, 0] and seq.tolist() == [5, 7] and nxt.tolist() == [9, 9] and rows.tolist() == tokens.tolist() == [[-1], [-1]]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", [700, 4675, 30001])
+def test_token_logprobs_far_from_zero(dtype, vocab):
+    """Log probabilities do not depend on where the logits lie: no rounding may grow with them."""
+    from test_tree_ops_gpu import _logprobs
+
+    g = torch.Generator().manual_seed(vocab)
+    for offset in (418.0, -700.0, 9000.0, -80000.0, 99999.0, 200000.0):
+        x = torch.randn(3, vocab, generator=g) * 3
+        x[1] *= 20
+        x[2, vocab // 2] += 200
+        x = (x + offset).to(dtype)
+        _logprobs(x.to(DEV), [0, vocab - 1, vocab // 2], 11, host=x.float())
