@@ -352,7 +352,8 @@ __device__ __forceinline__ void load_masks(const TreeParams& p, const TreeItem& 
     for (int rb = 0; rb < RB; ++rb) asm volatile("" : "+v"(word[rb]));
 }
 
-// Hides what the rows do not see of the tile that begins at key0.
+// Scales the scores of the tile that begins at key0 (log2 units from here on) and hides what the rows do not see: in this order, so that what is
+// hidden is -inf for a scale of 0 too.
 // s[rb][i]: key 8 (i >> 2) + 4 half + (i & 3) of the tile, row lane & 31 of the block.
 template <int RB>
 __device__ __forceinline__ void tile_mask(const TreeParams& p, const TreeItem& it, int row0, const uint64_t (&word)[RB], int key0, int lane, f32x16_t (&s)[RB]) {
@@ -361,7 +362,7 @@ __device__ __forceinline__ void tile_mask(const TreeParams& p, const TreeItem& i
         const uint32_t bits = row_sees(p, it, row0 + rb * 32 + (lane & 31), word[rb], key0) >> (4 * (lane >> 5));
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-            if (!(bits >> (8 * (i >> 2) + (i & 3)) & 1)) s[rb][i] = -INFINITY;
+            s[rb][i] = bits >> (8 * (i >> 2) + (i & 3)) & 1 ? s[rb][i] * p.scale_log2e : -INFINITY;
     }
 }
 
@@ -656,8 +657,8 @@ __device__ __forceinline__ void narrow_run(const TreeParams& p, const TreeItem& 
             uint64_t word[RB];  // (a wave has one such tile as a rule: asked for at the start, its mask would only make that longer)
             load_masks<RB>(p, it, it.r0, lane, word);
             tile_mask<RB>(p, it, it.r0, word, it.t0 + (wave + j * kTreeWaves) * kTreeKeys, lane, s);
-            tile_reference<RB>(p.scale_log2e, s, st);
-            tile_probabilities<RB>(p.scale_log2e, s, st, pf);
+            tile_reference<RB>(1.f, s, st);
+            tile_probabilities<RB>(1.f, s, st, pf);
             if (tile_values_masked<RB>(wait_values(j), lane, pf, st)) odd |= 1ull << (j - plain);
             if (j + SL < T) issue_rows(j + SL, true);
         }
@@ -894,9 +895,10 @@ __device__ __forceinline__ void wide_run(const TreeParams& p, const TreeItem& it
         refill(j);
         read_keys(tile_at(j), lane, kf);
         tile_scores<1>(kf, qf, s);
-        if (j >= plain) tile_mask<1>(p, it, row0, word, it.t0 + j * kTreeKeys, lane, s);
-        tile_reference<1>(p.scale_log2e, s, st);
-        tile_probabilities<1>(p.scale_log2e, s, st, pf);
+        float scale = p.scale_log2e;
+        if (j >= plain) tile_mask<1>(p, it, row0, word, it.t0 + j * kTreeKeys, lane, s), scale = 1.f;
+        tile_reference<1>(scale, s, st);
+        tile_probabilities<1>(scale, s, st, pf);
         if (j < plain) tile_values<1>(tile_at(j) + kTreeHalf, lane, pf, st);
         else if (tile_values_masked<1>(tile_at(j) + kTreeHalf, lane, pf, st)) odd |= 1ull << (j - plain);
     }

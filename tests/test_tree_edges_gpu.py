@@ -1,0 +1,40 @@
+"""Edges of the speculative-decoding operators."""
+import pytest
+import torch
+
+import tree_cases as tc
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+D = 128
+
+
+def _ops():
+    from mini_sglang_amd import ops
+    return ops
+
+
+def _attend(c, **kw):
+    d = {k: v.to(DEV) if isinstance(v, torch.Tensor) else v for k, v in c.items()}
+    return _ops().tree_attention(d["q"], d["k"], d["v"], d["r2t"], d["rows"], d["cu"], d["prefix"], d["mask"], max(c["nodes"]),
+                                 max(n + p for n, p in zip(c["nodes"], c["prefix_list"])), c["scale"], **kw)
+
+
+FORMS = [(form, shares) for form in (0, 1) for shares in (0, 1)]
+# rows per kv head: up to 32, 64, 128, 256 and beyond; prefixes that end inside a tile, at its end and that are empty
+SHAPES = [([3, 1, 4], [40, 0, 64], 16, 8), ([7, 12, 0], [333, 31, 5], 8, 2), ([25, 6], [500, 96], 8, 2), ([40, 33], [1300, 0], 8, 1)]
+
+
+@pytest.mark.parametrize("form,shares", FORMS)
+@pytest.mark.parametrize("nodes,prefix,Hq,Hkv", SHAPES)
+def test_scale_zero_is_the_mean_of_the_visible_values(variants, form, shares, nodes, prefix, Hq, Hkv):
+    variants("tree_form", form), variants("tree_shares", shares)
+    c = tc.attention_case(nodes, prefix, Hq, Hkv, 16, 3 + sum(nodes))
+    c["scale"] = 0.0
+    c["masks"][1] = 0   # sees its prefix alone
+    if 0 in prefix:
+        c["masks"][sum(nodes[: prefix.index(0)])] = 0   # sees nothing
+    c["mask"] = tc.pack_masks(c["masks"], c["mask"].shape[1])
+    exact, absv, size = tc.attention_oracle(c)
+    err = (_attend(c).cpu().double() - exact).abs()
+    assert bool((err <= tc.attention_tolerance(exact, absv, size)).all())
