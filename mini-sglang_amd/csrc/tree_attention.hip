@@ -40,6 +40,7 @@ constexpr int kTreeMergeRow = kHD + 4;              // floats per row of the exc
 constexpr int merge_bytes(int waves, int rb) { return waves * 32 * rb * (kTreeMergeRow + 2) * 4; }
 constexpr int kTreeBegin = 16;                      // tiles that the start of a run is worth (TreeWalk)
 constexpr int kLeastTiles = 4;                      // least tiles of a share: one per wave of the narrow kernel
+constexpr float kLowestScore = -3.40282347e38f;     // reference maximum before the first score: nothing that 32 bits hold is below it
 constexpr float kRescaleAt = 8.f;                   // log2 units a row's maximum may outgrow its reference before O is rescaled
 
 struct TreeParams {
@@ -259,7 +260,7 @@ struct TreeState {
             for (int mb = 0; mb < 4; ++mb)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[rb][mb][i] = 0.f;
-            m[rb] = kNegBigE, l[rb] = 0.f;
+            m[rb] = kLowestScore, l[rb] = 0.f;
         }
     }
 };
@@ -504,7 +505,7 @@ __device__ __forceinline__ void join_and_store(const TreeParams& p, const TreeIt
         const int g = idx / (R * 32), r = (idx >> 5) % R, d = (idx & 31) * 4;
         const int row = row0(g) + r;
         if (row >= it.rows) continue;
-        float M = kNegBigE;
+        float M = kLowestScore;
 #pragma unroll
         for (int w = 0; w < WPH; ++w) M = fmaxf(M, lds_ml[((g * WPH + w) * R + r) * 2]);
         float L = 0.f;
@@ -934,7 +935,7 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeParams p) {
     const int nsplit = r < n * p.Hq ? p.ws_n[pair] : 0;
     const bool live = nsplit > 1;  // (one run: written by the first kernel)
     const int64_t at = pair * p.splits;
-    float M = kNegBigE, L = 0.f;
+    float M = kLowestScore, L = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     if (live) {
         for (int s0 = g; s0 < nsplit; s0 += 4 * GROUPS) {  // four runs' loads under way at a time
@@ -966,7 +967,7 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeParams p) {
         if (lane == 0) lds[hw][kHD] = M, lds[hw][kHD + 1] = L;
         __syncthreads();
         if (g != 0) return;
-        float top = kNegBigE;
+        float top = kLowestScore;
 #pragma unroll
         for (int k = 0; k < GROUPS; ++k) top = fmaxf(top, lds[hw + k][kHD]);
         L = 0.f;

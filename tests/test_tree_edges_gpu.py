@@ -38,3 +38,25 @@ def test_scale_zero_is_the_mean_of_the_visible_values(variants, form, shares, no
     exact, absv, size = tc.attention_oracle(c)
     err = (_attend(c).cpu().double() - exact).abs()
     assert bool((err <= tc.attention_tolerance(exact, absv, size)).all())
+
+
+@pytest.mark.parametrize("form,shares", FORMS)
+@pytest.mark.parametrize("nodes,prefix,Hq,Hkv", SHAPES)
+def test_scores_far_below_zero_are_ordinary_scores(variants, form, shares, nodes, prefix, Hq, Hkv):
+    """Scores -scale and -2 scale (or with the other sign), exact in 32 bits: the softmax is the mean over the keys with the larger one, whatever
+    the scale."""
+    variants("tree_form", form), variants("tree_shares", shares)
+    c = tc.attention_case(nodes, prefix, Hq, Hkv, 16, 5 + sum(nodes))
+    k = torch.zeros_like(c["k"])
+    k[:, :, 0] = -1.0 - torch.randint(0, 2, k.shape[:2], generator=torch.Generator().manual_seed(1)).to(k.dtype)
+    c["k"] = k
+    for sign in (1.0, -1.0):
+        c["q"] = torch.zeros_like(c["q"])
+        c["q"][:, :, 0] = sign
+        c["scale"] = 64.0                 # e^-64 is nothing beside 1: the limit that every larger scale has
+        exact, absv, _ = tc.attention_oracle(c)
+        tol = tc.attention_tolerance(exact, absv, torch.zeros(exact.shape[:2], dtype=torch.float64)) + absv * 2.0 ** -64
+        for scale in (64.0, 1e20, 1e31, 1e36, 1e38):
+            c["scale"] = scale
+            err = (_attend(c).cpu().double() - exact).abs()
+            assert bool((err <= tol).all()), (sign, scale)
