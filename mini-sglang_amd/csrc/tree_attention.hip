@@ -41,6 +41,7 @@ constexpr int merge_bytes(int waves, int rb) { return waves * 32 * rb * (kTreeMe
 constexpr int kTreeBegin = 16;                      // tiles that the start of a run is worth (TreeWalk)
 constexpr int kLeastTiles = 4;                      // least tiles of a share: one per wave of the narrow kernel
 constexpr float kLowestScore = -3.40282347e38f;     // reference maximum before the first score: nothing that 32 bits hold is below it
+constexpr float kTameScore = 4096.f;                // log2 units up to which half a step of a reference (2^-13) is nothing beside a bf16 probability's
 constexpr float kRescaleAt = 8.f;                   // log2 units a row's maximum may outgrow its reference before O is rescaled
 
 struct TreeParams {
@@ -403,7 +404,9 @@ __device__ __forceinline__ void tile_reference(float scale_log2e, const f32x16_t
     follow_maximum<RB>(scale_log2e, top, st);
 }
 
-// Scores to probabilities relative to the reference, their sum, and the second product's operand.
+// Scores to probabilities relative to the reference, their sum, and the second product's operand.  The scaled score is rounded before the reference is
+// subtracted, as the reference was: the row's largest score then gives a power of two of a whole difference of 32-bit numbers, whatever its size (one
+// multiply-add, with the product not rounded, is off by half a step of the reference: 0.5 at 2^24, beyond all numbers at 2^32).
 template <int RB>
 __device__ __forceinline__ void tile_probabilities(float scale_log2e, f32x16_t (&s)[RB], TreeState<RB>& st, bf16x8_t (&pf)[RB][2]) {
 #pragma unroll
@@ -411,7 +414,7 @@ __device__ __forceinline__ void tile_probabilities(float scale_log2e, f32x16_t (
         float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            s[rb][i] = fast_exp2(__builtin_fmaf(s[rb][i], scale_log2e, -st.m[rb]));
+            s[rb][i] = fast_exp2(s[rb][i] * scale_log2e - st.m[rb]);
             sum += s[rb][i];
         }
         st.l[rb] += sum;
@@ -719,8 +722,11 @@ __device__ __forceinline__ void dma_rows4(uint64_t k, uint64_t v, uint32_t dst) 
                      : "memory", "scc");
 }
 
+// tame: long prefixes go through the steady state below, whose exponentials take one multiply-add each.  Where a row's reference then turns out to lie
+// where tile_probabilities needs its two steps (or where a NaN says that it may have), nothing is stored, the result is false and the run is to be done
+// again without.
 template <int NW, bool NT>
-__device__ __forceinline__ void wide_run(const TreeParams& p, const TreeItem& it, int h, int wave, char* smem) {
+__device__ __forceinline__ bool wide_run(const TreeParams& p, const TreeItem& it, int h, int wave, char* smem, bool tame) {
     using W = TreeWide<NW>;
     const int lane = fresh_lane();
     const int g4 = lane >> 4, q16 = lane & 15;
@@ -781,7 +787,7 @@ __device__ __forceinline__ void wide_run(const TreeParams& p, const TreeItem& it
     int j = 0;
     if (row0 >= it.rows) {  // no rows for this wave: it loads and keeps the barriers
         for (; j < T; ++j) arrive(j), refill(j);
-    } else if (plain > 2) {
+    } else if (tame && plain > 2) {
         // The steady state is one stream of 16 matrix instructions per tile, each a slice with its share of everything else:
         //   slices 0 .. 7     S^T of tile j + 1 (its K fragments are in registers); V^T fragments of tile j are read
         //   slices 8 .. 15    O^T of tile j; tile j + 2 arrives, its K fragments are read
@@ -904,11 +910,14 @@ __device__ __forceinline__ void wide_run(const TreeParams& p, const TreeItem& it
         else if (tile_values_masked<1>(tile_at(j) + kTreeHalf, lane, pf, st)) odd |= 1ull << (j - plain);
     }
     wait_loads<0>();
-    if (!__syncthreads_or(odd != 0)) {
+    const bool wild = tame && plain > 2 && ((fabsf(st.m[0]) > kTameScore && st.m[0] != kLowestScore) || st.l[0] != st.l[0]);
+    if (!__syncthreads_or(odd != 0 || wild)) {
         store_rows(p, it, st, row0, h, lane);
-        return;
+        return true;
     }
+    if (__syncthreads_or(wild)) return false;
     join_and_store<1, 1, NW>(p, it, st, smem, wave, lane, odd, it.t0 + plain * kTreeKeys, kTreeKeys, [&](int g) { return it.r0 + g * 32; }, [&](int) { return h; });
+    return true;
 }
 template <int NW, bool NT>
 __global__ __launch_bounds__(NW * 64, 2) void tree_attention_wide_kernel(TreeParams p) {
@@ -918,8 +927,11 @@ __global__ __launch_bounds__(NW * 64, 2) void tree_attention_wide_kernel(TreePar
     const int r0 = at.row_tile * 32 * NW, h = at.item & (p.Hkv - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     TreeItem it;
-    for (TreeWalk walk(p, at.item >> p.hkv_shift, r0, threadIdx.x & 63, it); walk.any; __syncthreads(), walk.next(p, r0, it))
-        wide_run<NW, NT>(p, it, h, wave, smem);
+    bool tame = true;
+    for (TreeWalk walk(p, at.item >> p.hkv_shift, r0, threadIdx.x & 63, it); walk.any; __syncthreads()) {
+        tame = wide_run<NW, NT>(p, it, h, wave, smem, tame);
+        if (tame) walk.next(p, r0, it);
+    }
 }
 
 // Joins the runs of a (token, head): GROUPS half-waves per row take every GROUPS-th run, four dims per lane, and meet in LDS.

@@ -60,3 +60,21 @@ def test_scores_far_below_zero_are_ordinary_scores(variants, form, shares, nodes
             c["scale"] = scale
             err = (_attend(c).cpu().double() - exact).abs()
             assert bool((err <= tol).all()), (sign, scale)
+
+
+@pytest.mark.parametrize("form,shares", FORMS)
+@pytest.mark.parametrize("nodes,prefix,Hq,Hkv", SHAPES)
+def test_large_scores_leave_the_largest_and_its_ties(variants, form, shares, nodes, prefix, Hq, Hkv):
+    """Whole-number queries and keys, so that products and ties are exact: from a scale of a few hundred on the softmax is the mean over the keys with
+    the largest product, however far the scores lie apart."""
+    variants("tree_form", form), variants("tree_shares", shares)
+    c = tc.attention_case(nodes, prefix, Hq, Hkv, 16, 9 + sum(nodes))
+    g = torch.Generator().manual_seed(2)
+    c["q"], c["k"] = (torch.randint(-2, 3, x.shape, generator=g).to(torch.bfloat16) for x in (c["q"], c["k"]))
+    c["scale"] = 300.0     # e^-300 is nothing beside 1
+    exact, absv, _ = tc.attention_oracle(c)
+    tol = tc.attention_tolerance(exact, absv, torch.zeros(exact.shape[:2], dtype=torch.float64))
+    for scale in (300.0, 1.7e5, 3.3e7, 1e10, 1e20, 1e35):   # (products up to 512: the largest scores are 5e37)
+        c["scale"] = scale
+        err = (_attend(c).cpu().double() - exact).abs()
+        assert bool((err <= tol).all()), scale
