@@ -52,6 +52,9 @@ class TreeDecoder:
         self.accept_rows, self.accept_tokens = torch.zeros((bs, max_nodes), **i32), torch.zeros((bs, max_nodes), **i32)
         self.layers = ops.kv_layers(mr.kv_cache_pool.k_buffer, mr.kv_cache_pool.v_buffer)
         self.seq_lens_cpu = batch.seq_lens_cpu.clone()
+        self.synced_lens = self.seq_lens_cpu.clone()            # the batch's lengths as this decoder last took or left them
+        self.reqs = list(batch.reqs)
+        self.ahead = [len(r.token_ids) - int(n) for r, n in zip(self.reqs, self.seq_lens_cpu)]  # tokens a request has beyond its cached ones
         self.last_logprobs: List[list] = [[] for _ in range(bs)]
         self._scores = None
         self._upload_free_list()
@@ -69,6 +72,20 @@ class TreeDecoder:
         if changed and self.pending:
             raise RuntimeError("the page allocator changed under a running TreeDecoder: call sync_host() before other batches allocate or free")
         return changed
+
+    def _take_lengths(self) -> None:
+        """The batch's lengths, where its requests were decoded by other means since the last sync_host()."""
+        b = self.batch
+        if len(b.reqs) != self.bs or any(r is not mine for r, mine in zip(b.reqs, self.reqs)):
+            raise RuntimeError("the batch's requests changed: a TreeDecoder serves those it was made for")
+        if not torch.equal(b.seq_lens_cpu, self.synced_lens):
+            if self.pending:
+                raise RuntimeError("the batch was decoded by other means under a running TreeDecoder: call sync_host() before")
+            self.prefix_lens.copy_(b.seq_lens)
+            self.alloc_lens.copy_(self.prefix_lens)
+            self.seq_lens_cpu, self.synced_lens = b.seq_lens_cpu.clone(), b.seq_lens_cpu.clone()
+        if any(len(r.token_ids) - n != a for r, n, a in zip(self.reqs, self.seq_lens_cpu.tolist(), self.ahead)):
+            raise RuntimeError("a request's tokens and its cached positions do not go together any more")
 
     def _prepare(self) -> None:
         """Bounds, metadata and (captured) step for contexts up to max_new_tokens longer than now."""
@@ -116,6 +133,7 @@ class TreeDecoder:
         the request's last token).  Empty lists decode one token.  Returns the accepted tokens per request, appended to the requests too."""
         if len(drafts) != self.bs:
             raise ValueError(f"{len(drafts)} drafts for {self.bs} requests")
+        self._take_lengths()
         ids, parents, lens = [], [], []
         for r, (tokens, par) in zip(self.batch.reqs, drafts):
             if len(tokens) != len(par) or len(tokens) >= self.max_nodes:
@@ -159,6 +177,7 @@ class TreeDecoder:
         """Host state in line with the device: lengths, last slots, and the page allocator without the pages the contexts fill, those that
         rejected drafts had taken given back.  Decoding can go on by any other means afterwards, or here."""
         mr, b, ps = self.mr, self.batch, self.mr.page_size
+        self._take_lengths()
         if self._host_pages_changed():
             self._upload_free_list()
         mr.page_allocator.alloc(int(self.free_range[0].item()))  # the same pages, in the same order, leave the host's free list
@@ -174,6 +193,6 @@ class TreeDecoder:
             mr.page_allocator.free(torch.cat(spare))
         self.alloc_lens.copy_(self.prefix_lens)
         self._upload_free_list()
-        b.seq_lens_cpu = self.seq_lens_cpu.clone()
+        b.seq_lens_cpu, self.synced_lens = self.seq_lens_cpu.clone(), self.seq_lens_cpu.clone()
         b.seq_lens = self.prefix_lens.clone()
         b.forward_mode = ForwardMode.DECODE

@@ -1,4 +1,6 @@
-"""Edges of the speculative-decoding operators."""
+"""Edges of the speculative-decoding operators and of the decoder that runs them."""
+import random
+
 import pytest
 import torch
 
@@ -78,3 +80,87 @@ def test_large_scores_leave_the_largest_and_its_ties(variants, form, shares, nod
         c["scale"] = scale
         err = (_attend(c).cpu().double() - exact).abs()
         assert bool((err <= tol).all()), scale
+
+
+def _build(ps, lens, budget=120, use_graph=True):
+    from test_tree_decode_gpu import _build as build
+    return build(ps, lens, budget, use_graph)
+
+
+@pytest.mark.parametrize("ps,use_graph", [(1, True), (16, True), (16, False)])
+def test_tree_steps_go_on_after_plain_decoding(ps, use_graph):
+    """Tree steps, plain decoding, tree steps, chained decoding, tree steps: one greedy stream, and no page lost on the way."""
+    from mini_sglang_amd.runtime import decode_loop
+    from mini_sglang_amd.runtime.device_decode import DeviceDecodeLoop
+    from mini_sglang_amd.runtime.tree_decode import TreeDecoder
+
+    lens, steps = [15, 16, 33, 300], 70
+    mr, batch = _build(ps, lens, use_graph=use_graph)
+    start = [len(r.token_ids) for r in batch.reqs]
+    decode_loop.decode_steps(mr, batch, steps)
+    truth = [r.token_ids[n:] for r, n in zip(batch.reqs, start)]
+
+    mr, batch = _build(ps, lens, use_graph=use_graph)
+    pages = mr.page_allocator.free_count()
+    dec = TreeDecoder(mr, batch, 6, max_new_tokens=16, use_graph=use_graph)
+    rng = random.Random(ps)
+
+    def done():
+        return [len(r.token_ids) - n for r, n in zip(batch.reqs, start)]
+
+    def tree_steps(n):
+        for _ in range(n):
+            drafts = []
+            for t, d in zip(truth, done()):
+                right = rng.randint(0, 3)   # that many of the chain's five tokens are the true ones
+                drafts.append((t[d: d + right] + [rng.randrange(2048) for _ in range(5 - right)], [0, 1, 2, 3, 4]))
+            dec.step(drafts)
+        dec.sync_host()
+
+    def check():
+        for r, n, t, d, length in zip(batch.reqs, start, truth, done(), lens):
+            assert r.token_ids[n:] == t[:d]
+        assert batch.seq_lens_cpu.tolist() == [n + d for n, d in zip(lens, done())]
+        assert mr.page_allocator.free_count() == pages - sum(-(-(n + d) // ps) - -(-n // ps) for n, d in zip(lens, done()))
+
+    tree_steps(3)
+    check()
+    decode_loop.decode_steps(mr, batch, 5)
+    check()
+    tree_steps(3)
+    check()
+    decode_loop.decode_steps(mr, batch, 18)   # beyond what the captured bounds were made for
+    tree_steps(2)
+    check()
+    if use_graph:
+        loop = DeviceDecodeLoop(mr, batch, max_steps=4)
+        loop.run(4)
+        loop.sync_host()
+        tree_steps(1)
+        check()
+    assert max(done()) <= steps
+
+
+def test_decoder_refuses_requests_that_moved_on_without_it():
+    from mini_sglang_amd.runtime import decode_loop
+    from mini_sglang_amd.runtime.tree_decode import TreeDecoder
+
+    mr, batch = _build(64, [10, 70])     # (a page has room for all that follows: the page allocator does not change)
+    dec = TreeDecoder(mr, batch, 4)
+    none = [([], [])] * 2
+    dec.step(none)
+    decode_loop.decode_steps(mr, batch, 1)   # without sync_host
+    with pytest.raises(RuntimeError, match="sync_host"):
+        dec.step(none)
+    mr, batch = _build(64, [10, 70])
+    dec = TreeDecoder(mr, batch, 4)
+    batch.reqs[0].token_ids.append(5)        # a token that no cache row stands behind
+    with pytest.raises(RuntimeError, match="token"):
+        dec.step(none)
+    batch.reqs[0].token_ids.pop()
+    dec.step(none)
+    batch.filter_reqs([1])
+    with pytest.raises(RuntimeError, match="requests"):
+        dec.step(none)
+    with pytest.raises(RuntimeError, match="requests"):
+        dec.sync_host()
