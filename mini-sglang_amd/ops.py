@@ -686,7 +686,8 @@ def _scratch(workspace: Optional[torch.Tensor], need: int, index: int) -> Tuple[
 
 
 def prepare_extend_workspace_bytes(bs: int, capacity: int, max_ctx: int, in_place: bool = True) -> int:
-    """Bytes prepare_extend wants as workspace; in_place: without alloc_out or without free_range_out."""
+    """Bytes prepare_extend wants as workspace; in_place: alloc_out or free_range_out left out, or given as alloc_lens or free_range
+    themselves."""
     return int(_lib.msgl_prepare_extend_workspace_bytes(int(bs), int(capacity), int(max_ctx), int(in_place)))
 
 
@@ -703,7 +704,6 @@ def prepare_extend(req_pool_indices: torch.Tensor, prefix_lens: torch.Tensor, ne
     (int32[1]) becomes non-zero if the step was refused, and nothing but empty outputs is written then."""
     index = _gpu_index(req_pool_indices, "req_pool_indices")
     bs, capacity = req_pool_indices.numel(), out_cache_loc.numel()
-    in_place = alloc_out is None or free_range_out is None
     if alloc_out is None:
         alloc_out = alloc_lens
     if free_range_out is None:
@@ -732,11 +732,13 @@ def prepare_extend(req_pool_indices: torch.Tensor, prefix_lens: torch.Tensor, ne
         page_at, page_stride = req_to_page.data_ptr(), req_to_page.stride(0)
     if bs == 0:
         return
+    alloc_at, alloc_out_at, range_at, range_out_at = alloc_lens.data_ptr(), alloc_out.data_ptr(), free_range.data_ptr(), free_range_out.data_ptr()
+    in_place = alloc_at == alloc_out_at or range_at == range_out_at  # (left out, or given and the same)
     ws, ws_at, ws_bytes = _scratch(workspace, _lib.msgl_prepare_extend_workspace_bytes(bs, capacity, max_ctx, in_place), index)
-    _launch(index, _lib.msgl_prepare_extend, req_pool_indices.data_ptr(), prefix_lens.data_ptr(), new_lens.data_ptr(), alloc_lens.data_ptr(),
-            free_pages.data_ptr(), free_pages.numel(), free_range.data_ptr(), req_to_token.data_ptr(), req_to_token.stride(0), rows, max_ctx,
+    _launch(index, _lib.msgl_prepare_extend, req_pool_indices.data_ptr(), prefix_lens.data_ptr(), new_lens.data_ptr(), alloc_at,
+            free_pages.data_ptr(), free_pages.numel(), range_at, req_to_token.data_ptr(), req_to_token.stride(0), rows, max_ctx,
             page_at, page_stride, parents_at, mask_at, words, positions.data_ptr(), out_cache_loc.data_ptr(), capacity, cu_seqlens_q.data_ptr(),
-            seq_lens.data_ptr(), alloc_out.data_ptr(), free_range_out.data_ptr(), status.data_ptr(), bs, page_size, ws_at, ws_bytes)
+            seq_lens.data_ptr(), alloc_out_at, range_out_at, status.data_ptr(), bs, page_size, ws_at, ws_bytes)
 
 
 def tree_attention_splits(bs: int, max_seqlen_q: int, max_seqlen_k: int, Hq: int, Hkv: int, total_kv: int = 0) -> int:

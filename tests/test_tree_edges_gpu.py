@@ -16,6 +16,10 @@ def _ops():
     return ops
 
 
+def _i32(v):
+    return torch.tensor(v, dtype=torch.int32, device=DEV)
+
+
 def _attend(c, **kw):
     d = {k: v.to(DEV) if isinstance(v, torch.Tensor) else v for k, v in c.items()}
     return _ops().tree_attention(d["q"], d["k"], d["v"], d["r2t"], d["rows"], d["cu"], d["prefix"], d["mask"], max(c["nodes"]),
@@ -164,3 +168,26 @@ def test_decoder_refuses_requests_that_moved_on_without_it():
         dec.step(none)
     with pytest.raises(RuntimeError, match="requests"):
         dec.sync_host()
+
+
+@pytest.mark.parametrize("bs,capacity,tree", [(3, 40, True), (3, 5000, True), (3, 5000, False), (1500, 3000, False)])
+@pytest.mark.parametrize("named", [(True, True), (True, False), (False, True)])
+def test_prepare_extend_in_place_by_name(bs, capacity, tree, named):
+    """alloc_out = alloc_lens and free_range_out = free_range by name are the in-place call, and one of them may be."""
+    ops = _ops()
+    rng = random.Random(bs)
+    prefix = [rng.randint(0, 30) for _ in range(bs)]
+    new = [rng.randint(0, 2) for _ in range(bs)]
+    results = []
+    for by_name in (False, True):
+        alloc, fr = _i32(prefix), _i32([0, 4 * bs])
+        r2t = torch.arange(bs * 64, dtype=torch.int32, device=DEV).view(bs, 64) + 16 * (4 * bs + 1)
+        out = [_i32([9] * capacity), _i32([9] * capacity), _i32([9] * (bs + 1)), _i32([9] * bs), _i32([0])]
+        mask = torch.zeros(capacity, 1, dtype=torch.int64, device=DEV) if tree else None
+        extra = dict(alloc_out=alloc if named[0] else _i32([9] * bs), free_range_out=fr if named[1] else _i32([9, 9])) if by_name else {}
+        ops.prepare_extend(_i32(list(range(bs))), _i32(prefix), _i32(new), alloc, _i32(list(range(1, 4 * bs + 1))), fr, r2t, *out, 16,
+                           parents=_i32([-1] * capacity) if tree else None, tree_mask=mask, **extra)
+        results.append([r2t, *out, *([mask] if tree else []), extra.get("alloc_out", alloc), extra.get("free_range_out", fr)])
+    assert int(results[0][5]) == 0
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
