@@ -428,6 +428,8 @@ int msgl_prepare_decode_paged(const int32_t* req_pool_indices, int32_t* seq_lens
  * length, alloc_lens outside prefix_lens .. max_ctx, a table row outside 0 .. table_rows - 1) or
  * 4 (more tokens than `capacity`, more nodes than the mask has bits); then cu_seqlens_q is all 0,
  * every row is a row behind the last token, and lengths, table and free range stay as they were.
+ * bs = 0 launches nothing and writes nothing: a caller that runs a step of `capacity` rows over an empty batch clears them itself, as
+ * ops.prepare_extend does.
  * req_to_page (NULL = none) gets the page ids of pages taken.  parents and tree_mask: both or
  * neither.  workspace: msgl_prepare_extend_workspace_bytes bytes, 16-byte aligned (0, and NULL, for small steps, and for most that are not
  * in place; in_place: alloc_out is alloc_lens or free_range_out is free_range). */

@@ -730,7 +730,11 @@ def prepare_extend(req_pool_indices: torch.Tensor, prefix_lens: torch.Tensor, ne
         if req_to_page.shape[0] != rows:
             raise ValueError("req_to_page needs a row per row of req_to_token")
         page_at, page_stride = req_to_page.data_ptr(), req_to_page.stride(0)
-    if bs == 0:
+    if bs == 0:  # (no kernel: the entry point has no request to launch for)
+        for t in (positions, out_cache_loc, cu_seqlens_q, *(() if tree_mask is None else (tree_mask,))):
+            t.zero_()
+        if free_range_out is not free_range:
+            free_range_out.copy_(free_range)
         return
     alloc_at, alloc_out_at, range_at, range_out_at = alloc_lens.data_ptr(), alloc_out.data_ptr(), free_range.data_ptr(), free_range_out.data_ptr()
     in_place = alloc_at == alloc_out_at or range_at == range_out_at  # (left out, or given and the same)

@@ -191,3 +191,20 @@ def test_prepare_extend_in_place_by_name(bs, capacity, tree, named):
     assert int(results[0][5]) == 0
     for a, b in zip(*results):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("tree", [True, False])
+def test_prepare_extend_of_an_empty_batch_clears_every_row(tree):
+    """Rows behind the last token are the dummy slot's, also where there is no request at all: a model run over them writes nothing that is somebody's."""
+    ops = _ops()
+    none = _i32([])
+    for apart in (False, True):
+        pos, loc, cu, fr, st = _i32([7] * 9), _i32([7] * 9), _i32([7]), _i32([3, 8]), _i32([0])
+        mask = torch.full((9, 2), 7, dtype=torch.int64, device=DEV) if tree else None
+        fro = _i32([9, 9]) if apart else None
+        r2t = torch.full((2, 32), 5, dtype=torch.int32, device=DEV)
+        ops.prepare_extend(none, none, none, none, _i32([1] * 8), fr, r2t, pos, loc, cu, none, st, 16, parents=_i32([0] * 9) if tree else None,
+                           tree_mask=mask, free_range_out=fro)
+        assert pos.tolist() == loc.tolist() == [0] * 9 and cu.tolist() == [0] and int(st) == 0
+        assert fr.tolist() == [3, 8] and (fro is None or fro.tolist() == [3, 8]) and bool((r2t == 5).all())
+        assert mask is None or not bool(mask.any())
