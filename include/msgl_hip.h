@@ -421,7 +421,7 @@ int msgl_prepare_decode_paged(const int32_t* req_pool_indices, int32_t* seq_lens
  * positions / out_cache_loc / tree_mask have `capacity` rows; rows behind the last token are set
  * to position 0, the dummy slot 0 and an empty mask, so that a captured step of fixed size writes
  * nothing that belongs to a request.  alloc_out may be alloc_lens and free_range_out may be
- * free_range (in place); no other output may be an input.  A table row belongs to one request of the step: a row given
+ * free_range (in place); otherwise no output shares memory with an input or another output (refused).  A table row belongs to one request of the step: a row given
  * twice gets both requests' entries in no set order.
  * All or nothing: *status (left as it is on success, sticky like msgl_prepare_decode's) becomes
  * 1 (free list exhausted), 2 (a request outgrows its table row of max_ctx entries), 3 (a negative

@@ -43,6 +43,34 @@ int variant(int which);
 
 static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// An array argument: `rows` rows of `width` bytes, `stride` bytes apart.
+struct Span {
+    const void* at;
+    uint64_t width, rows = 1, stride = 0;
+    unsigned __int128 start() const { return reinterpret_cast<uintptr_t>(at); }
+    bool empty() const { return at == nullptr || width == 0 || rows == 0; }
+};
+// Whether two of them have a byte in common.  Rows are looked at one by one only where the arrays lie inside one another (columns of one buffer).
+static inline bool spans_meet(Span a, Span b) {
+    if (a.empty() || b.empty()) return false;
+    auto end = [](const Span& s) { return s.start() + (unsigned __int128)(s.rows - 1) * s.stride + s.width; };
+    if (end(a) <= b.start() || end(b) <= a.start()) return false;
+    if (a.rows > b.rows) {
+        const Span t = a;
+        a = b, b = t;
+    }
+    for (uint64_t r = 0; r < a.rows; ++r) {
+        const unsigned __int128 lo = a.start() + (unsigned __int128)r * a.stride, hi = lo + a.width;
+        unsigned __int128 i = 0;  // first row of b that ends behind lo
+        if (lo >= b.start() + b.width) {
+            if (b.stride == 0) continue;
+            i = (lo - b.start() - b.width) / b.stride + 1;
+        }
+        if (i < b.rows && b.start() + i * b.stride < hi) return true;
+    }
+    return false;
+}
+
 // ---- device side -----------------------------------------------------------------
 typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2_t;
 

@@ -436,12 +436,6 @@ extern "C" int msgl_prepare_extend(const int32_t* req_pool_indices, const int32_
     MSGL_REQUIRE(r2t_stride >= max_ctx, "msgl_prepare_extend: r2t_stride %lld < max_ctx %d", (long long)r2t_stride, max_ctx);
     MSGL_REQUIRE(req_to_page == nullptr || r2p_stride >= (max_ctx + page_size - 1) / page_size, "msgl_prepare_extend: r2p_stride %lld < pages of a row",
                  (long long)r2p_stride);
-    const int32_t* const inputs[] = {alloc_lens, free_range, req_pool_indices, prefix_lens, new_lens, free_pages, parents};
-    const int32_t* const results[] = {alloc_out, free_range_out, positions, out_cache_loc, cu_seqlens_q, seq_lens, status};
-    for (int i = 0; i < 7; ++i)
-        for (int j = 0; j < 7; ++j)
-            MSGL_REQUIRE(inputs[i] == nullptr || inputs[i] != results[j] || (i == j && i < 2),
-                         "msgl_prepare_extend: an output overwrites an input (only alloc_out may be alloc_lens, free_range_out free_range)");
     const bool in_place = alloc_out == alloc_lens || free_range_out == free_range;
     const size_t need = msgl_prepare_extend_workspace_bytes(bs, capacity, max_ctx, in_place);
     if (need && (workspace_bytes < need || workspace == nullptr)) {
@@ -449,6 +443,22 @@ extern "C" int msgl_prepare_extend(const int32_t* req_pool_indices, const int32_
         return MSGL_E_WORKSPACE;
     }
     MSGL_REQUIRE(aligned16(workspace), "msgl_prepare_extend: workspace must be 16-byte aligned");
+    // work groups read while others write
+    const uint64_t per_req = 4 * (uint64_t)bs, per_token = 4 * (uint64_t)capacity;
+    const Span inputs[] = {{alloc_lens, per_req}, {free_range, 8}, {req_pool_indices, per_req}, {prefix_lens, per_req}, {new_lens, per_req},
+                           {free_pages, 4 * (uint64_t)free_capacity}, {parents, per_token}};
+    const Span results[] = {{alloc_out, per_req}, {free_range_out, 8}, {positions, per_token}, {out_cache_loc, per_token}, {cu_seqlens_q, per_req + 4},
+                            {seq_lens, per_req}, {status, 4}, {tree_mask, 2 * per_token * (uint64_t)(parents ? mask_words : 0)},
+                            {req_to_token, 4 * (uint64_t)max_ctx, (uint64_t)table_rows, 4 * (uint64_t)r2t_stride},
+                            {page_size > 1 ? req_to_page : nullptr, 4 * (((uint64_t)max_ctx + page_size - 1) / page_size), (uint64_t)table_rows, 4 * (uint64_t)r2p_stride},
+                            {workspace, need}};
+    constexpr int kInputs = sizeof(inputs) / sizeof(Span), kResults = sizeof(results) / sizeof(Span);
+    for (int j = 0; j < kResults; ++j) {
+        for (int i = 0; i < kInputs; ++i)
+            MSGL_REQUIRE((i == j && i < 2 && inputs[i].at == results[j].at) || !spans_meet(inputs[i], results[j]),
+                         "msgl_prepare_extend: an output overwrites an input (only alloc_out may be alloc_lens, free_range_out free_range)");
+        for (int i = 0; i < j; ++i) MSGL_REQUIRE(!spans_meet(results[i], results[j]), "msgl_prepare_extend: an output overwrites another");
+    }
     ExtendPrepParams p;
     p.req_idx = req_pool_indices, p.prefix = prefix_lens, p.new_lens = new_lens, p.alloc = alloc_lens;
     p.free_pages = free_pages, p.free_capacity = free_capacity, p.free_range = free_range;

@@ -1,0 +1,25 @@
+"""What the speculative-decoding operators refuse because memory is shared that must not be: several work groups read while others write.  Every call
+here is refused before any launch."""
+import pytest
+
+from test_tree_ops_cpu import A, PREPARE, PREPARE_OK, _call
+
+I32 = 4
+
+
+@pytest.mark.parametrize("change", [
+    dict(seq=A[1] + I32), dict(cu=A[2] - I32), dict(status=A[2] + I32),           # an output that begins inside an input, or ends in one
+    dict(positions=A[7] + 7 * I32), dict(loc=A[7] - 7 * I32), dict(alloc_out=A[3] + I32), dict(range_out=A[5] - I32), dict(mask=A[4] + 9 * I32),
+    dict(r2t=A[0] - 3 * 64 * I32 - 63 * I32),                                     # the last entry of the table's last row
+    dict(r2p=A[1] - 3 * 8 * I32 - 3 * I32, r2p_stride=8),
+    dict(loc=A[9] + 7 * I32), dict(status=A[11] + 2 * I32), dict(seq=A[3]), dict(positions=A[6] + 64 * I32), dict(mask=A[10] - 7 * 8)])  # two outputs
+def test_prepare_extend_refuses_memory_that_is_shared(change):
+    rc, error = _call("msgl_prepare_extend", PREPARE, PREPARE_OK, change)
+    assert rc < 0 and "overwrites" in error, error
+
+
+def test_prepare_extend_refuses_a_workspace_on_its_arrays():
+    big = dict(req=1 << 30, prefix=2 << 30, new=3 << 30, alloc=4 << 30, alloc_out=4 << 30, seq=5 << 30, cu=6 << 30, bs=2000, ws_bytes=1 << 20)
+    for ws in ((1 << 30) - 16, (5 << 30) + 7984):
+        rc, error = _call("msgl_prepare_extend", PREPARE, PREPARE_OK, dict(big, ws=ws))
+        assert rc < 0 and "overwrites" in error, error

@@ -208,3 +208,34 @@ def test_prepare_extend_of_an_empty_batch_clears_every_row(tree):
         assert pos.tolist() == loc.tolist() == [0] * 9 and cu.tolist() == [0] and int(st) == 0
         assert fr.tolist() == [3, 8] and (fro is None or fro.tolist() == [3, 8]) and bool((r2t == 5).all())
         assert mask is None or not bool(mask.any())
+
+
+@pytest.mark.parametrize("bs", [3, 1500])
+def test_prepare_extend_with_arrays_side_by_side(bs):
+    """Cut out of one buffer, next to one another and in the gaps between the table's rows, arrays share no memory; page_size 1 has one table for both."""
+    ops = _ops()
+    prefix, new = [i % 7 for i in range(bs)], [1 + i % 3 for i in range(bs)]
+    total = sum(new)
+    results = []
+    for side_by_side in (False, True):
+        if side_by_side:
+            flat = torch.full((8 * bs + 2 * total + 200,), 9, dtype=torch.int32, device=DEV)
+            wide = torch.zeros(bs, 16 + 8, dtype=torch.int32, device=DEV)
+            at = [0]
+
+            def make(values):
+                at[0] += len(values)
+                flat[at[0] - len(values): at[0]] = _i32(values)
+                return flat[at[0] - len(values): at[0]]
+
+            table, fr = wide[:, :16], wide[bs - 2, 16:18]
+            fr.copy_(_i32([0, 3 * bs]))
+        else:
+            make, table, fr = _i32, torch.zeros(bs, 16, dtype=torch.int32, device=DEV), _i32([0, 3 * bs])
+        args = [make(list(range(bs))), make(prefix), make(new), make(prefix), _i32(list(range(1, 3 * bs + 1))), fr, table]
+        out = [make([9] * total), make([9] * total), make([9] * (bs + 1)), make([9] * bs), make([0])]
+        ops.prepare_extend(*args, *out, 1, req_to_page=table)
+        results.append([args[3], args[5], table, *out])
+    assert int(results[0][-1]) == 0
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
