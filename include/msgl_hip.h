@@ -473,7 +473,8 @@ int msgl_tree_attention(const void* q, int64_t q_stride, const void* k_cache, co
  *   accept_rows[b, i] = row (in the packed arrays) of the i-th node, accept_tokens[b, i] = target_tokens of that row, i.e. the
  *   i-th token generated; -1 behind the path ([bs, max_accept] both, dense);
  *   next_tokens[b] = the last of these (the next step's root; left as it is for a request without nodes);
- *   seq_lens[b] = prefix_lens[b] + accept_lens[b]  (seq_lens may be prefix_lens; no other output may be an input);
+ *   seq_lens[b] = prefix_lens[b] + accept_lens[b]  (seq_lens may be prefix_lens; otherwise no output shares memory with an input or another
+ *   output: refused, but for the nodes' arrays only as far as their beginnings go, their length being known on the device);
  *   and in every layer the K and V rows of the i-th node move to the slot of position prefix_lens[b] + i, which is
  *   out_cache_loc[cu_seqlens_q[b] + i].
  * kv_layers: device array [num_layers][2] of the K and V cache addresses ([slots, Hkv, D] bf16, slot stride cache_stride

@@ -491,12 +491,19 @@ extern "C" int msgl_accept_tree(const int32_t* draft_tokens, const int32_t* targ
     MSGL_REQUIRE(draft_tokens && target_tokens && parents && cu_seqlens_q && prefix_lens && out_cache_loc && accept_lens && accept_rows && accept_tokens &&
                      next_tokens && seq_lens && (num_layers == 0 || kv_layers),
                  "msgl_accept_tree: null pointer argument");
-    // a request may be read by several work groups while one writes its results: no result may lie on an input
-    for (const int32_t* in : {draft_tokens, target_tokens, parents, cu_seqlens_q, out_cache_loc})
-        for (const int32_t* result : {accept_lens, accept_rows, accept_tokens, next_tokens, seq_lens})
-            MSGL_REQUIRE(in != result, "msgl_accept_tree: an output overwrites an input (only seq_lens may be prefix_lens)");
-    MSGL_REQUIRE(accept_lens != prefix_lens && next_tokens != prefix_lens && accept_rows != prefix_lens && accept_tokens != prefix_lens,
-                 "msgl_accept_tree: an output overwrites an input (only seq_lens may be prefix_lens)");
+    // a request may be read by several work groups while one writes its results: no result may lie on an input (how long the nodes' arrays are is
+    // known on the device only: of these the beginnings are looked at here)
+    const uint64_t per_req = 4 * (uint64_t)bs;
+    const Span inputs[] = {{prefix_lens, per_req}, {cu_seqlens_q, per_req + 4}, {draft_tokens, 4}, {target_tokens, 4}, {parents, 4}, {out_cache_loc, 4},
+                           {kv_layers, 16 * (uint64_t)num_layers}};
+    const Span results[] = {{seq_lens, per_req}, {accept_lens, per_req}, {accept_rows, per_req * (uint64_t)max_accept}, {accept_tokens, per_req * (uint64_t)max_accept},
+                            {next_tokens, per_req}};
+    for (const Span& result : results) {
+        for (const Span& in : inputs)
+            MSGL_REQUIRE((result.at == seq_lens && in.at == prefix_lens && seq_lens == prefix_lens) || !spans_meet(in, result),
+                         "msgl_accept_tree: an output overwrites an input (only seq_lens may be prefix_lens)");
+        for (const Span* other = results; other != &result; ++other) MSGL_REQUIRE(!spans_meet(*other, result), "msgl_accept_tree: an output overwrites another");
+    }
     MSGL_REQUIRE(num_layers == 0 || (Hkv > 0 && D > 0 && (int64_t)Hkv * D % 8 == 0 && cache_stride >= (int64_t)Hkv * D && cache_stride % 8 == 0),
                  "msgl_accept_tree: Hkv=%d D=%d cache_stride=%lld (rows must be whole 16-byte pieces)", Hkv, D, (long long)cache_stride);
     AcceptParams p;

@@ -856,9 +856,15 @@ def accept_tree(draft_tokens: torch.Tensor, target_tokens: torch.Tensor, parents
         _, Hkv, D = layers.k[0].shape
     cu_at = cu_seqlens_q.data_ptr()
     nodes = [t.data_ptr() for t in (draft_tokens, target_tokens, parents, out_cache_loc)] if T else [cu_at] * 4  # (no node: none of them is read)
-    _launch(index, _lib.msgl_accept_tree, *nodes[:3], cu_at, prefix_lens.data_ptr(), nodes[3], table, count, stride, Hkv, D,
-            accept_lens.data_ptr(), accept_rows.data_ptr(),
-            accept_tokens.data_ptr(), next_tokens.data_ptr(), seq_lens.data_ptr(), bs, accept_rows.shape[1])
+    most = accept_rows.shape[1]
+    lens_at, rows_at, tokens_at, next_at, seq_at = (t.data_ptr() for t in (accept_lens, accept_rows, accept_tokens, next_tokens, seq_lens))
+    small, large, length = 4 * bs, 4 * bs * most, 4 * T
+    for at in nodes:  # (the entry point sees where these begin; how long they are is known here)
+        if lens_at - length < at < lens_at + small or next_at - length < at < next_at + small or seq_at - length < at < seq_at + small \
+                or rows_at - length < at < rows_at + large or tokens_at - length < at < tokens_at + large:
+            raise ValueError("an output overwrites an input (only seq_lens may be prefix_lens)")
+    _launch(index, _lib.msgl_accept_tree, *nodes[:3], cu_at, prefix_lens.data_ptr(), nodes[3], table, count, stride, Hkv, D, lens_at, rows_at, tokens_at,
+            next_at, seq_at, bs, most)
 
 
 def token_logprobs_workspace_bytes(rows: int, vocab: int, dtype: torch.dtype, top_k: int = 0) -> int:

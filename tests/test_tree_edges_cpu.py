@@ -2,7 +2,7 @@
 here is refused before any launch."""
 import pytest
 
-from test_tree_ops_cpu import A, PREPARE, PREPARE_OK, _call
+from test_tree_ops_cpu import A, ACCEPT, ACCEPT_OK, PREPARE, PREPARE_OK, _call
 
 I32 = 4
 
@@ -23,3 +23,11 @@ def test_prepare_extend_refuses_a_workspace_on_its_arrays():
     for ws in ((1 << 30) - 16, (5 << 30) + 7984):
         rc, error = _call("msgl_prepare_extend", PREPARE, PREPARE_OK, dict(big, ws=ws))
         assert rc < 0 and "overwrites" in error, error
+
+
+@pytest.mark.parametrize("change", [
+    dict(lens=A[3] + 2 * I32), dict(next=A[4] - I32), dict(seq=A[4] + I32), dict(rows=A[5] - 15 * I32), dict(tokens=A[6] - 8 * I32), dict(rows=A[6] + 7 * I32),
+    dict(lens=A[8] + 15 * I32), dict(next=A[9] + 3 * I32), dict(seq=A[10] - I32)])
+def test_accept_tree_refuses_memory_that_is_shared(change):
+    rc, error = _call("msgl_accept_tree", ACCEPT, ACCEPT_OK, change)
+    assert rc < 0 and "overwrites" in error, error

@@ -239,3 +239,20 @@ def test_prepare_extend_with_arrays_side_by_side(bs):
     assert int(results[0][-1]) == 0
     for a, b in zip(*results):
         assert torch.equal(a, b)
+
+
+def test_accept_tree_refuses_outputs_among_its_nodes():
+    ops = _ops()
+    flat = _i32([0] * 40)
+    good = dict(draft=flat[:6], target=flat[6: 12], parents=flat[12: 18], cu=_i32([0, 3, 6]), prefix=_i32([1, 2]), loc=flat[18: 24], lens=flat[24: 26],
+                rows=flat[26: 30].view(2, 2), tokens=flat[30: 34].view(2, 2), next=flat[34: 36], seq=flat[36: 38])
+
+    def call(**change):
+        a = dict(good, **change)
+        ops.accept_tree(a["draft"], a["target"], a["parents"], a["cu"], a["prefix"], a["loc"], None, a["lens"], a["rows"], a["tokens"], a["next"], a["seq"])
+
+    call()   # side by side is apart
+    for change in (dict(lens=flat[4: 6]), dict(next=flat[5: 7]), dict(seq=flat[10: 12]), dict(rows=flat[20: 24].view(2, 2)), dict(tokens=flat[15: 19].view(2, 2)),
+                   dict(loc=flat[23: 29])):
+        with pytest.raises(Exception, match="overwrites"):
+            call(**change)
