@@ -456,7 +456,8 @@ int msgl_prepare_extend(const int32_t* req_pool_indices, const int32_t* prefix_l
  * workspace: msgl_tree_attention_workspace_bytes(total_tokens, Hq, D, splits) bytes, 16-byte aligned, for
  * splits = msgl_tree_attention_splits(...) of the same bounds, the most runs that a request's keys are cut into (1: every request is one work
  * group's, and no workspace is needed); a smaller one (NULL) is legal, requests are then cut less.  Different cuts agree to fp32 rounding of the sums; one cut always gives the same bits.
- * Supported: D == 128; Hq/Hkv in {1, 2, 4, 8}; Hkv in {1, 2, 4, 8}; 0 <= scale <= 1e38; max_seqlen_k <= 2^30; out apart from q.
+ * Supported: D == 128; Hq/Hkv in {1, 2, 4, 8}; Hkv in {1, 2, 4, 8}; 0 <= scale <= 1e38; max_seqlen_k <= 2^30; out and
+ * workspace share no memory with q, the lengths, the mask or each other (refused).
  * Scores are fp32 in units of ln 2: beyond its range they are infinite (a row with +inf among the scores it sees is NaN, one with nothing above -inf zeros). */
 int msgl_tree_attention_splits(int bs, int max_seqlen_q, int max_seqlen_k, int64_t total_kv, int Hq, int Hkv);
 size_t msgl_tree_attention_workspace_bytes(int64_t total_tokens, int Hq, int D, int splits);

@@ -47,26 +47,29 @@ static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t
 struct Span {
     const void* at;
     uint64_t width, rows = 1, stride = 0;
-    unsigned __int128 start() const { return reinterpret_cast<uintptr_t>(at); }
+    __int128 start() const { return (__int128)reinterpret_cast<uintptr_t>(at); }
+    __int128 end() const { return start() + (__int128)(rows - 1) * stride + width; }
     bool empty() const { return at == nullptr || width == 0 || rows == 0; }
 };
-// Whether two of them have a byte in common.  Rows are looked at one by one only where the arrays lie inside one another (columns of one buffer).
+// Whether two of them have a byte in common.  Rows are looked at one by one only where the arrays lie inside one another with strides of their own.
 static inline bool spans_meet(Span a, Span b) {
-    if (a.empty() || b.empty()) return false;
-    auto end = [](const Span& s) { return s.start() + (unsigned __int128)(s.rows - 1) * s.stride + s.width; };
-    if (end(a) <= b.start() || end(b) <= a.start()) return false;
+    if (a.empty() || b.empty() || a.end() <= b.start() || b.end() <= a.start()) return false;
     if (a.rows > b.rows) {
         const Span t = a;
         a = b, b = t;
     }
+    // the first of b's rows least .. that ends behind lo, if it begins before hi
+    auto some_row = [&b](__int128 lo, __int128 hi, __int128 least) {
+        const __int128 gap = lo - b.start() - (__int128)b.width;
+        if (b.stride == 0) return gap < 0 && b.start() < hi;
+        __int128 i = gap < 0 ? -((-gap + b.stride - 1) / b.stride) + 1 : gap / b.stride + 1;
+        if (i < least) i = least;
+        return i < (__int128)b.rows && b.start() + i * b.stride < hi;
+    };
+    if (a.stride == b.stride) return some_row(a.start(), a.start() + a.width, 1 - (__int128)a.rows);  // only the difference of the rows' numbers counts
     for (uint64_t r = 0; r < a.rows; ++r) {
-        const unsigned __int128 lo = a.start() + (unsigned __int128)r * a.stride, hi = lo + a.width;
-        unsigned __int128 i = 0;  // first row of b that ends behind lo
-        if (lo >= b.start() + b.width) {
-            if (b.stride == 0) continue;
-            i = (lo - b.start() - b.width) / b.stride + 1;
-        }
-        if (i < b.rows && b.start() + i * b.stride < hi) return true;
+        const __int128 lo = a.start() + (__int128)r * a.stride;
+        if (some_row(lo, lo + a.width, 0)) return true;
     }
     return false;
 }

@@ -1147,6 +1147,12 @@ extern "C" int msgl_tree_attention(const void* q, int64_t q_stride, const void* 
     p.ws_ml = p.ws_o + (splits > 1 ? (size_t)total_tokens * Hq * splits * kHD : 0);
     p.ws_n = reinterpret_cast<int32_t*>(p.ws_ml + (splits > 1 ? (size_t)total_tokens * Hq * splits * 2 : 0));
     MSGL_REQUIRE(splits == 1 || aligned16(workspace), "msgl_tree_attention: workspace must be 16-byte aligned");
+    const uint64_t tokens = (uint64_t)total_tokens, row = 2 * (uint64_t)Hq * D;  // work groups read while others write
+    const Span inputs[] = {{q, row, tokens, 2 * (uint64_t)q_stride}, {req_pool_indices, 4 * (uint64_t)bs}, {cu_seqlens_q, 4 * (uint64_t)bs + 4},
+                           {prefix_lens, 4 * (uint64_t)bs}, {tree_mask, 8 * tokens * (uint64_t)mask_words}};
+    const Span result = {out, row, tokens, 2 * (uint64_t)out_stride}, runs = {workspace, splits > 1 ? msgl_tree_attention_workspace_bytes(total_tokens, Hq, D, splits) : 0};
+    for (const Span& in : inputs) MSGL_REQUIRE(!spans_meet(in, result) && !spans_meet(in, runs), "msgl_tree_attention: an output or the workspace overwrites an input");
+    MSGL_REQUIRE(!spans_meet(result, runs), "msgl_tree_attention: the workspace overwrites out");
     const int64_t items = (int64_t)plan.shares * Hkv;
     const int64_t blocks = (items + 7) / 8 * 8 * p.row_tiles;
     MSGL_REQUIRE(blocks <= 0x7fffff, "msgl_tree_attention: %lld work groups", (long long)blocks);

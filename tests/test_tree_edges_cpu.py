@@ -2,7 +2,7 @@
 here is refused before any launch."""
 import pytest
 
-from test_tree_ops_cpu import A, ACCEPT, ACCEPT_OK, PREPARE, PREPARE_OK, _call
+from test_tree_ops_cpu import A, ACCEPT, ACCEPT_OK, ATTEND, ATTEND_OK, PREPARE, PREPARE_OK, _call
 
 I32 = 4
 
@@ -30,4 +30,15 @@ def test_prepare_extend_refuses_a_workspace_on_its_arrays():
     dict(lens=A[8] + 15 * I32), dict(next=A[9] + 3 * I32), dict(seq=A[10] - I32)])
 def test_accept_tree_refuses_memory_that_is_shared(change):
     rc, error = _call("msgl_accept_tree", ACCEPT, ACCEPT_OK, change)
+    assert rc < 0 and "overwrites" in error, error
+
+
+# (8 rows of 8 heads x 128: q and out are 16 KiB each, rows of 2 KiB)
+@pytest.mark.parametrize("change", [
+    dict(out=A[0] + 2048), dict(out=A[0] - 16), dict(out=A[0] + 8 * 2048 - 16), dict(q_stride=4096, out=A[0] + 2 * 4096 + 2032, out_stride=4096),
+    dict(q_stride=0, out=A[0] + 2032), dict(out=A[0] - 2048 * 5 + 16, out_stride=2048, q_stride=1024),
+    dict(cu=A[8] - 8), dict(prefix=A[8] + 8 * 2048 - 4), dict(req=A[8] + 48), dict(mask=A[8] - 7 * 8), dict(ws=A[8] + 1024, ws_bytes=1 << 20, max_k=1 << 20),
+    dict(ws=A[0] - 4096, ws_bytes=1 << 20, max_k=1 << 20)])
+def test_tree_attention_refuses_memory_that_is_shared(change):
+    rc, error = _call("msgl_tree_attention", ATTEND, ATTEND_OK, change)
     assert rc < 0 and "overwrites" in error, error

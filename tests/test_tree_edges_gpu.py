@@ -256,3 +256,23 @@ def test_accept_tree_refuses_outputs_among_its_nodes():
                    dict(loc=flat[23: 29])):
         with pytest.raises(Exception, match="overwrites"):
             call(**change)
+
+
+def test_tree_attention_with_queries_and_outputs_in_one_buffer():
+    """Columns of one wide buffer and rows taken in turn are apart, whatever their strides; the query's own place is not."""
+    c = tc.attention_case([5, 12, 1], [60, 9, 100], 8, 2, 16, 12)
+    exact, absv, size = tc.attention_oracle(c)
+    tol = tc.attention_tolerance(exact, absv, size)
+    for make in (lambda n: torch.zeros(n, 20 * D, dtype=torch.bfloat16, device=DEV).split([2 * D, 8 * D, 2 * D, 8 * D], 1)[1::2],
+                 lambda n: torch.zeros(n, 2, 8 * D, dtype=torch.bfloat16, device=DEV).unbind(1),
+                 lambda n: torch.zeros(2, n, 8 * D, dtype=torch.bfloat16, device=DEV).unbind(0)):
+        q, out = (x.unflatten(1, (8, D)) for x in make(18))
+        q.copy_(c["q"])
+        d = dict(c, q=q)
+        assert _attend(d, out=out) is out
+        assert bool(((out.cpu().double() - exact).abs() <= tol).all())
+        with pytest.raises(Exception, match="overwrites"):
+            _attend(d, out=q)
+    flat = torch.zeros(20 * 8 * D, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(Exception, match="overwrites"):   # half a head further on
+        _attend(dict(c, q=flat[: 18 * 8 * D].view(18, 8, D)), out=flat[64: 64 + 18 * 8 * D].view(18, 8, D))
