@@ -494,7 +494,7 @@ int msgl_accept_tree(const int32_t* draft_tokens, const int32_t* target_tokens, 
  * Next to the sampled token's choice (mini_sglang/layers/sampler.py:13-23) this is what a caller that reports log
  * probabilities needs; sums in fp32, one read of the logits.
  * 0 <= top <= min(vocab, MSGL_LOGPROBS_MAX_TOP), vocab <= 2^30, rows * ceil(vocab / 4096) < 2^24.  workspace: msgl_token_logprobs_workspace_bytes bytes, 16-byte
- * aligned. */
+ * aligned.  Outputs and workspace share no memory with the inputs or each other (refused). */
 #define MSGL_LOGPROBS_MAX_TOP 32
 size_t msgl_token_logprobs_workspace_bytes(int rows, int vocab, int elem_bytes, int top);
 int msgl_token_logprobs(const void* logits, int64_t row_stride, int elem_bytes, const int32_t* token_ids, float* logprobs,

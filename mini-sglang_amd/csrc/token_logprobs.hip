@@ -472,6 +472,13 @@ extern "C" int msgl_token_logprobs(const void* logits, int64_t row_stride, int e
         return MSGL_E_WORKSPACE;
     }
     MSGL_REQUIRE(aligned16(workspace), "msgl_token_logprobs: workspace must be 16-byte aligned");
+    const uint64_t per_row = 4 * (uint64_t)rows, per_top = per_row * (uint64_t)top;  // work groups read while others write
+    const Span inputs[] = {{logits, (uint64_t)vocab * elem_bytes, (uint64_t)rows, (uint64_t)row_stride * elem_bytes}, {token_ids, per_row}};
+    const Span results[] = {{logprobs, per_row}, {entropy, per_row}, {top_ids, per_top}, {top_logprobs, per_top}, {workspace, need}};
+    for (const Span& result : results) {
+        for (const Span& in : inputs) MSGL_REQUIRE(!spans_meet(in, result), "msgl_token_logprobs: an output or the workspace overwrites an input");
+        for (const Span* other = results; other != &result; ++other) MSGL_REQUIRE(!spans_meet(*other, result), "msgl_token_logprobs: an output overwrites another");
+    }
     p.logits = static_cast<const char*>(logits), p.row_bytes = row_stride * elem_bytes, p.tokens = token_ids;
     p.logprobs = logprobs, p.entropy = entropy, p.top_ids = top_ids, p.top_logprobs = top_logprobs;
     p.stats = static_cast<SegmentStats*>(workspace);

@@ -2,7 +2,8 @@
 here is refused before any launch."""
 import pytest
 
-from test_tree_ops_cpu import A, ACCEPT, ACCEPT_OK, ATTEND, ATTEND_OK, PREPARE, PREPARE_OK, _call
+from test_tree_ops_cpu import (A, ACCEPT, ACCEPT_OK, ATTEND, ATTEND_OK, LOGPROBS, LOGPROBS_OK, PREPARE, PREPARE_OK,
+                               _call)
 
 I32 = 4
 
@@ -41,4 +42,13 @@ def test_accept_tree_refuses_memory_that_is_shared(change):
     dict(ws=A[0] - 4096, ws_bytes=1 << 20, max_k=1 << 20)])
 def test_tree_attention_refuses_memory_that_is_shared(change):
     rc, error = _call("msgl_tree_attention", ATTEND, ATTEND_OK, change)
+    assert rc < 0 and "overwrites" in error, error
+
+
+@pytest.mark.parametrize("change", [
+    dict(logprobs=(1 << 30) + 2 * 200 + 196), dict(entropy=(1 << 30) + 402), dict(top_lp=A[1] + 8), dict(top_ids=A[1] - 4 * 12 + 4), dict(entropy=A[2] + 8),
+    dict(top_lp=A[4]), dict(ws=(1 << 30) - 16, vocab=20000, stride=20000)])
+def test_token_logprobs_refuses_memory_that_is_shared(change):
+    ok = dict(LOGPROBS_OK, logits=1 << 30, stride=200, vocab=100)
+    rc, error = _call("msgl_token_logprobs", LOGPROBS, ok, change)
     assert rc < 0 and "overwrites" in error, error
