@@ -1,7 +1,9 @@
-"""What the speculative-decoding operators refuse because memory is shared that must not be: several work groups read while others write.  Every call
-here is refused before any launch."""
+"""What the speculative-decoding operators refuse because memory is shared that must not be: several work groups read while others write (every call
+here is refused before any launch); and what the GPU tests' inputs of growing scores ask of a kernel."""
 import pytest
 
+import tree_cases as tc
+import tree_growth_cases as growth
 from test_tree_ops_cpu import (A, ACCEPT, ACCEPT_OK, ATTEND, ATTEND_OK, LOGPROBS, LOGPROBS_OK, PREPARE, PREPARE_OK,
                                _call)
 
@@ -52,3 +54,20 @@ def test_token_logprobs_refuses_memory_that_is_shared(change):
     ok = dict(LOGPROBS_OK, logits=1 << 30, stride=200, vocab=100)
     rc, error = _call("msgl_token_logprobs", LOGPROBS, ok, change)
     assert rc < 0 and "overwrites" in error, error
+
+
+@pytest.mark.parametrize("shape", growth.SHAPES)
+@pytest.mark.parametrize("waves", [1, 4])
+def test_growing_scores_ask_for_every_rescale(shape, waves):
+    """The inputs of the GPU test of growing scores: rows are rescaled again and again, and a kernel that left one kind of rescale out would be wrong by
+    many times the test's tolerance in a tenth of its rows or more."""
+    c = growth.growing_case(*shape, 5)
+    exact, absv, size = tc.attention_oracle(c)
+    tol = tc.attention_tolerance(exact, absv, size)
+    got, count = growth.online_softmax(c, waves)
+    assert bool(((got - exact).abs() <= 1e-9 * (1 + absv)).all())
+    assert 2 * count > sum(shape[0]) * shape[2]   # one for every other (node, head) pair: a quarter of them look along rising levels, several steps each
+    for left_out in ("o", "l") if waves == 1 else ("o", "l", "join"):
+        wrong, _ = growth.online_softmax(c, waves, skip=(left_out,))
+        rows = ((wrong - exact).abs() > 10 * tol).any(-1)
+        assert float(rows.double().mean()) > 0.1, left_out

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import tree_cases as tc
+import tree_growth_cases as growth
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -84,6 +85,23 @@ def test_large_scores_leave_the_largest_and_its_ties(variants, form, shares, nod
         c["scale"] = scale
         err = (_attend(c).cpu().double() - exact).abs()
         assert bool((err <= tol).all()), scale
+
+
+@pytest.mark.parametrize("form,shares", FORMS)
+@pytest.mark.parametrize("shape", growth.SHAPES)
+def test_scores_that_grow_along_the_context(variants, form, shares, shape):
+    """Maxima that rise by 10 to 40 log2 units several times, fall and peak, at other places for every direction a query looks in: every rescale of a
+    state, and factors of the joins between waves and runs from 1 to nothing."""
+    variants("tree_form", form), variants("tree_shares", shares)
+    for seed in (5, 6):
+        c = growth.growing_case(*shape, seed)
+        exact, absv, size = tc.attention_oracle(c)
+        tol = tc.attention_tolerance(exact, absv, size)
+        err = (_attend(c).cpu().double() - exact).abs()
+        assert bool((err <= tol).all()), seed
+        ws = torch.empty(_ops().tree_attention_workspace_bytes(sum(shape[0]), shape[2], D, 3), dtype=torch.uint8, device=DEV)
+        err = (_attend(c, workspace=ws).cpu().double() - exact).abs()   # room for three runs per request
+        assert bool((err <= tol).all()), seed
 
 
 def _build(ps, lens, budget=120, use_graph=True):
