@@ -6,8 +6,8 @@
 // All nodes of a request read the same keys, so they are rows of one matrix product: the (node, head of the GQA group) pairs of a kv
 // head, packed node after node, 32 to a block.  S^T = K.Q^T and O^T += V^T.P^T on v_mfma_f32_32x32x16_bf16: the row sits on the lane in
 // both products (lane & 31), so maximum, sum and rescaling are in-lane plus one swap of lane halves, and the exponentiated scores,
-// packed to bf16, are the second product's operand as they stand.  (P is rounded to bf16 as that product's operand type asks: half a
-// step, 2^-8 relative at most, per probability, unbiased, and the sum is taken of the unrounded ones.)
+// packed to bf16, are the second product's operand as they stand.  (That product's operand type rounds P: half a step, 2^-8 relative at most, per
+// probability, unbiased, where one part holds it, 2^-16 where two do, see probability_parts; the sum is taken of the unrounded ones.)
 //
 // The narrow kernel, for up to 64 rows per kv head and for tiles of 32 rows of small launches: the pass over K and V bounds it (a 32-key tile
 // costs a wave 512 matrix cycles per 32 rows where HBM takes 1250 cycles of the compute unit).  The work group's four waves take every fourth 32-key
@@ -35,6 +35,11 @@ constexpr int kTreeKeys = 32;                       // keys per tile
 constexpr int kTreeHalf = kTreeKeys * kHD * 2;      // bytes of a K or V tile
 constexpr int tile_slots(int rb) { return rb == 1 ? 1 : 2; }                 // narrow kernel: tiles of K, and of V, a wave has room for
 constexpr int tree_ring(int rb) { return 2 * tile_slots(rb) * kTreeHalf; }  // and their bytes
+// bf16 parts that a probability is held in (tile_probabilities): two where up to 32 rows per kv head wait for memory anyway (64 requests of 4096 to 8192
+// tokens x 4 to 8 nodes 274 us either way), as the decode kernel that such a step stands in for holds them in 32 bits; one, as in extend, where the second
+// costs time: two blocks of rows (16 of 2000 to 4000 x 8 to 16 nodes, 47.2 us, would take 51.1), row tiles (1 of 1000 x 60, 14.6, would take 15.6) and
+// the wide kernel, which is bound by such products.
+constexpr int probability_parts(int rb, bool only_row_tile) { return rb == 1 && only_row_tile ? 2 : 1; }
 constexpr int kTreeSlotRing = 4 * 256;              // per wave: table entries of four tiles (64 words each)
 constexpr int kTreeMergeRow = kHD + 4;              // floats per row of the exchange at the end (spread over the banks)
 constexpr int merge_bytes(int waves, int rb) { return waves * 32 * rb * (kTreeMergeRow + 2) * 4; }
@@ -407,8 +412,9 @@ __device__ __forceinline__ void tile_reference(float scale_log2e, const f32x16_t
 // Scores to probabilities relative to the reference, their sum, and the second product's operand.  The scaled score is rounded before the reference is
 // subtracted, as the reference was: the row's largest score then gives a power of two of a whole difference of 32-bit numbers, whatever its size (one
 // multiply-add, with the product not rounded, is off by half a step of the reference: 0.5 at 2^24, beyond all numbers at 2^32).
-template <int RB>
-__device__ __forceinline__ void tile_probabilities(float scale_log2e, f32x16_t (&s)[RB], TreeState<RB>& st, bf16x8_t (&pf)[RB][2]) {
+// PARTS: the operand is bf16, so a probability is held in one part (2^-8 off at most) or in two, the second what the first left out (2^-16).
+template <int PARTS, int RB>
+__device__ __forceinline__ void tile_probabilities(float scale_log2e, f32x16_t (&s)[RB], TreeState<RB>& st, bf16x8_t (&pf)[PARTS][RB][2]) {
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
         float sum = 0.f;
@@ -419,28 +425,38 @@ __device__ __forceinline__ void tile_probabilities(float scale_log2e, f32x16_t (
         }
         st.l[rb] += sum;
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
-            pf[rb][ks] = as_bf16x8(make_uint4(pack_bf16(s[rb][8 * ks], s[rb][8 * ks + 1]), pack_bf16(s[rb][8 * ks + 2], s[rb][8 * ks + 3]),
-                                              pack_bf16(s[rb][8 * ks + 4], s[rb][8 * ks + 5]), pack_bf16(s[rb][8 * ks + 6], s[rb][8 * ks + 7])));
+        for (int ks = 0; ks < 2; ++ks) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = pack_bf16(s[rb][8 * ks + 2 * i], s[rb][8 * ks + 2 * i + 1]);
+            pf[0][rb][ks] = as_bf16x8(make_uint4(w[0], w[1], w[2], w[3]));
+            if constexpr (PARTS == 2) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = pack_bf16(s[rb][8 * ks + 2 * i] - bf16_lo(w[i]), s[rb][8 * ks + 2 * i + 1] - bf16_hi(w[i]));
+                pf[1][rb][ks] = as_bf16x8(make_uint4(w[0], w[1], w[2], w[3]));
+            }
+        }
     }
 }
 
-template <int RB>
-__device__ __forceinline__ void tile_values(const char* vt, int lane, const bf16x8_t (&pf)[RB][2], TreeState<RB>& st) {
+template <int PARTS, int RB>
+__device__ __forceinline__ void tile_values(const char* vt, int lane, const bf16x8_t (&pf)[PARTS][RB][2], TreeState<RB>& st) {
 #pragma unroll
     for (int mb = 0; mb < 4; ++mb)
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
             const bf16x8_t vf = read_values(vt, lane, mb, ks);
 #pragma unroll
-            for (int rb = 0; rb < RB; ++rb) st.o[rb][mb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[rb][ks], st.o[rb][mb], 0, 0, 0);
+            for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) st.o[rb][mb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[part][rb][ks], st.o[rb][mb], 0, 0, 0);
         }
 }
 
 // In a tile with hidden keys a row must not touch what it does not see: 0 * NaN and 0 * inf are NaN.  There the product is taken of the finite
 // values; whether there were others (a branch of the tree that went wrong) is returned, and add_odd_values deals with them at the end.
-template <int RB>
-__device__ __forceinline__ bool tile_values_masked(const char* vt, int lane, const bf16x8_t (&pf)[RB][2], TreeState<RB>& st) {
+template <int PARTS, int RB>
+__device__ __forceinline__ bool tile_values_masked(const char* vt, int lane, const bf16x8_t (&pf)[PARTS][RB][2], TreeState<RB>& st) {
     bool odd = false;
 #pragma unroll
     for (int mb = 0; mb < 4; ++mb)
@@ -456,7 +472,9 @@ __device__ __forceinline__ bool tile_values_masked(const char* vt, int lane, con
             }
             const bf16x8_t vf = as_bf16x8(make_uint4(w[0], w[1], w[2], w[3]));
 #pragma unroll
-            for (int rb = 0; rb < RB; ++rb) st.o[rb][mb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[rb][ks], st.o[rb][mb], 0, 0, 0);
+            for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) st.o[rb][mb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[part][rb][ks], st.o[rb][mb], 0, 0, 0);
         }
     return __any(odd);
 }
@@ -580,6 +598,7 @@ __device__ __forceinline__ void narrow_run(const TreeParams& p, const TreeItem& 
 
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
     constexpr int SL = tile_slots(RB), kRing = tree_ring(RB);
+    constexpr int kParts = probability_parts(RB, NT);
     char* ring = smem + wave * kRing;
     char* words = smem + kTreeWaves * kRing + wave * kTreeSlotRing;
     const uint32_t ring_at = lds0 + wave * kRing;
@@ -647,23 +666,23 @@ __device__ __forceinline__ void narrow_run(const TreeParams& p, const TreeItem& 
         int j = 0;
         for (; j < plain; ++j) {
             f32x16_t s[RB];
-            bf16x8_t pf[RB][2];
+            bf16x8_t pf[kParts][RB][2];
             keys_of(j, s);
             tile_reference<RB>(p.scale_log2e, s, st);
-            tile_probabilities<RB>(p.scale_log2e, s, st, pf);
-            tile_values<RB>(wait_values(j), lane, pf, st);
+            tile_probabilities(p.scale_log2e, s, st, pf);
+            tile_values(wait_values(j), lane, pf, st);
             if (j + SL < T) issue_rows(j + SL, true);
         }
         for (; j < T; ++j) {
             f32x16_t s[RB];
-            bf16x8_t pf[RB][2];
+            bf16x8_t pf[kParts][RB][2];
             keys_of(j, s);
             uint64_t word[RB];  // (a wave has one such tile as a rule: asked for at the start, its mask would only make that longer)
             load_masks<RB>(p, it, it.r0, lane, word);
             tile_mask<RB>(p, it, it.r0, word, it.t0 + (wave + j * kTreeWaves) * kTreeKeys, lane, s);
             tile_reference<RB>(1.f, s, st);
-            tile_probabilities<RB>(1.f, s, st, pf);
-            if (tile_values_masked<RB>(wait_values(j), lane, pf, st)) odd |= 1ull << (j - plain);
+            tile_probabilities(1.f, s, st, pf);
+            if (tile_values_masked(wait_values(j), lane, pf, st)) odd |= 1ull << (j - plain);
             if (j + SL < T) issue_rows(j + SL, true);
         }
     }
@@ -795,7 +814,7 @@ __device__ __forceinline__ bool wide_run(const TreeParams& p, const TreeItem& it
         // maximum of the new scores.  A step is one basic block (a branch inside would let the compiler sink the exponentials behind it), and
         // four steps are unrolled: a tile's place in a 64 KiB half of the ring is then an immediate of the reads.
         f32x16_t sa[1], sb[1];
-        bf16x8_t kf[8], vf[4][2], pf[1][2];
+        bf16x8_t kf[8], vf[4][2], pf[1][1][2];
         float top[1];
         arrive(0);
         read_keys(tile_at(0), lane, kf);
@@ -836,7 +855,7 @@ __device__ __forceinline__ bool wide_run(const TreeParams& p, const TreeItem& it
                 } else {
                     constexpr int e = k - 8, ks = e / 4, mb = e % 4;
                     if constexpr (e == 0) arrive(j + 2);
-                    st.o[0][mb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[mb][ks], pf[0][ks], st.o[0][mb], 0, 0, 0);
+                    st.o[0][mb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[mb][ks], pf[0][0][ks], st.o[0][mb], 0, 0, 0);
                     kf[e] = __builtin_bit_cast(bf16x8_t, *(const __attribute__((address_space(3))) u32x4_t*)((lds_char*)(uintptr_t)kat[e] + kimm));
                 }
                 // exponential i in slice 11 i / 16
@@ -846,8 +865,8 @@ __device__ __forceinline__ bool wide_run(const TreeParams& p, const TreeItem& it
                     if constexpr (i * 11 / 16 == k - 1) {
                         st.l[0] += s[i];
                         if constexpr (i % 2 == 1) pk[i / 2] = pack_bf16(s[i - 1], s[i]);
-                        if constexpr (i == 7) pf[0][0] = as_bf16x8(make_uint4(pk[0], pk[1], pk[2], pk[3]));
-                        if constexpr (i == 15) pf[0][1] = as_bf16x8(make_uint4(pk[4], pk[5], pk[6], pk[7]));
+                        if constexpr (i == 7) pf[0][0][0] = as_bf16x8(make_uint4(pk[0], pk[1], pk[2], pk[3]));
+                        if constexpr (i == 15) pf[0][0][1] = as_bf16x8(make_uint4(pk[4], pk[5], pk[6], pk[7]));
                     }
                 });
                 if constexpr (k >= 12) {  // (the last S^T instruction lies four matrix instructions back: its result is there)
@@ -887,17 +906,17 @@ __device__ __forceinline__ bool wide_run(const TreeParams& p, const TreeItem& it
         }
         if ((plain - 2 - j) & 1) sa[0] = sb[0];
         j = plain - 2;
-        tile_probabilities<1>(p.scale_log2e, sa, st, pf);
-        tile_values<1>(tile_at(j) + kTreeHalf, lane, pf, st);
+        tile_probabilities(p.scale_log2e, sa, st, pf);
+        tile_values(tile_at(j) + kTreeHalf, lane, pf, st);
         tile_scores<1>(kf, qf, sa);
         tile_reference<1>(p.scale_log2e, sa, st);
-        tile_probabilities<1>(p.scale_log2e, sa, st, pf);
-        tile_values<1>(tile_at(j + 1) + kTreeHalf, lane, pf, st);
+        tile_probabilities(p.scale_log2e, sa, st, pf);
+        tile_values(tile_at(j + 1) + kTreeHalf, lane, pf, st);
         j = plain;
     }
     for (; j < T; ++j) {
         f32x16_t s[1];
-        bf16x8_t kf[8], pf[1][2];
+        bf16x8_t kf[8], pf[1][1][2];
         arrive(j);
         refill(j);
         read_keys(tile_at(j), lane, kf);
@@ -905,9 +924,9 @@ __device__ __forceinline__ bool wide_run(const TreeParams& p, const TreeItem& it
         float scale = p.scale_log2e;
         if (j >= plain) tile_mask<1>(p, it, row0, word, it.t0 + j * kTreeKeys, lane, s), scale = 1.f;
         tile_reference<1>(scale, s, st);
-        tile_probabilities<1>(scale, s, st, pf);
-        if (j < plain) tile_values<1>(tile_at(j) + kTreeHalf, lane, pf, st);
-        else if (tile_values_masked<1>(tile_at(j) + kTreeHalf, lane, pf, st)) odd |= 1ull << (j - plain);
+        tile_probabilities(scale, s, st, pf);
+        if (j < plain) tile_values(tile_at(j) + kTreeHalf, lane, pf, st);
+        else if (tile_values_masked(tile_at(j) + kTreeHalf, lane, pf, st)) odd |= 1ull << (j - plain);
     }
     wait_loads<0>();
     const bool wild = tame && plain > 2 && ((fabsf(st.m[0]) > kTameScore && st.m[0] != kLowestScore) || st.l[0] != st.l[0]);

@@ -87,6 +87,20 @@ def test_large_scores_leave_the_largest_and_its_ties(variants, form, shares, nod
         assert bool((err <= tol).all()), scale
 
 
+@pytest.mark.parametrize("nodes,prefix,Hq,Hkv", [([3, 1, 4], [400, 0, 64], 16, 8), ([7, 8, 0], [1333, 31, 5], 8, 2), ([4, 1, 3], [40, 700, 3], 8, 1),
+                                                 ([32, 20], [2000, 0], 4, 4)])
+@pytest.mark.parametrize("shares", [0, 1])
+def test_up_to_32_rows_per_kv_head_the_result_is_rounded_once(variants, shares, nodes, prefix, Hq, Hkv):
+    """As in the decode kernel that such a step stands in for: 2^-8 of the result, for its own rounding, beside errors of 32-bit arithmetic and 2^-16 of
+    sum p |v| for the probabilities in two bf16 parts (each half a step: 2^-8 of what the first leaves)."""
+    variants("tree_shares", shares)
+    c = tc.attention_case(nodes, prefix, Hq, Hkv, 16, 40 + sum(nodes))
+    exact, absv, size = tc.attention_oracle(c)
+    rest = absv * (2 * 129 * 2.0 ** -24 * size.unsqueeze(-1) + 2.0 ** -20 + 2.0 ** -16)
+    err = (_attend(c).cpu().double() - exact).abs()
+    assert bool((err <= 2.0 ** -8 * (exact.abs() + rest) + rest).all()), float((err / (2.0 ** -8 * (exact.abs() + rest) + rest)).max())
+
+
 @pytest.mark.parametrize("form,shares", FORMS)
 @pytest.mark.parametrize("shape", growth.SHAPES)
 def test_scores_that_grow_along_the_context(variants, form, shares, shape):
