@@ -43,32 +43,32 @@ int variant(int which);
 
 static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-// An array argument: `rows` rows of `width` bytes, `stride` bytes apart.
+// An array argument: `rows` rows of `width` bytes, `stride` bytes apart, in [lo, hi).
 struct Span {
     const void* at;
-    uint64_t width, rows = 1, stride = 0;
-    __int128 start() const { return (__int128)reinterpret_cast<uintptr_t>(at); }
-    __int128 end() const { return start() + (__int128)(rows - 1) * stride + width; }
-    bool empty() const { return at == nullptr || width == 0 || rows == 0; }
+    uint64_t width, rows, stride, lo, hi;
+    Span(const void* at_, uint64_t width_, uint64_t rows_ = 1, uint64_t stride_ = 0) : at(at_), width(width_), rows(rows_), stride(stride_) {
+        lo = reinterpret_cast<uintptr_t>(at), hi = 0;
+        if (at == nullptr || width == 0 || rows == 0) lo = ~0ull;  // empty: meets nothing
+        else if (__builtin_mul_overflow(rows - 1, stride, &hi) || __builtin_add_overflow(hi, width, &hi) || __builtin_add_overflow(hi, lo, &hi)) hi = ~0ull;
+    }
 };
 // Whether two of them have a byte in common.  Rows are looked at one by one only where the arrays lie inside one another with strides of their own.
-static inline bool spans_meet(Span a, Span b) {
-    if (a.empty() || b.empty() || a.end() <= b.start() || b.end() <= a.start()) return false;
-    if (a.rows > b.rows) {
-        const Span t = a;
-        a = b, b = t;
-    }
+static inline bool spans_meet(const Span& x, const Span& y) {
+    if (x.hi <= y.lo || y.hi <= x.lo) return false;
+    const Span &a = x.rows > y.rows ? y : x, &b = x.rows > y.rows ? x : y;
+    const __int128 a0 = a.lo, b0 = b.lo;
     // the first of b's rows least .. that ends behind lo, if it begins before hi
-    auto some_row = [&b](__int128 lo, __int128 hi, __int128 least) {
-        const __int128 gap = lo - b.start() - (__int128)b.width;
-        if (b.stride == 0) return gap < 0 && b.start() < hi;
+    auto some_row = [&](__int128 lo, __int128 hi, __int128 least) {
+        const __int128 gap = lo - b0 - b.width;
+        if (b.stride == 0) return gap < 0 && b0 < hi;
         __int128 i = gap < 0 ? -((-gap + b.stride - 1) / b.stride) + 1 : gap / b.stride + 1;
         if (i < least) i = least;
-        return i < (__int128)b.rows && b.start() + i * b.stride < hi;
+        return i < (__int128)b.rows && b0 + i * b.stride < hi;
     };
-    if (a.stride == b.stride) return some_row(a.start(), a.start() + a.width, 1 - (__int128)a.rows);  // only the difference of the rows' numbers counts
+    if (a.stride == b.stride) return some_row(a0, a0 + a.width, 1 - (__int128)a.rows);  // only the difference of the rows' numbers counts
     for (uint64_t r = 0; r < a.rows; ++r) {
-        const __int128 lo = a.start() + (__int128)r * a.stride;
+        const __int128 lo = a0 + (__int128)r * a.stride;
         if (some_row(lo, lo + a.width, 0)) return true;
     }
     return false;

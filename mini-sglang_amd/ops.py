@@ -859,10 +859,13 @@ def accept_tree(draft_tokens: torch.Tensor, target_tokens: torch.Tensor, parents
     most = accept_rows.shape[1]
     lens_at, rows_at, tokens_at, next_at, seq_at = (t.data_ptr() for t in (accept_lens, accept_rows, accept_tokens, next_tokens, seq_lens))
     small, large, length = 4 * bs, 4 * bs * most, 4 * T
-    for at in nodes:  # (the entry point sees where these begin; how long they are is known here)
-        if lens_at - length < at < lens_at + small or next_at - length < at < next_at + small or seq_at - length < at < seq_at + small \
-                or rows_at - length < at < rows_at + large or tokens_at - length < at < tokens_at + large:
-            raise ValueError("an output overwrites an input (only seq_lens may be prefix_lens)")
+    first, end = min(nodes), max(nodes) + length  # (the entry point sees where these begin; how long they are is known here)
+    if lens_at < end and lens_at + small > first or next_at < end and next_at + small > first or seq_at < end and seq_at + small > first \
+            or rows_at < end and rows_at + large > first or tokens_at < end and tokens_at + large > first:
+        for at in nodes:
+            if lens_at - length < at < lens_at + small or next_at - length < at < next_at + small or seq_at - length < at < seq_at + small \
+                    or rows_at - length < at < rows_at + large or tokens_at - length < at < tokens_at + large:
+                raise ValueError("an output overwrites an input (only seq_lens may be prefix_lens)")
     _launch(index, _lib.msgl_accept_tree, *nodes[:3], cu_at, prefix_lens.data_ptr(), nodes[3], table, count, stride, Hkv, D, lens_at, rows_at, tokens_at,
             next_at, seq_at, bs, most)
 
