@@ -2,7 +2,8 @@
 
 A step takes, per request, the tokens a drafter proposes as a tree below the last accepted token, runs the model over all of them at once and
 keeps the longest path the model itself would have produced greedily, plus the token behind it: between one and depth + 1 tokens per request and
-forward, and always the tokens that plain greedy decoding gives.  Everything between the drafts and the accepted tokens happens on the
+forward, those of greedy decoding whatever was drafted.  (Up to the rounding of the logits: plain decoding has products of other shapes and another
+order of sums, and two tokens within that of each other may change places.)  Everything between the drafts and the accepted tokens happens on the
 device (``ops.prepare_extend`` -> model -> ``ops.argmax`` -> ``ops.accept_tree``, with ``ops.token_logprobs`` where they are asked for), in one captured
 hipGraph per decoder.  The reference decodes one token per step (mini_sglang/managers/scheduler.py:409-419) and has no counterpart.
 
