@@ -10,8 +10,8 @@
 // probability, unbiased, where one part holds it, 2^-16 where two do, see probability_parts; the sum is taken of the unrounded ones.)
 //
 // The narrow kernel, for up to 64 rows per kv head and for tiles of 32 rows of small launches: the pass over K and V bounds it (a 32-key tile
-// costs a wave 512 matrix cycles per 32 rows, 768 with probabilities in two parts, where HBM takes 1250 cycles of the compute unit).  The work group's four waves take every fourth 32-key
-// tile each, with RB blocks of 32 rows: tiles are private to a wave, so the loop has no barrier.
+// costs a wave 512 matrix cycles per 32 rows, 768 with probabilities in two parts, where HBM takes 1250 cycles of the compute unit).  The work
+// group's four waves take every fourth 32-key tile each, with RB blocks of 32 rows: tiles are private to a wave, so the loop has no barrier.
 //   * K and V rows go from HBM to LDS without passing registers, 16 bytes a lane, four rows of 256 bytes an instruction; the XOR swizzles that
 //     spread the fragment reads over the banks are applied to the source address.  With one block of rows a wave has room for one tile, and
 //     a second work group fits on the compute unit: its loop runs beside the other's start and end (200 requests of 500 to 1000 tokens
@@ -707,8 +707,8 @@ __global__ __launch_bounds__(kTreeWaves * 64, tile_slots(RB) == 1 ? 2 : 1) void 
 // then the barrier says that everybody's have landed and that everybody is done with tile j - 2, whose slot is filled anew.  Two waves per SIMD either
 // way (NW = 8 and one work group per compute unit, or NW = 4 and two): a wave issues an instruction about every eighth cycle, whatever it is, so one
 // wave cannot keep softmax and matrix products side by side.  Measured: 32 requests of 16000 tokens x 64 nodes, 32 / 8 heads, 550 to 607 us = 980 to
-// 890 TFLOP/s, K and V at 3.8 to 3.5 TB/s beside it (a dense product of 8192^3 reaches 1228 on this chip, whose clock gives way under such load); 40 requests of 4000 to 8000
-// x 30 nodes (four waves) 208 us = 4.8 TB/s, bound by the issue of its one wave per SIMD.
+// 890 TFLOP/s, K and V at 3.8 to 3.5 TB/s beside it (a dense product of 8192^3 reaches 1228 on this chip, whose clock gives way under such load);
+// 40 requests of 4000 to 8000 x 15 to 30 nodes (four waves) 205 us = 4.8 TB/s, bound by the issue of its one wave per SIMD.
 template <int NW>
 struct TreeWide {
     static constexpr int kSlots = NW == 8 ? 8 : 4;
